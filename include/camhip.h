@@ -75,6 +75,31 @@ CAMHIP_API camhipStatus camhipMoeRouteGetWorkspaceSize(const float *logits, cons
 CAMHIP_API camhipStatus camhipMoeRoute(void *workspace, uint64_t workspaceSize, camhipExecutor *executor,
                                        void *stream);
 
+/* Routing over groups of experts (extension; no reference counterpart).
+ * logits [numTokens, numExperts] of logitsDtype (bf16, fp16, fp32), logitsRowStride elements between two tokens;
+ * bias [numExperts] fp32 or NULL.  With s = softmax(logits) or sigmoid(logits) and c = s + bias:
+ * the experts form numGroups groups of numExperts / numGroups consecutive ids; a group's score is its largest c
+ * (CAMHIP_ROUTE_GROUP_MAX) or the sum of its two largest (CAMHIP_ROUTE_GROUP_TOP2; of one, if it has no second); the
+ * topkGroups best groups are kept (ties -> lower group).  topkIdx[t,k]: the k-th largest c within them (ties -> lower
+ * expert id; scores nearer than 2^-43 of their size are ties).  topkWeights[t,k] = s at topkIdx[t,k] (without the bias),
+ * if renormalize over (the sum of the K picks' + 1e-20), times routedScaling.
+ * An expert whose logit or bias is -inf or NaN is not picked (nor counted in the softmax, if its logit is); a group with
+ * none to pick is not kept; slots left without an expert hold id -1 (the calls below skip it) and weight 0.
+ * topkIdxInt64 (optional, may be NULL): the same ids as int64.
+ * Limits: numTokens <= 65536, 1 <= topK <= 16, numExperts <= 512, numGroups <= 64 and a divisor of numExperts,
+ * topK <= topkGroups * numExperts / numGroups. */
+#define CAMHIP_ROUTE_SOFTMAX 0
+#define CAMHIP_ROUTE_SIGMOID 1
+#define CAMHIP_ROUTE_GROUP_MAX 1
+#define CAMHIP_ROUTE_GROUP_TOP2 2
+CAMHIP_API camhipStatus camhipMoeRouteGroupedGetWorkspaceSize(
+    const void *logits, const float *bias, int64_t numTokens, int64_t numExperts, int64_t topK, int64_t logitsDtype,
+    int64_t logitsRowStride, int64_t numGroups, int64_t topkGroups, int64_t scoreFunc, int64_t groupScore,
+    int64_t renormalize, double routedScaling, int32_t *topkIdx, float *topkWeights, int64_t *topkIdxInt64,
+    uint64_t *workspaceSize, camhipExecutor **executor);
+CAMHIP_API camhipStatus camhipMoeRouteGrouped(void *workspace, uint64_t workspaceSize, camhipExecutor *executor,
+                                              void *stream);
+
 /* ------------------------------------------------------------------ layout
  * Replaces aclnnDispatchLayoutGetWorkspaceSize / aclnnDispatchLayout
  * (dispatch_layout/op_api/aclnn_dispatch_layout.h:33-46; kernel
@@ -235,8 +260,10 @@ CAMHIP_API camhipStatus camhipMoeCombineNormalNoAlloc(const uint16_t *recvX, con
  * value = ((float)acc * weightScale[n]) * xScale[m]
  * (block_epilogue_per_token_dequant.hpp:338-361). */
 #define CAMHIP_DTYPE_BF16 0
+#define CAMHIP_DTYPE_FP16 1 /* the operators around the expert layer only */
 #define CAMHIP_DTYPE_INT8 2
 #define CAMHIP_DTYPE_FP8 3
+#define CAMHIP_DTYPE_FP32 4 /* likewise */
 /* OR'ed into camhipFusedDeepMoe's weightDtype: separated weights, the reference's per-expert
  * tensor lists (pybind/fused_deep_moe.cpp:33-36, TensorList gmm1Weight ...; dynamic EPLB,
  * test_fused_deep_moe.py:256-269).  gmm1Weight, gmm1WeightScale, gmm2Weight and
@@ -347,6 +374,42 @@ CAMHIP_API camhipStatus camhipFusedDeepMoeGetWorkspaceSize(
     camhipExecutor **executor);
 CAMHIP_API camhipStatus camhipFusedDeepMoe(void *workspace, uint64_t workspaceSize, camhipExecutor *executor,
                                            void *stream);
+
+/* ------------------------------------------------------------------ residual addition + norm
+ * Extension; no reference counterpart (its layers take normalised rows).  Per row of x [numTokens, hidden] (dtype bf16
+ * or fp16, xRowStride elements between two rows), with residual [numTokens, hidden] of dtype or NULL and weight
+ * [hidden] of dtype or fp32:
+ *   v = x + residual (fp32);  residualOut [numTokens, hidden] = v in dtype (with a residual only; may be the residual
+ *   itself);  y = v / sqrt(mean(v^2) + eps) * weight, v unrounded.
+ * outQuant CAMHIP_QUANT_NONE: y [numTokens, hidden] in dtype.  CAMHIP_QUANT_INT8_TOKEN: y int8 with yScales [numTokens],
+ * code = rint(t * (127 / a)), scale = a / 127 * r, where t = v * weight, a = max |t| over the row (at least 2^-100) and
+ * r the reciprocal root: the rows and scales of camhipQuantMatmul.  CAMHIP_QUANT_FP8_BLOCK_KMAJOR: y fp8 e4m3fn, the same per 1x128
+ * block with 448, yScales k-major [hidden/128, numTokens] (xScaleLayout 1 of the grouped GEMMs).  Values are
+ * code * scale.  A row with an infinity or a NaN has NaN scales.
+ * Limits: hidden in [1,32768] (a multiple of 128 for fp8), eps in [0,1].  Any element alignment is taken; rows that
+ * start on 16 bytes are the fast ones. */
+CAMHIP_API camhipStatus camhipAddRmsNormGetWorkspaceSize(const void *x, const void *residual, const void *weight,
+                                                         int64_t numTokens, int64_t hidden, int64_t xRowStride,
+                                                         int64_t dtype, int64_t weightDtype, int64_t outQuant,
+                                                         double eps, void *y, float *yScales, void *residualOut,
+                                                         uint64_t *workspaceSize, camhipExecutor **executor);
+CAMHIP_API camhipStatus camhipAddRmsNorm(void *workspace, uint64_t workspaceSize, camhipExecutor *executor,
+                                         void *stream);
+
+/* ------------------------------------------------------------------ int8 product
+ * Extension: the dense form of the int8 grouped GEMM (its epilogue's formula, block_epilogue_per_token_dequant.hpp:338-361),
+ * for the projections and dense layers beside the experts.  x [m, k] and weight [n, k] int8 (k contiguous), xScale [m],
+ * weightScale [n], bias [n] fp32 or NULL:
+ *   out[m, n] = ((float)sum_k x[m, k] weight[n, k] * weightScale[n]) * xScale[m] + bias[n]
+ * with the exact int32 sum, rounded once to outDtype (bf16, fp16 or fp32); the result does not hang on how the product
+ * is split.  Limits: m <= 2^20, n <= 2^20, k a multiple of 16 and at most 131056 (the sum then fits 32 bits for all
+ * codes, -128 among them), x and weight 16-byte aligned. */
+CAMHIP_API camhipStatus camhipQuantMatmulGetWorkspaceSize(const void *x, const float *xScale, const void *weight,
+                                                          const float *weightScale, const float *bias, int64_t m,
+                                                          int64_t n, int64_t k, int64_t outDtype, void *out,
+                                                          uint64_t *workspaceSize, camhipExecutor **executor);
+CAMHIP_API camhipStatus camhipQuantMatmul(void *workspace, uint64_t workspaceSize, camhipExecutor *executor,
+                                          void *stream);
 
 #ifdef __cplusplus
 }

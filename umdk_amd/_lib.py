@@ -17,8 +17,9 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int64
 _U64P = ctypes.POINTER(ctypes.c_uint64)
 _EXP = ctypes.POINTER(ctypes.c_void_p)
+_KIND = {"p": _P, "i": _I, "d": ctypes.c_double}
 
-# argument kinds of each *GetWorkspaceSize entry point ('p' pointer, 'i' int64)
+# argument kinds of each *GetWorkspaceSize entry point ('p' pointer, 'i' int64, 'd' double)
 SIGNATURES = {
     "camhipMoeRoute": "pp iii ppp",
     "camhipDispatchLayout": "p iiii pppp",
@@ -31,6 +32,9 @@ SIGNATURES = {
     "camhipMoePrefillDispatch": "ppp iiiiiii pppppppp",
     "camhipMoePrefillCombine": "ppppp iiiii p",
     "camhipMoeExperts": "ppp iiii pppp ii ppp",
+    "camhipMoeRouteGrouped": "pp iiiiiiiiii d ppp",
+    "camhipAddRmsNorm": "ppp iiiiii d ppp",
+    "camhipQuantMatmul": "ppppp iiii p",
 }
 
 _lib = None
@@ -56,7 +60,7 @@ def lib():
             kinds = sig.replace(" ", "")
             f = getattr(L, name + "GetWorkspaceSize")
             f.restype = ctypes.c_int
-            f.argtypes = [(_P if k == "p" else _I) for k in kinds] + [_U64P, _EXP]
+            f.argtypes = [_KIND[k] for k in kinds] + [_U64P, _EXP]
             g = getattr(L, name)
             g.restype = ctypes.c_int
             g.argtypes = [_P, ctypes.c_uint64, _P, _P]

@@ -23,6 +23,53 @@ hipError_t launch_route_hist(const float *logits, const float *bias, int T, int 
                              float *topk_w, int32_t *chunk_counts, int32_t *chunk_pref, int32_t *chunk_rank,
                              hipStream_t s);
 
+// ---- routing over groups of experts (route_grouped.hip)
+enum RouteScore { ROUTE_SOFTMAX = 0, ROUTE_SIGMOID = 1 };
+enum RouteDtype { ROUTE_BF16 = 0, ROUTE_FP16 = 1, ROUTE_FP32 = 4 };  // the CAMHIP_DTYPE_* codes
+struct RouteGroupedArgs {
+    const void *logits;
+    int64_t row_bytes;  // between two tokens' logits
+    const float *bias;  // or nullptr
+    int T, E, K, G, KG;
+    int score, group_top2, renorm, dtype;
+    float scaling;
+    int32_t *topk_idx;
+    float *topk_w;
+    int64_t *topk_idx64;  // or nullptr
+    // set by the launcher: experts per group, lanes per group, whether the keys are the logits
+    int gs, lpg, by_logit;
+};
+hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s);
+
+// ---- residual addition + root-mean-square norm (+ quantisation) (norm.hip)
+struct NormArgs {
+    const uint16_t *x;
+    int64_t x_stride;          // elements between two rows of x
+    const uint16_t *residual;  // or nullptr; rows of H
+    const void *weight;        // [H], x's type or fp32 (weight_fp32)
+    int64_t T;
+    int H;
+    float eps;
+    int fp16, weight_fp32, quant;  // quant: QUANT_NONE, QUANT_INT8_TOKEN, QUANT_FP8_BLOCK (k-major scales)
+    void *y;                       // [T, H]
+    float *scales;                 // [T] (int8), [H/128, T] (fp8)
+    uint16_t *residual_out;        // [T, H], with a residual only
+};
+hipError_t launch_add_rms_norm(const NormArgs &a, hipStream_t s);
+
+// ---- int8 matrix product (qmm.hip)
+enum QmmOut { QMM_BF16 = 0, QMM_FP16 = 1, QMM_FP32 = 4 };  // the CAMHIP_DTYPE_* codes
+struct QmmArgs {
+    const int8_t *x, *w;     // [M, K], [N, K]
+    const float *xs, *ws;    // [M], [N]
+    const float *bias;       // [N] or nullptr
+    int64_t M;
+    int N, K, out_dtype;
+    void *out;               // [M, N]
+};
+size_t qmm_workspace_bytes(int64_t M, int N, int K);
+hipError_t launch_quant_matmul(const QmmArgs &a, void *ws, hipStream_t s);
+
 // ---- dispatch layout (layout.hip)
 struct LayoutPlan {
     int tokens_per_chunk;

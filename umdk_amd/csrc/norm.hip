@@ -1,0 +1,278 @@
+// N1: residual addition, root-mean-square norm and the quantisation of its rows, in one pass.  Per row of H columns
+//   v = x + residual (fp32);  residual_out = v in x's type
+//   r = 1 / sqrt(mean(v^2) + eps);  y = v * r * w
+// rows in x's type, in int8 with one scale per row, or in fp8 e4m3 with one scale per 128 columns:
+//   int8: t = v * w, a = max |t|, code = rint(t * (127 / a)), scale = a / 127 * r
+//   fp8:  per block of 128 columns code = e4m3(t * (448 / a)), scale = a / 448 * r
+// r cancels out of the codes, so they hang on a sum, a product, a maximum and a division of fp32 and not on the order in
+// which the squares are added up, and need not wait for that sum.  (a is taken as at least 2^-100: 127 / a stays finite,
+// and a row of zeros gives codes 0 and scale 2^-100 / 127 * r.)  A row that holds an infinity or a NaN has NaN scales.
+//
+// The norm reads v before it is rounded to 16 bits (the stored residual stream is the rounded one): one rounding per
+// output.
+#include "cam_device.h"
+#include "launchers.h"
+
+namespace cam {
+
+namespace {
+
+constexpr float NORM_TINY = 0x1p-100f;
+
+// 8 elements from p (aligned for its type only: global memory takes unaligned 16-byte accesses)
+__device__ __forceinline__ u32x4 load16(const void *p)
+{
+    u32x4 v;
+    __builtin_memcpy(&v, p, 16);
+    return v;
+}
+template <bool FP16> __device__ __forceinline__ float unpack1(uint32_t h)
+{
+    return FP16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)h) : bf16_to_f32(h);
+}
+template <bool FP16> __device__ __forceinline__ void unpack8(const u32x4 v, float *f)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = unpack1<FP16>(v[i] & 0xffffu);
+        f[2 * i + 1] = unpack1<FP16>(v[i] >> 16);
+    }
+}
+typedef _Float16 cam_f16x2 __attribute__((ext_vector_type(2)));
+template <bool FP16> __device__ __forceinline__ uint32_t pack2(float a, float b)
+{
+    if constexpr (FP16)
+        return __builtin_bit_cast(uint32_t, cam_f16x2{(_Float16)a, (_Float16)b});
+    else
+        return f32x2_to_bf16x2(a, b);
+}
+template <bool FP16> __device__ __forceinline__ u32x4 pack8(const float *f)
+{
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = pack2<FP16>(f[2 * i], f[2 * i + 1]);
+    return r;
+}
+// the first n (1..8) of 8 packed 16-bit elements
+__device__ __forceinline__ void store16(void *p, const u32x4 v, int n)
+{
+    if (n >= 8) {
+        __builtin_memcpy(p, &v, 16);
+        return;
+    }
+    uint16_t *q = reinterpret_cast<uint16_t *>(p);
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n)
+            q[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+}
+__device__ __forceinline__ u32x4 load16_n(const void *p, int n)
+{
+    if (n >= 8)
+        return load16(p);
+    const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
+    u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n)
+            v[i >> 1] |= (uint32_t)q[i] << (16 * (i & 1));
+    return v;
+}
+
+__device__ __forceinline__ float wave_sum(float v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+__device__ __forceinline__ uint32_t int8x4(const float *t, float inv)
+{
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r |= ((uint32_t)(int)__builtin_rintf(t[i] * inv) & 0xffu) << (8 * i);
+    return r;
+}
+
+// One row per ROW_WAVES waves, ROWS rows per block; a thread holds NIT pieces of 8 columns, 8 ROW_THREADS apart.
+template <bool FP16, int QUANT, int NIT, int ROW_WAVES, int ROWS>
+__global__ __launch_bounds__(64 * ROW_WAVES *ROWS) void add_rms_norm_kernel(const NormArgs p)
+{
+#pragma clang fp contract(off)
+    constexpr int RT = 64 * ROW_WAVES;
+    static_assert(ROWS == 1 || ROW_WAVES == 1, "a block holds one row, or a row per wave");
+    const int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? (int)(threadIdx.x >> 6) : 0);
+    if (ROWS > 1 && row >= p.T)
+        return;
+    const int tid = ROWS > 1 ? threadIdx.x & 63 : threadIdx.x;
+    const uint16_t *x = p.x + row * p.x_stride;
+    const uint16_t *res = p.residual ? p.residual + row * p.H : nullptr;
+
+    u32x4 xv[NIT], rv[NIT];
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+        const int col = (i * RT + tid) * 8;
+        xv[i] = col < p.H ? load16_n(x + col, p.H - col) : u32x4{0, 0, 0, 0};
+    }
+    if (res) {
+#pragma unroll
+        for (int i = 0; i < NIT; ++i) {
+            const int col = (i * RT + tid) * 8;
+            rv[i] = col < p.H ? load16_n(res + col, p.H - col) : u32x4{0, 0, 0, 0};
+        }
+    }
+    float t[NIT][8];
+    float ss = 0.0f, am = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+        const int col = (i * RT + tid) * 8, n = p.H - col;
+        unpack8<FP16>(xv[i], t[i]);
+        if (res) {
+            float r[8];
+            unpack8<FP16>(rv[i], r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                t[i][j] += r[j];
+            if (n > 0)
+                store16(p.residual_out + row * p.H + col, pack8<FP16>(t[i]), n);
+        }
+        float s8 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            s8 += t[i][j] * t[i][j];
+        ss += s8;
+        float w[8] = {};
+        if (n > 0) {
+            if (p.weight_fp32) {
+                const float *wp = reinterpret_cast<const float *>(p.weight) + col;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    w[j] = j < n ? wp[j] : 0.0f;
+            } else {
+                unpack8<FP16>(load16_n(reinterpret_cast<const uint16_t *>(p.weight) + col, n), w);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            t[i][j] *= w[j];
+        if constexpr (QUANT == QUANT_INT8_TOKEN) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                am = fmaxf(am, fabsf(t[i][j]));
+        }
+    }
+    ss = wave_sum(ss);
+    if constexpr (QUANT == QUANT_INT8_TOKEN)
+        am = group_max<64>(am);
+    if constexpr (ROW_WAVES > 1) {
+        __shared__ float red[2][ROW_WAVES];
+        if ((tid & 63) == 0) {
+            red[0][tid >> 6] = ss;
+            red[1][tid >> 6] = am;
+        }
+        __syncthreads();
+        ss = 0.0f;
+        am = 0.0f;
+#pragma unroll
+        for (int w = 0; w < ROW_WAVES; ++w) {
+            ss += red[0][w];
+            am = fmaxf(am, red[1][w]);
+        }
+    }
+    const float rms = 1.0f / __builtin_sqrtf(ss / (float)p.H + p.eps);
+
+    if constexpr (QUANT == QUANT_NONE) {
+        uint16_t *y = reinterpret_cast<uint16_t *>(p.y) + row * p.H;
+#pragma unroll
+        for (int i = 0; i < NIT; ++i) {
+            const int col = (i * RT + tid) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                t[i][j] *= rms;
+            if (col < p.H)
+                store16(y + col, pack8<FP16>(t[i]), p.H - col);
+        }
+    } else if constexpr (QUANT == QUANT_INT8_TOKEN) {
+        int8_t *y = reinterpret_cast<int8_t *>(p.y) + row * p.H;
+        const float a = fmaxf(am, NORM_TINY), inv = 127.0f / a;
+#pragma unroll
+        for (int i = 0; i < NIT; ++i) {
+            const int col = (i * RT + tid) * 8, n = p.H - col;
+            const u32x2 v = {int8x4(t[i], inv), int8x4(t[i] + 4, inv)};
+            if (n >= 8) {
+                __builtin_memcpy(y + col, &v, 8);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 7; ++j)
+                    if (j < n)
+                        y[col + j] = (int8_t)(v[j >> 2] >> (8 * (j & 3)));
+            }
+        }
+        if (tid == 0)
+            p.scales[row] = a / 127.0f * rms;
+    } else {
+        uint8_t *y = reinterpret_cast<uint8_t *>(p.y) + row * p.H;
+#pragma unroll
+        for (int i = 0; i < NIT; ++i) {
+            const int col = (i * RT + tid) * 8;  // H % 128 == 0: 16 lanes hold a block, whole or not at all
+            float a = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                a = fmaxf(a, fabsf(t[i][j]));
+            a = fmaxf(group_max<16>(a), NORM_TINY);
+            const float inv = 448.0f / a;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                t[i][j] *= inv;
+            if (col < p.H) {
+                const u32x2 v = {f32x4_to_e4m3(t[i][0], t[i][1], t[i][2], t[i][3]),
+                                 f32x4_to_e4m3(t[i][4], t[i][5], t[i][6], t[i][7])};
+                __builtin_memcpy(y + col, &v, 8);
+                if ((tid & 15) == 0)
+                    p.scales[(int64_t)(col / 128) * p.T + row] = a / 448.0f * rms;
+            }
+        }
+    }
+}
+
+template <bool FP16, int QUANT> hipError_t launch_quant(const NormArgs &a, hipStream_t s)
+{
+#define NORM_CASE(NIT, RW, ROWS)                                                                                    \
+    if (a.H <= NIT * 512 * RW) {                                                                                    \
+        const int64_t grid = (a.T + ROWS - 1) / ROWS;                                                               \
+        hipLaunchKernelGGL((add_rms_norm_kernel<FP16, QUANT, NIT, RW, ROWS>), dim3((uint32_t)grid),                 \
+                           dim3(64 * RW * ROWS), 0, s, a);                                                          \
+        return hipGetLastError();                                                                                   \
+    }
+    NORM_CASE(1, 1, 4)
+    NORM_CASE(2, 1, 4)
+    NORM_CASE(1, 4, 1)
+    NORM_CASE(2, 4, 1)
+    NORM_CASE(2, 8, 1)
+    NORM_CASE(2, 16, 1)
+    NORM_CASE(4, 16, 1)
+#undef NORM_CASE
+    return hipErrorInvalidValue;
+}
+
+}  // namespace
+
+hipError_t launch_add_rms_norm(const NormArgs &a, hipStream_t s)
+{
+    if (a.T == 0)
+        return hipSuccess;
+    if (a.H < 1 || a.T < 0 || a.T > 0x7fffffff || (a.quant == QUANT_FP8_BLOCK && a.H % 128))
+        return hipErrorInvalidValue;
+    if (a.quant == QUANT_NONE)
+        return a.fp16 ? launch_quant<true, QUANT_NONE>(a, s) : launch_quant<false, QUANT_NONE>(a, s);
+    if (a.quant == QUANT_INT8_TOKEN)
+        return a.fp16 ? launch_quant<true, QUANT_INT8_TOKEN>(a, s) : launch_quant<false, QUANT_INT8_TOKEN>(a, s);
+    if (a.quant == QUANT_FP8_BLOCK)
+        return a.fp16 ? launch_quant<true, QUANT_FP8_BLOCK>(a, s) : launch_quant<false, QUANT_FP8_BLOCK>(a, s);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace cam

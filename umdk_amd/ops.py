@@ -16,7 +16,8 @@ Differences, all documented in the op docstrings:
     follow use_quant as the reference does: 2 if use_quant else 0); 3 selects
     FP8 e4m3fn rows with [rows, hidden/128] fp32 block scales.
   * moe_route (routing) and grouped expert GEMM ops are additions with no
-    reference counterpart.
+    reference counterpart, and so are the operators around the expert layer:
+    moe_route_grouped, add_rms_norm and quant_matmul.
 """
 import weakref
 
@@ -40,6 +41,14 @@ _def.define("grouped_matmul_swiglu(Tensor x, Tensor? x_scale, Tensor group_list,
             "Tensor? weight_scale, int out_quant=0) -> (Tensor, Tensor)")
 _def.define("grouped_matmul(Tensor x, Tensor? x_scale, Tensor group_list, Tensor weight, Tensor? weight_scale) "
             "-> Tensor")
+
+_def.define("moe_route_grouped(Tensor logits, Tensor? bias, int topk, int n_group=1, int topk_group=1, "
+            "str score_func='softmax', str group_score='top2', bool renormalize=True, float routed_scaling=1.0) "
+            "-> (Tensor, Tensor)")
+_def.define("add_rms_norm(Tensor x, Tensor? residual, Tensor weight, float eps=1e-6, int out_quant=0) "
+            "-> (Tensor, Tensor, Tensor)")
+_def.define("quant_matmul(Tensor x, Tensor x_scale, Tensor weight, Tensor weight_scale, Tensor? bias=None, "
+            "ScalarType? out_dtype=None) -> Tensor")
 
 _def.define(
     "fused_deep_moe(Tensor x, Tensor expert_ids, Tensor[] gmm1_weight, Tensor[] gmm1_weight_scale, "
@@ -277,6 +286,180 @@ def grouped_matmul(x, x_scale, group_list, weight, weight_scale):
               _lib.ptr(weight), _lib.ptr(weight_scale), dt, _x_scale_layout(x_scale), _lib.ptr(out),
               device=x.device)
     return out
+
+
+_DTYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 4}  # CAMHIP_DTYPE_*
+_SCORE = {"softmax": 0, "sigmoid": 1}
+_GROUP_SCORE = {"max": 1, "top2": 2}
+
+
+def _inputs(op, first, *others):
+    """What the operators around the expert layer ask of their tensors: one GPU, and no gradient (they have no
+    backward)."""
+    dev = first.device
+    grad = torch.is_grad_enabled()
+    for t in (first,) + others:
+        if t is None:
+            continue
+        if t.device != dev:
+            raise RuntimeError(f"{op}: all tensors must be on one device (got {dev} and {t.device})")
+        if grad and t.requires_grad:
+            raise RuntimeError(f"{op}: no backward; call it under torch.no_grad() or detach its inputs")
+    if dev.type != "cuda":
+        raise _lib.CamHipError(f"{op} runs on the GPU only; got a tensor on {dev}")
+    return dev
+
+
+def _run(name, dev, *args):
+    """One entry point on the current stream of `dev`, which need not be the current device."""
+    if dev.index == torch.cuda.current_device():
+        _lib.call(name, *args, device=dev)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, device=dev)
+
+
+def _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score):
+    op = "moe_route_grouped"
+    _check(logits.dim() == 2 and logits.dtype in _DTYPE, f"{op}: logits must be [T,E] float32, bfloat16 or float16")
+    _check(score_func in _SCORE, f"{op}: score_func must be 'softmax' or 'sigmoid' (got {score_func!r})")
+    _check(group_score in _GROUP_SCORE, f"{op}: group_score must be 'max' or 'top2' (got {group_score!r})")
+    E = logits.shape[1]
+    if bias is not None:
+        _check(bias.dtype == torch.float32 and tuple(bias.shape) == (E,), f"{op}: bias must be [E] float32")
+    _check(E > 0, f"{op}: no experts")
+    return E
+
+
+def moe_route_grouped(logits, bias, topk, n_group=1, topk_group=1, score_func="softmax", group_score="top2",
+                      renormalize=True, routed_scaling=1.0):
+    """Top-K routing over groups of experts (addition; no reference
+    counterpart): returns (topk_idx [T,K] int32, topk_weights [T,K] fp32), the
+    inputs of get_dispatch_layout, moe_dispatch_prefill and fused_deep_moe.
+
+    s = softmax or sigmoid of the logits; the choice goes by c = s + bias: of
+    n_group groups of consecutive experts the topk_group with the best group
+    score ("top2": the sum of the two largest c, "max": the largest) are kept,
+    and the topk largest c in them picked, ties to the lower id.  The weights
+    are s at the picks, over their sum (+ 1e-20) if renormalize, times
+    routed_scaling.  Experts whose logit or bias is -inf (or NaN) are never
+    picked; slots left without an expert hold id -1 and weight 0.  logits:
+    float32, bfloat16 or float16, rows of any stride."""
+    E = _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
+    dev = _inputs("moe_route_grouped", logits, bias)
+    T = logits.shape[0]
+    lg = logits if logits.stride(1) == 1 and (T < 2 or logits.stride(0) >= E) else logits.contiguous()
+    b = None if bias is None else bias.contiguous()
+    idx = torch.empty((T, topk), dtype=torch.int32, device=dev)
+    w = torch.empty((T, topk), dtype=torch.float32, device=dev)
+    _run("camhipMoeRouteGrouped", dev, lg.data_ptr(), None if b is None else b.data_ptr(), T, E, topk, _DTYPE[lg.dtype],
+         lg.stride(0) if T > 1 else E, n_group, topk_group, _SCORE[score_func], _GROUP_SCORE[group_score],
+         1 if renormalize else 0, routed_scaling, idx.data_ptr(), w.data_ptr(), None)
+    return idx, w
+
+
+def _norm_check(x, residual, weight, out_quant):
+    op = "add_rms_norm"
+    _check(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float16),
+           f"{op}: x must be [tokens, hidden] bfloat16 or float16")
+    _check(weight.dtype in (x.dtype, torch.float32) and tuple(weight.shape) == (x.shape[1],),
+           f"{op}: weight must be [hidden] of x's dtype or float32")
+    if residual is not None:
+        _check(residual.dtype == x.dtype and residual.shape == x.shape,
+               f"{op}: residual must have x's shape and dtype")
+    _check(out_quant in (QUANT_NONE, QUANT_INT8_TOKEN, QUANT_FP8_BLOCK), f"{op}: out_quant must be 0, 2 or 3")
+    _check(x.shape[1] > 0, f"{op}: no columns")
+    _check(out_quant != QUANT_FP8_BLOCK or x.shape[1] % 128 == 0, f"{op}: fp8 rows need hidden % 128 == 0")
+
+
+def _norm_outputs(x, residual, out_quant):
+    T, H = x.shape
+    dev = x.device
+    new = torch.empty((T, H) if residual is not None else (0,), dtype=x.dtype, device=dev)
+    if out_quant == QUANT_NONE:
+        return torch.empty((T, H), dtype=x.dtype, device=dev), torch.empty(0, dtype=torch.float32, device=dev), new
+    if out_quant == QUANT_INT8_TOKEN:
+        return (torch.empty((T, H), dtype=torch.int8, device=dev), torch.empty(T, dtype=torch.float32, device=dev),
+                new)
+    return (torch.empty((T, H), dtype=torch.float8_e4m3fn, device=dev),
+            torch.empty((H // 128, T), dtype=torch.float32, device=dev).t(), new)
+
+
+def add_rms_norm(x, residual, weight, eps=1e-6, out_quant=0):
+    """The residual's addition and the root-mean-square norm (addition; no
+    reference counterpart): returns (y, y_scale, residual_out).
+
+    v = x + residual in fp32 (v = x without one); residual_out = v in x's
+    dtype (empty without a residual); y = v / sqrt(mean(v^2) + eps) * weight.
+    out_quant 0: y in x's dtype, y_scale empty.  2: int8 y with y_scale
+    [tokens], the rows of quant_matmul and of the int8 grouped GEMMs.  3: fp8
+    e4m3 y with y_scale [tokens, hidden/128], the transpose of k-major storage
+    as grouped_matmul_swiglu reads it.  x may be a column slice of a wider
+    tensor (rows of any stride)."""
+    _norm_check(x, residual, weight, out_quant)
+    dev = _inputs("add_rms_norm", x, residual, weight)
+    T, H = x.shape
+    xc = x if x.stride(1) == 1 and (T < 2 or x.stride(0) >= H) else x.contiguous()
+    r = None if residual is None else residual.contiguous()
+    w = weight.contiguous()
+    y, scale, new = _norm_outputs(x, residual, out_quant)
+    _run("camhipAddRmsNorm", dev, xc.data_ptr(), None if r is None else r.data_ptr(), w.data_ptr(), T, H,
+         xc.stride(0) if T > 1 else H, _DTYPE[x.dtype], _DTYPE[w.dtype],
+         QUANT_FP8_BLOCK_KMAJOR if out_quant == QUANT_FP8_BLOCK else out_quant, eps, y.data_ptr(), scale.data_ptr(),
+         new.data_ptr())
+    return y, scale, new
+
+
+def _quant_matmul_check(x, x_scale, weight, weight_scale, bias, out_dtype):
+    op = "quant_matmul"
+    _check(x.dim() == 2 and x.dtype == torch.int8 and x.is_contiguous(), f"{op}: x must be [m, k] int8, contiguous")
+    _check(weight.dim() == 2 and weight.dtype == torch.int8 and weight.is_contiguous(),
+           f"{op}: weight must be [n, k] int8, contiguous")
+    (m, k), n = x.shape, weight.shape[0]
+    _check(weight.shape[1] == k, f"{op}: x has {k} columns, weight k = {weight.shape[1]}")
+    _check(x_scale.dtype == torch.float32 and tuple(x_scale.shape) == (m,) and x_scale.is_contiguous(),
+           f"{op}: x_scale must be float32 [m] (per token)")
+    _check(weight_scale.dtype == torch.float32 and tuple(weight_scale.shape) == (n,) and weight_scale.is_contiguous(),
+           f"{op}: weight_scale must be float32 [n] (per channel)")
+    if bias is not None:
+        _check(bias.dtype == torch.float32 and tuple(bias.shape) == (n,) and bias.is_contiguous(),
+               f"{op}: bias must be float32 [n]")
+    _check(out_dtype in _DTYPE, f"{op}: out_dtype must be bfloat16, float16 or float32")
+    return m, n, k
+
+
+def quant_matmul(x, x_scale, weight, weight_scale, bias=None, out_dtype=None):
+    """int8 product with a scale for each token and each channel (addition: the
+    dense form of the int8 grouped_matmul): out[m, n] =
+    ((float)(x W^T) * weight_scale[n]) * x_scale[m] (+ bias[n]), the sum exact
+    in int32, rounded once to out_dtype (bfloat16 by default, float16,
+    float32).  x [m, k] int8 and x_scale [m] as add_rms_norm(out_quant=2) gives
+    them, weight [n, k] int8, k a multiple of 16."""
+    out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+    m, n, k = _quant_matmul_check(x, x_scale, weight, weight_scale, bias, out_dtype)
+    dev = _inputs("quant_matmul", x, x_scale, weight, weight_scale, bias)
+    out = torch.empty((m, n), dtype=out_dtype, device=dev)
+    _run("camhipQuantMatmul", dev, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
+         None if bias is None else bias.data_ptr(), m, n, k, _DTYPE[out_dtype], out.data_ptr())
+    return out
+
+
+def moe_route_grouped_meta(logits, bias, topk, n_group=1, topk_group=1, score_func="softmax", group_score="top2",
+                           renormalize=True, routed_scaling=1.0):
+    _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
+    T = logits.shape[0]
+    return (logits.new_empty((T, topk), dtype=torch.int32), logits.new_empty((T, topk), dtype=torch.float32))
+
+
+def add_rms_norm_meta(x, residual, weight, eps=1e-6, out_quant=0):
+    _norm_check(x, residual, weight, out_quant)
+    return _norm_outputs(x, residual, out_quant)
+
+
+def quant_matmul_meta(x, x_scale, weight, weight_scale, bias=None, out_dtype=None):
+    out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+    m, n, _ = _quant_matmul_check(x, x_scale, weight, weight_scale, bias, out_dtype)
+    return x.new_empty((m, n), dtype=out_dtype)
 
 
 def prepack_weight(w_lkn):
@@ -555,3 +738,9 @@ _impl.impl("get_dispatch_layout", get_dispatch_layout)
 _impl.impl("moe_dispatch_prefill", moe_dispatch_prefill)
 _impl.impl("moe_combine_prefill", moe_combine_prefill)
 _impl.impl("moe_route", moe_route)
+_impl.impl("moe_route_grouped", moe_route_grouped)
+_impl.impl("add_rms_norm", add_rms_norm)
+_impl.impl("quant_matmul", quant_matmul)
+_meta.impl("moe_route_grouped", moe_route_grouped_meta)
+_meta.impl("add_rms_norm", add_rms_norm_meta)
+_meta.impl("quant_matmul", quant_matmul_meta)

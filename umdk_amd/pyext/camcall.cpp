@@ -5,7 +5,8 @@
 // chain at T = 1021: 90 and 75 us).
 //
 // name(alloc, workspace, workspace_bytes, stream, *args) -> buffer or None
-//   args: the GetWorkspaceSize arguments (pointers as int or None, sizes as any integer), without the two outputs;
+//   args: the GetWorkspaceSize arguments (pointers as int or None, sizes as any integer, doubles as any number), without
+//   the two outputs;
 //   alloc: called with the workspace size when it is not 0, returns a tensor (its data_ptr is used and the tensor is
 //          returned); None: the caller's workspace is used;
 //   a failed call raises bind's exception with the library's message.
@@ -39,6 +40,8 @@ template <typename A> bool convert(PyObject *o, A &out)
             return false;
         }
         out = (A)PyLong_AsVoidPtr(o);
+    } else if constexpr (std::is_floating_point_v<A>) {
+        out = (A)PyFloat_AsDouble(o);
     } else {
         // any integer type, numpy's among them, through __index__ (a float has none: TypeError); taken modulo 2^64
         out = (A)PyLong_AsUnsignedLongLongMask(o);
@@ -125,7 +128,10 @@ PyObject *entry(const char *name, camhipStatus (*get)(P...), RunFn run, PyObject
     X(camhipFusedDeepMoe)                                                                                            \
     X(camhipMoePrefillDispatch)                                                                                      \
     X(camhipMoePrefillCombine)                                                                                       \
-    X(camhipMoeExperts)
+    X(camhipMoeExperts)                                                                                              \
+    X(camhipMoeRouteGrouped)                                                                                         \
+    X(camhipAddRmsNorm)                                                                                              \
+    X(camhipQuantMatmul)
 
 #define DEFINE(f)                                                                                                    \
     decltype(&f##GetWorkspaceSize) get_##f = nullptr;                                                                \
