@@ -232,8 +232,7 @@ camhipStatus camhipQuantMatmulGetWorkspaceSize(const void *x, const float *xScal
     a.out = out;
     return guarded(op, [&] {
         return cam::api_make_executor(
-            cam::qmm_workspace_bytes(a.M, a.N, a.K),
-            [a](void *w, hipStream_t s) { return cam::launch_quant_matmul(a, w, s); }, workspaceSize, executor);
+            0, [a](void *, hipStream_t s) { return cam::launch_quant_matmul(a, s); }, workspaceSize, executor);
     });
 }
 

@@ -67,8 +67,7 @@ struct QmmArgs {
     int N, K, out_dtype;
     void *out;               // [M, N]
 };
-size_t qmm_workspace_bytes(int64_t M, int N, int K);
-hipError_t launch_quant_matmul(const QmmArgs &a, void *ws, hipStream_t s);
+hipError_t launch_quant_matmul(const QmmArgs &a, hipStream_t s);
 
 // ---- dispatch layout (layout.hip)
 struct LayoutPlan {
