@@ -36,8 +36,8 @@ struct RouteGroupedArgs {
     int32_t *topk_idx;
     float *topk_w;
     int64_t *topk_idx64;  // or nullptr
-    // set by the launcher: experts per group, lanes per group, whether the keys are the logits
-    int gs, lpg, by_logit;
+    // set by the launcher: experts per group, lanes per group, whether the keys are the logits, vector loads
+    int gs, lpg, by_logit, vec;
 };
 hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s);
 

@@ -81,70 +81,126 @@ template <int STEP> __device__ __forceinline__ void top2_step(double &m1, double
     m1 = fmax(m1, o1);
 }
 
-// exp(x) in 64 bits for x in [-745, 700]: x = n ln 2 + r, |r| <= ln 2 / 2, the Taylor sum of exp(r) to r^12 / 12!
-// (what is left out is below 2e-16 of it).
-__device__ __forceinline__ double exp64(double x)
-{
-    const double n = __builtin_rint(x * 1.4426950408889634074);
-    double r = __builtin_fma(n, -0x1.62e42fefa39efp-1, x);
-    r = __builtin_fma(n, -0x1.abc9e3b39803fp-56, r);
-    double p = 1.0 / 479001600.0;
-    p = __builtin_fma(p, r, 1.0 / 39916800.0);
-    p = __builtin_fma(p, r, 1.0 / 3628800.0);
-    p = __builtin_fma(p, r, 1.0 / 362880.0);
-    p = __builtin_fma(p, r, 1.0 / 40320.0);
-    p = __builtin_fma(p, r, 1.0 / 5040.0);
-    p = __builtin_fma(p, r, 1.0 / 720.0);
-    p = __builtin_fma(p, r, 1.0 / 120.0);
-    p = __builtin_fma(p, r, 1.0 / 24.0);
-    p = __builtin_fma(p, r, 1.0 / 6.0);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return __builtin_ldexp(p, (int)n);
-}
-// 1 / d for d in [1, 1e304]: the hardware's estimate and two Newton steps
+// exp(x) in 64 bits for x in [-745, 700]: x = n ln 2 + r, |r| <= ln 2 / 2, and the polynomial of degree 9 that meets
+// exp(r) in the ten Chebyshev nodes of that interval: within 1.9e-14 of it, below the 2^-43 that count as equal.  The
+// coefficients sit in scalar registers (as literals each costs two moves to the FMA that uses it).
+struct Exp64 {
+    double c[10], log2e, ln2_hi, ln2_lo;
+    __device__ __forceinline__ Exp64()
+        : c{0x1.000000000003dp+0,  0x1.0000000000006p+0,  0x1.ffffffffe74f0p-2,  0x1.5555555550d87p-3,  0x1.55555588b8538p-5,
+            0x1.11111123bf1c5p-7, 0x1.6c162bb7b3ef5p-10, 0x1.a01994c82e1c6p-13, 0x1.a17df105a3981p-16, 0x1.72e107e8d8eb6p-19},
+          log2e(0x1.71547652b82fep+0), ln2_hi(-0x1.62e42fefa39efp-1), ln2_lo(-0x1.abc9e3b39803fp-56)
+    {
+#pragma unroll
+        for (int i = 0; i < 10; ++i)
+            asm("" : "+s"(c[i]));
+        asm("" : "+s"(log2e));
+        asm("" : "+s"(ln2_hi));
+        asm("" : "+s"(ln2_lo));
+    }
+    __device__ __forceinline__ double operator()(double x) const
+    {
+        const double n = __builtin_rint(x * log2e);
+        double r = __builtin_fma(n, ln2_hi, x);
+        r = __builtin_fma(n, ln2_lo, r);
+        double p = __builtin_fma(c[9], r, c[8]);
+#pragma unroll
+        for (int i = 7; i >= 0; --i)
+            p = __builtin_fma(p, r, c[i]);
+        return __builtin_ldexp(p, (int)n);
+    }
+};
+// 1 / d for d in [1, 1e304]: the hardware's estimate (of single precision) and one step of third order
 __device__ __forceinline__ double recip64(double d)
 {
-    double y = __builtin_amdgcn_rcp(d);
-    y = __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
-    return __builtin_fma(__builtin_fma(-d, y, 1.0), y, y);
+    const double y = __builtin_amdgcn_rcp(d), e = __builtin_fma(-d, y, 1.0);
+    return __builtin_fma(y, __builtin_fma(e, e, e), y);
 }
-__device__ __forceinline__ double sigmoid64(float l)
+// (exp of less than -745 would be 0: nothing beside 1; a NaN gives some number, its expert is not eligible)
+__device__ __forceinline__ double sigmoid64(const Exp64 &exp64, float l)
 {
-    return recip64(1.0 + exp64(fmin(-(double)l, 700.0)));  // (exp64 of less than -745 would be 0: nothing beside 1)
+    return recip64(1.0 + exp64((double)fmaxf(fminf(-l, 700.0f), -745.0f)));
 }
 // exp(l - mx), 0 for an expert that has no logit (-inf or NaN)
-__device__ __forceinline__ double exp_rel(float l, float mx)
+__device__ __forceinline__ double exp_rel(const Exp64 &exp64, float l, float mx)
 {
-    return l > -INFINITY ? exp64(fmax((double)l - (double)mx, -745.0)) : 0.0;
+    const double e = exp64(fmin(fmax((double)l - (double)mx, -745.0), 0.0));
+    return l > -INFINITY ? e : 0.0;
 }
 
 // c with `id` in its low BITS bits, the lower id the larger of two equal c
 template <int BITS> __device__ __forceinline__ double tag(double c, int id)
 {
     constexpr uint32_t M = (1u << BITS) - 1;
-    c = fmin(c + 0.0, 0x1p1023);  // (-0 becomes +0; an infinity would turn into a NaN with its low bits set)
-    const uint64_t u = __builtin_bit_cast(uint64_t, c);
-    const uint32_t hi = (uint32_t)(u >> 32);
-    const uint32_t lo = ((uint32_t)u & ~M) | ((hi >> 31) ? (uint32_t)id : M - (uint32_t)id);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    const uint64_t u = __builtin_bit_cast(uint64_t, fmin(c, 0x1p1023));  // (an infinity would turn into a NaN)
+    const uint32_t hi = (uint32_t)(u >> 32), low = (M ^ (uint32_t)id) ^ (uint32_t)((int32_t)hi >> 31);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | (((uint32_t)u & ~M) | (low & M)));
 }
 template <int BITS> __device__ __forceinline__ int untag(double key)
 {
     constexpr uint32_t M = (1u << BITS) - 1;
     const uint64_t u = __builtin_bit_cast(uint64_t, key);
-    const uint32_t lo = (uint32_t)u & M;
-    return (int)((u >> 63) ? lo : M - lo);
+    return (int)(((uint32_t)u ^ M ^ (uint32_t)((int64_t)u >> 63)) & M);
+}
+// a key (a group) that is out: the value below RG_NONE_MAX, whatever its low word
+__device__ __forceinline__ double none_if(bool out, double key)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, key);
+    return __builtin_bit_cast(double, (uint64_t)(out ? RG_NONE_HI : (uint32_t)(u >> 32)) << 32 | (uint32_t)u);
 }
 __device__ __forceinline__ double none() { return __builtin_bit_cast(double, (uint64_t)RG_NONE_HI << 32); }
+// whether two tagged keys are the same expert's (group's): their low words hold its id
+__device__ __forceinline__ bool same_id(double a, double b)
+{
+    return (uint32_t)__builtin_bit_cast(uint64_t, a) == (uint32_t)__builtin_bit_cast(uint64_t, b);
+}
 
-__device__ __forceinline__ float logit(const void *row, int dtype, int e)
+__device__ __forceinline__ float half_to_f32(uint32_t h, bool bf16)
+{
+    return bf16 ? bf16_to_f32(h & 0xffffu) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+__device__ __forceinline__ float logit(const char *row, int dtype, int e)
 {
     if (dtype == ROUTE_FP32)
         return reinterpret_cast<const float *>(row)[e];
-    const uint16_t h = reinterpret_cast<const uint16_t *>(row)[e];
-    return dtype == ROUTE_BF16 ? bf16_to_f32(h) : (float)__builtin_bit_cast(_Float16, h);
+    return half_to_f32(reinterpret_cast<const uint16_t *>(row)[e], dtype == ROUTE_BF16);
+}
+// the logits e0 ... e0 + PER - 1 of a row (past the last expert the last one again)
+template <int PER> __device__ __forceinline__ void load_logits(const char *row, const RouteGroupedArgs &p, int e0, float *lg)
+{
+    if (PER % 4 == 0 && p.vec) {
+        if (p.dtype == ROUTE_FP32) {
+#pragma unroll
+            for (int j = 0; j < PER / 4; ++j) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(row + (e0 + 4 * j) * 4);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    lg[4 * j + q] = v[q];
+            }
+            return;
+        }
+        u32x2 v[PER / 4 ? PER / 4 : 1];
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j)
+            v[j] = *reinterpret_cast<const u32x2 *>(row + (e0 + 4 * j) * 2);
+        const bool bf16 = p.dtype == ROUTE_BF16;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            lg[j] = half_to_f32(v[j / 4][(j >> 1) & 1] >> (16 * (j & 1)), bf16);
+    } else if (p.dtype == ROUTE_FP32) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            lg[j] = reinterpret_cast<const float *>(row)[min(e0 + j, p.E - 1)];
+    } else {
+        uint32_t h[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            h[j] = reinterpret_cast<const uint16_t *>(row)[min(e0 + j, p.E - 1)];
+        const bool bf16 = p.dtype == ROUTE_BF16;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            lg[j] = half_to_f32(h[j], bf16);
+    }
 }
 
 template <int LANES, int PER>
@@ -155,20 +211,38 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
     const int t = ((int)blockIdx.x * RG_WAVES + (int)(threadIdx.x >> 6)) * TPW + lane / LANES;
     const bool live = t < p.T;  // dead rows run along (they read row 0)
     const char *row = reinterpret_cast<const char *>(p.logits) + (size_t)(live ? t : 0) * (size_t)p.row_bytes;
-    const int g = rl / p.lpg, pos0 = (rl % p.lpg) * PER, e0 = g * p.gs + pos0;
-    // the slots of this lane that hold an expert
+    // (lanes past the last group look at expert 0's, so that their loads stay inside the row, and hold none)
+    const int g = rl / p.lpg, pos0 = (rl % p.lpg) * PER, e0 = g < p.G ? g * p.gs + pos0 : 0;
     const int have = g < p.G ? min(max(p.gs - pos0, 0), PER) : 0;
 
-    float lg[PER];
+    float lg[PER], bs[PER];
+    load_logits<PER>(row, p, e0, lg);
+    if (p.bias) {
+        if (PER % 4 == 0 && p.vec) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-        lg[j] = logit(row, p.dtype, min(e0 + j, p.E - 1));
+            for (int j = 0; j < PER / 4; ++j) {
+                const f32x4 v = *reinterpret_cast<const f32x4 *>(p.bias + e0 + 4 * j);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    bs[4 * j + q] = v[q];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+                bs[j] = p.bias[min(e0 + j, p.E - 1)];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            bs[j] = 0.0f;
+    }
     float mx = -INFINITY;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
         lg[j] = j < have ? lg[j] : -INFINITY;
         mx = fmaxf(mx, lg[j]);
     }
+    const Exp64 exp64;
     const bool softmax = p.score == ROUTE_SOFTMAX;
     const bool by_logit = p.by_logit != 0;
     double denom = 0.0;
@@ -180,21 +254,17 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         if (softmax && !p.renorm) {
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                denom += exp_rel(lg[j], mx);
+                denom += exp_rel(exp64, lg[j], mx);
             denom = row_sum<LANES>(denom);
         }
 #pragma unroll
-        for (int j = 0; j < PER; ++j)
-            key[j] = lg[j] > -INFINITY ? tag<9>((double)lg[j], e0 + j) : none();
+        for (int j = 0; j < PER; ++j)  // (+ 0: the zeros of both signs are equal)
+            key[j] = none_if(!(lg[j] > -INFINITY), tag<9>((double)lg[j] + 0.0, e0 + j));
     } else {
-        float bs[PER];
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            bs[j] = p.bias ? p.bias[min(e0 + j, p.E - 1)] : 0.0f;
         if (softmax) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                key[j] = exp_rel(lg[j], mx);
+                key[j] = exp_rel(exp64, lg[j], mx);
                 denom += key[j];
             }
             denom = row_sum<LANES>(denom);
@@ -205,12 +275,12 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         } else {
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                key[j] = sigmoid64(lg[j]);
+                key[j] = sigmoid64(exp64, lg[j]);
         }
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const double c = key[j] + (double)bs[j];
-            key[j] = lg[j] > -INFINITY && c > -INFINITY ? tag<9>(c, e0 + j) : none();
+            key[j] = none_if(!(lg[j] > -INFINITY) | !(bs[j] > -INFINITY), tag<9>(c, e0 + j));
         }
     }
 
@@ -235,19 +305,17 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         }
         // (the ids in the low bits change a score by 2^-43 of itself at most)
         const double two = p.group_top2 && m2 > RG_NONE_MAX ? m1 + m2 : m1;
-        double gk = m1 > RG_NONE_MAX ? tag<6>(two, g) : none();
+        double gk = none_if(!(m1 > RG_NONE_MAX), tag<6>(two, g));
         bool kept = false;
         for (int i = 0; i < p.KG; ++i) {
             const double win = row_max<LANES>(gk);
-            const bool mine = gk == win && win > RG_NONE_MAX;
+            const bool mine = same_id(gk, win) && win > RG_NONE_MAX;
             kept |= mine;
-            gk = mine ? none() : gk;
+            gk = none_if(mine, gk);
         }
-        if (!kept) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
-                key[j] = none();
-        }
+        for (int j = 0; j < PER; ++j)
+            key[j] = none_if(!kept, key[j]);
     }
 
     int my_idx = -1;
@@ -260,7 +328,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         best = row_max<LANES>(best);
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            key[j] = key[j] == best ? none() : key[j];
+            key[j] = none_if(same_id(key[j], best), key[j]);
         if (rl == k)
             my_idx = best > RG_NONE_MAX ? untag<9>(best) : -1;
     }
@@ -269,9 +337,9 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
     if (my_idx >= 0) {
         const float l = logit(row, p.dtype, my_idx);
         if (!softmax) {
-            gate = sigmoid64(l);
+            gate = sigmoid64(exp64, l);
         } else {
-            gate = exp_rel(l, mx);
+            gate = exp_rel(exp64, l, mx);
             if (denom > 0.0)
                 gate *= recip64(denom);
         }
@@ -311,10 +379,12 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
         lanes = 16;
     a.lpg = lanes / g2;
     const int per = (a.gs + a.lpg - 1) / a.lpg;
+    const uintptr_t bases = (uintptr_t)a.logits | (uintptr_t)a.bias | (uintptr_t)a.row_bytes;
     const int tokens = RG_WAVES * (64 / lanes);
     const dim3 grid((a.T + tokens - 1) / tokens), block(RG_WAVES * 64);
 #define RG_CASE(L, P)                                                                                               \
     if (lanes == L && per <= P) {                                                                                   \
+        a.vec = P % 4 == 0 && a.gs == a.lpg * P && bases % 16 == 0; /* every lane's experts in whole vectors */      \
         hipLaunchKernelGGL((route_grouped_kernel<L, P>), grid, block, 0, s, a);                                     \
         return hipGetLastError();                                                                                   \
     }

@@ -293,42 +293,55 @@ _SCORE = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 1, "top2": 2}
 
 
-def _inputs(op, first, *others):
-    """What the operators around the expert layer ask of their tensors: one GPU, and no gradient (they have no
-    backward)."""
-    dev = first.device
-    grad = torch.is_grad_enabled()
-    for t in (first,) + others:
+def _refuse(op, tensors):
+    """Why _device_index said no."""
+    dev = tensors[0].device
+    for t in tensors:
         if t is None:
             continue
         if t.device != dev:
             raise RuntimeError(f"{op}: all tensors must be on one device (got {dev} and {t.device})")
-        if grad and t.requires_grad:
+        if torch.is_grad_enabled() and t.requires_grad:
             raise RuntimeError(f"{op}: no backward; call it under torch.no_grad() or detach its inputs")
-    if dev.type != "cuda":
-        raise _lib.CamHipError(f"{op} runs on the GPU only; got a tensor on {dev}")
-    return dev
+    raise _lib.CamHipError(f"{op} runs on the GPU only; got a tensor on {dev}")
 
 
-def _run(name, dev, *args):
-    """One entry point on the current stream of `dev`, which need not be the current device."""
-    if dev.index == torch.cuda.current_device():
-        _lib.call(name, *args, device=dev)
+def _device_index(op, *tensors):
+    """What the operators around the expert layer ask of their tensors: one GPU, whose index this is, and no gradient
+    (they have no backward)."""
+    index = tensors[0].get_device()
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and (t.get_device() != index or grad and t.requires_grad):
+            _refuse(op, tensors)
+    if index < 0:
+        _refuse(op, tensors)
+    return index
+
+
+def _run(name, index, *args):
+    """One entry point without a workspace on the current stream of GPU `index`, which need not be the current one.
+    (Straight to the native caller: the smallest calls are bound by the host.)"""
+    entry = getattr(_lib._caller or _lib._calls(), name)
+    if index == torch._C._cuda_getDevice():
+        entry(None, None, 0, torch._C._cuda_getCurrentRawStream(index), *args)
     else:
-        with torch.cuda.device(dev):
-            _lib.call(name, *args, device=dev)
+        with torch.cuda.device(index):
+            entry(None, None, 0, torch._C._cuda_getCurrentRawStream(index), *args)
 
 
 def _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score):
     op = "moe_route_grouped"
-    _check(logits.dim() == 2 and logits.dtype in _DTYPE, f"{op}: logits must be [T,E] float32, bfloat16 or float16")
-    _check(score_func in _SCORE, f"{op}: score_func must be 'softmax' or 'sigmoid' (got {score_func!r})")
-    _check(group_score in _GROUP_SCORE, f"{op}: group_score must be 'max' or 'top2' (got {group_score!r})")
-    E = logits.shape[1]
+    _check(logits.dim() == 2 and logits.dtype in _DTYPE, "moe_route_grouped: logits must be [T,E] float32, bfloat16 or float16")
+    if score_func not in _SCORE:
+        raise RuntimeError(f"{op}: score_func must be 'softmax' or 'sigmoid' (got {score_func!r})")
+    if group_score not in _GROUP_SCORE:
+        raise RuntimeError(f"{op}: group_score must be 'max' or 'top2' (got {group_score!r})")
+    T, E = logits.shape
     if bias is not None:
-        _check(bias.dtype == torch.float32 and tuple(bias.shape) == (E,), f"{op}: bias must be [E] float32")
-    _check(E > 0, f"{op}: no experts")
-    return E
+        _check(bias.dtype == torch.float32 and bias.shape == (E,), "moe_route_grouped: bias must be [E] float32")
+    _check(E > 0, "moe_route_grouped: no experts")
+    return T, E
 
 
 def moe_route_grouped(logits, bias, topk, n_group=1, topk_group=1, score_func="softmax", group_score="top2",
@@ -345,44 +358,45 @@ def moe_route_grouped(logits, bias, topk, n_group=1, topk_group=1, score_func="s
     routed_scaling.  Experts whose logit or bias is -inf (or NaN) are never
     picked; slots left without an expert hold id -1 and weight 0.  logits:
     float32, bfloat16 or float16, rows of any stride."""
-    E = _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
-    dev = _inputs("moe_route_grouped", logits, bias)
-    T = logits.shape[0]
-    lg = logits if logits.stride(1) == 1 and (T < 2 or logits.stride(0) >= E) else logits.contiguous()
+    T, E = _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
+    index = _device_index("moe_route_grouped", logits, bias)
+    step, one = logits.stride()
+    lg = logits
+    if one != 1 or T > 1 and step < E:
+        lg, step = logits.contiguous(), E
     b = None if bias is None else bias.contiguous()
-    idx = torch.empty((T, topk), dtype=torch.int32, device=dev)
-    w = torch.empty((T, topk), dtype=torch.float32, device=dev)
-    _run("camhipMoeRouteGrouped", dev, lg.data_ptr(), None if b is None else b.data_ptr(), T, E, topk, _DTYPE[lg.dtype],
-         lg.stride(0) if T > 1 else E, n_group, topk_group, _SCORE[score_func], _GROUP_SCORE[group_score],
+    idx = lg.new_empty((T, topk), dtype=torch.int32)
+    w = lg.new_empty((T, topk), dtype=torch.float32)
+    _run("camhipMoeRouteGrouped", index, lg.data_ptr(), None if b is None else b.data_ptr(), T, E, topk,
+         _DTYPE[lg.dtype], step if T > 1 else E, n_group, topk_group, _SCORE[score_func], _GROUP_SCORE[group_score],
          1 if renormalize else 0, routed_scaling, idx.data_ptr(), w.data_ptr(), None)
     return idx, w
 
 
 def _norm_check(x, residual, weight, out_quant):
-    op = "add_rms_norm"
-    _check(x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float16),
-           f"{op}: x must be [tokens, hidden] bfloat16 or float16")
-    _check(weight.dtype in (x.dtype, torch.float32) and tuple(weight.shape) == (x.shape[1],),
-           f"{op}: weight must be [hidden] of x's dtype or float32")
+    dt = x.dtype
+    _check(x.dim() == 2 and (dt == torch.bfloat16 or dt == torch.float16),
+           "add_rms_norm: x must be [tokens, hidden] bfloat16 or float16")
+    shape = x.shape
+    H = shape[1]
+    _check((weight.dtype == dt or weight.dtype == torch.float32) and weight.shape == (H,),
+           "add_rms_norm: weight must be [hidden] of x's dtype or float32")
     if residual is not None:
-        _check(residual.dtype == x.dtype and residual.shape == x.shape,
-               f"{op}: residual must have x's shape and dtype")
-    _check(out_quant in (QUANT_NONE, QUANT_INT8_TOKEN, QUANT_FP8_BLOCK), f"{op}: out_quant must be 0, 2 or 3")
-    _check(x.shape[1] > 0, f"{op}: no columns")
-    _check(out_quant != QUANT_FP8_BLOCK or x.shape[1] % 128 == 0, f"{op}: fp8 rows need hidden % 128 == 0")
+        _check(residual.dtype == dt and residual.shape == shape, "add_rms_norm: residual must have x's shape and dtype")
+    _check(out_quant in (QUANT_NONE, QUANT_INT8_TOKEN, QUANT_FP8_BLOCK), "add_rms_norm: out_quant must be 0, 2 or 3")
+    _check(H > 0, "add_rms_norm: no columns")
+    _check(out_quant != QUANT_FP8_BLOCK or H % 128 == 0, "add_rms_norm: fp8 rows need hidden % 128 == 0")
+    return shape
 
 
-def _norm_outputs(x, residual, out_quant):
-    T, H = x.shape
-    dev = x.device
-    new = torch.empty((T, H) if residual is not None else (0,), dtype=x.dtype, device=dev)
+def _norm_outputs(x, shape, residual, out_quant):
+    T, H = shape
+    new = x.new_empty(shape if residual is not None else 0)
     if out_quant == QUANT_NONE:
-        return torch.empty((T, H), dtype=x.dtype, device=dev), torch.empty(0, dtype=torch.float32, device=dev), new
+        return x.new_empty(shape), x.new_empty(0, dtype=torch.float32), new
     if out_quant == QUANT_INT8_TOKEN:
-        return (torch.empty((T, H), dtype=torch.int8, device=dev), torch.empty(T, dtype=torch.float32, device=dev),
-                new)
-    return (torch.empty((T, H), dtype=torch.float8_e4m3fn, device=dev),
-            torch.empty((H // 128, T), dtype=torch.float32, device=dev).t(), new)
+        return x.new_empty(shape, dtype=torch.int8), x.new_empty(T, dtype=torch.float32), new
+    return (x.new_empty(shape, dtype=torch.float8_e4m3fn), x.new_empty((H // 128, T), dtype=torch.float32).t(), new)
 
 
 def add_rms_norm(x, residual, weight, eps=1e-6, out_quant=0):
@@ -396,35 +410,40 @@ def add_rms_norm(x, residual, weight, eps=1e-6, out_quant=0):
     e4m3 y with y_scale [tokens, hidden/128], the transpose of k-major storage
     as grouped_matmul_swiglu reads it.  x may be a column slice of a wider
     tensor (rows of any stride)."""
-    _norm_check(x, residual, weight, out_quant)
-    dev = _inputs("add_rms_norm", x, residual, weight)
-    T, H = x.shape
-    xc = x if x.stride(1) == 1 and (T < 2 or x.stride(0) >= H) else x.contiguous()
+    shape = _norm_check(x, residual, weight, out_quant)
+    index = _device_index("add_rms_norm", x, residual, weight)
+    T, H = shape
+    step, one = x.stride()
+    if one != 1 or T > 1 and step < H:
+        x, step = x.contiguous(), H
     r = None if residual is None else residual.contiguous()
     w = weight.contiguous()
-    y, scale, new = _norm_outputs(x, residual, out_quant)
-    _run("camhipAddRmsNorm", dev, xc.data_ptr(), None if r is None else r.data_ptr(), w.data_ptr(), T, H,
-         xc.stride(0) if T > 1 else H, _DTYPE[x.dtype], _DTYPE[w.dtype],
+    y, scale, new = _norm_outputs(x, shape, residual, out_quant)
+    _run("camhipAddRmsNorm", index, x.data_ptr(), None if r is None else r.data_ptr(), w.data_ptr(), T, H,
+         step if T > 1 else H, _DTYPE[x.dtype], _DTYPE[w.dtype],
          QUANT_FP8_BLOCK_KMAJOR if out_quant == QUANT_FP8_BLOCK else out_quant, eps, y.data_ptr(), scale.data_ptr(),
          new.data_ptr())
     return y, scale, new
 
 
 def _quant_matmul_check(x, x_scale, weight, weight_scale, bias, out_dtype):
-    op = "quant_matmul"
-    _check(x.dim() == 2 and x.dtype == torch.int8 and x.is_contiguous(), f"{op}: x must be [m, k] int8, contiguous")
-    _check(weight.dim() == 2 and weight.dtype == torch.int8 and weight.is_contiguous(),
-           f"{op}: weight must be [n, k] int8, contiguous")
-    (m, k), n = x.shape, weight.shape[0]
-    _check(weight.shape[1] == k, f"{op}: x has {k} columns, weight k = {weight.shape[1]}")
-    _check(x_scale.dtype == torch.float32 and tuple(x_scale.shape) == (m,) and x_scale.is_contiguous(),
-           f"{op}: x_scale must be float32 [m] (per token)")
-    _check(weight_scale.dtype == torch.float32 and tuple(weight_scale.shape) == (n,) and weight_scale.is_contiguous(),
-           f"{op}: weight_scale must be float32 [n] (per channel)")
+    xshape, wshape = x.shape, weight.shape
+    _check(len(xshape) == 2 and x.dtype == torch.int8 and x.is_contiguous(),
+           "quant_matmul: x must be [m, k] int8, contiguous")
+    _check(len(wshape) == 2 and weight.dtype == torch.int8 and weight.is_contiguous(),
+           "quant_matmul: weight must be [n, k] int8, contiguous")
+    m, k = xshape
+    n, kw = wshape
+    if kw != k:
+        raise RuntimeError(f"quant_matmul: x has {k} columns, weight k = {kw}")
+    _check(x_scale.dtype == torch.float32 and x_scale.shape == (m,) and x_scale.is_contiguous(),
+           "quant_matmul: x_scale must be float32 [m] (per token)")
+    _check(weight_scale.dtype == torch.float32 and weight_scale.shape == (n,) and weight_scale.is_contiguous(),
+           "quant_matmul: weight_scale must be float32 [n] (per channel)")
     if bias is not None:
-        _check(bias.dtype == torch.float32 and tuple(bias.shape) == (n,) and bias.is_contiguous(),
-               f"{op}: bias must be float32 [n]")
-    _check(out_dtype in _DTYPE, f"{op}: out_dtype must be bfloat16, float16 or float32")
+        _check(bias.dtype == torch.float32 and bias.shape == (n,) and bias.is_contiguous(),
+               "quant_matmul: bias must be float32 [n]")
+    _check(out_dtype in _DTYPE, "quant_matmul: out_dtype must be bfloat16, float16 or float32")
     return m, n, k
 
 
@@ -437,23 +456,21 @@ def quant_matmul(x, x_scale, weight, weight_scale, bias=None, out_dtype=None):
     them, weight [n, k] int8, k a multiple of 16."""
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
     m, n, k = _quant_matmul_check(x, x_scale, weight, weight_scale, bias, out_dtype)
-    dev = _inputs("quant_matmul", x, x_scale, weight, weight_scale, bias)
-    out = torch.empty((m, n), dtype=out_dtype, device=dev)
-    _run("camhipQuantMatmul", dev, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
+    index = _device_index("quant_matmul", x, x_scale, weight, weight_scale, bias)
+    out = x.new_empty((m, n), dtype=out_dtype)
+    _run("camhipQuantMatmul", index, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(), weight_scale.data_ptr(),
          None if bias is None else bias.data_ptr(), m, n, k, _DTYPE[out_dtype], out.data_ptr())
     return out
 
 
 def moe_route_grouped_meta(logits, bias, topk, n_group=1, topk_group=1, score_func="softmax", group_score="top2",
                            renormalize=True, routed_scaling=1.0):
-    _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
-    T = logits.shape[0]
+    T, _ = _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
     return (logits.new_empty((T, topk), dtype=torch.int32), logits.new_empty((T, topk), dtype=torch.float32))
 
 
 def add_rms_norm_meta(x, residual, weight, eps=1e-6, out_quant=0):
-    _norm_check(x, residual, weight, out_quant)
-    return _norm_outputs(x, residual, out_quant)
+    return _norm_outputs(x, _norm_check(x, residual, weight, out_quant), residual, out_quant)
 
 
 def quant_matmul_meta(x, x_scale, weight, weight_scale, bias=None, out_dtype=None):
