@@ -8,6 +8,11 @@
 // which the squares are added up, and need not wait for that sum.  (a is taken as at least 2^-100: 127 / a stays finite,
 // and a row of zeros gives codes 0 and scale 2^-100 / 127 * r.)  A row that holds an infinity or a NaN has NaN scales.
 //
+// Bound by memory: x, the residual, its sum and the rows pass once, the row in registers from its load to its last store
+// (T = 4096, H = 7168 with a residual: int8 36.4 us = 5.65 TB/s, fp8 39.4, bf16 41.6; T = 32768 bf16 312 us = 6.03 TB/s,
+// where a large copy reaches 4.7; T = 1 3.9 us).  A block per row of 8 waves with 16 columns a thread (4 waves of 32
+// columns: 37.2 us and 4.6 us for one row; 16 waves of 8: 38.6 and 3.75); up to 1024 columns a wave per row.
+//
 // The norm reads v before it is rounded to 16 bits (the stored residual stream is the rounded one): one rounding per
 // output.
 #include "cam_device.h"
@@ -19,12 +24,48 @@ namespace {
 
 constexpr float NORM_TINY = 0x1p-100f;
 
-// 8 elements from p (aligned for its type only: global memory takes unaligned 16-byte accesses)
-__device__ __forceinline__ u32x4 load16(const void *p)
+// Global memory takes 16- and 8-byte accesses at any address: rows of odd strides and widths need no code of their own.
+// Rows stream: read and written nontemporally (T = 4096, H = 7168: bf16 rows 48.6 -> 42.6 us, int8 43.7 -> 38.7, fp8 46.1
+// -> 40.9; T = 32768 324 -> 311 us; the loads or the stores alone about half of that); the weight is cached.
+typedef u32x4 u32x4_u __attribute__((aligned(2)));
+typedef u32x2 u32x2_u __attribute__((aligned(1)));
+// the first n of 8 consecutive 16-bit elements, the others 0
+template <bool STREAM> __device__ __forceinline__ u32x4 load8(const uint16_t *p, int n)
 {
-    u32x4 v;
-    __builtin_memcpy(&v, p, 16);
+    if (n >= 8) {
+        if constexpr (STREAM)
+            return __builtin_nontemporal_load(reinterpret_cast<const u32x4_u *>(p));
+        else
+            return *reinterpret_cast<const u32x4_u *>(p);
+    }
+    u32x4 v = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n)
+            v[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
     return v;
+}
+__device__ __forceinline__ void store8(uint16_t *p, const u32x4 v, int n)
+{
+    if (n >= 8) {
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x4_u *>(p));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n)
+            p[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
+}
+__device__ __forceinline__ void store8(uint8_t *p, const u32x2 v, int n)
+{
+    if (n >= 8) {
+        __builtin_nontemporal_store(v, reinterpret_cast<u32x2_u *>(p));
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n)
+            p[i] = (uint8_t)(v[i >> 2] >> (8 * (i & 3)));
 }
 template <bool FP16> __device__ __forceinline__ float unpack1(uint32_t h)
 {
@@ -54,32 +95,6 @@ template <bool FP16> __device__ __forceinline__ u32x4 pack8(const float *f)
         r[i] = pack2<FP16>(f[2 * i], f[2 * i + 1]);
     return r;
 }
-// the first n (1..8) of 8 packed 16-bit elements
-__device__ __forceinline__ void store16(void *p, const u32x4 v, int n)
-{
-    if (n >= 8) {
-        __builtin_memcpy(p, &v, 16);
-        return;
-    }
-    uint16_t *q = reinterpret_cast<uint16_t *>(p);
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-        if (i < n)
-            q[i] = (uint16_t)(v[i >> 1] >> (16 * (i & 1)));
-}
-__device__ __forceinline__ u32x4 load16_n(const void *p, int n)
-{
-    if (n >= 8)
-        return load16(p);
-    const uint16_t *q = reinterpret_cast<const uint16_t *>(p);
-    u32x4 v = {0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-        if (i < n)
-            v[i >> 1] |= (uint32_t)q[i] << (16 * (i & 1));
-    return v;
-}
-
 __device__ __forceinline__ float wave_sum(float v)
 {
 #pragma unroll
@@ -115,13 +130,27 @@ __global__ __launch_bounds__(64 * ROW_WAVES *ROWS) void add_rms_norm_kernel(cons
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
         const int col = (i * RT + tid) * 8;
-        xv[i] = col < p.H ? load16_n(x + col, p.H - col) : u32x4{0, 0, 0, 0};
+        xv[i] = load8<true>(x + col, p.H - col);
     }
     if (res) {
 #pragma unroll
         for (int i = 0; i < NIT; ++i) {
             const int col = (i * RT + tid) * 8;
-            rv[i] = col < p.H ? load16_n(res + col, p.H - col) : u32x4{0, 0, 0, 0};
+            rv[i] = load8<true>(res + col, p.H - col);
+        }
+    }
+    // (the weight before the first store, which the compiler has to think it may overlap: int8 38.7 -> 36.4 us)
+    u32x4 wv[NIT][2];
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+        const int col = (i * RT + tid) * 8;
+        if (p.weight_fp32) {
+            const uint32_t *wp = reinterpret_cast<const uint32_t *>(p.weight) + col;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                wv[i][j >> 2][j & 3] = col + j < p.H ? wp[j] : 0;
+        } else {
+            wv[i][0] = load8<false>(reinterpret_cast<const uint16_t *>(p.weight) + col, p.H - col);
         }
     }
     float t[NIT][8];
@@ -136,24 +165,20 @@ __global__ __launch_bounds__(64 * ROW_WAVES *ROWS) void add_rms_norm_kernel(cons
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 t[i][j] += r[j];
-            if (n > 0)
-                store16(p.residual_out + row * p.H + col, pack8<FP16>(t[i]), n);
+            store8(p.residual_out + row * p.H + col, pack8<FP16>(t[i]), n);
         }
         float s8 = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             s8 += t[i][j] * t[i][j];
         ss += s8;
-        float w[8] = {};
-        if (n > 0) {
-            if (p.weight_fp32) {
-                const float *wp = reinterpret_cast<const float *>(p.weight) + col;
+        float w[8];
+        if (p.weight_fp32) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    w[j] = j < n ? wp[j] : 0.0f;
-            } else {
-                unpack8<FP16>(load16_n(reinterpret_cast<const uint16_t *>(p.weight) + col, n), w);
-            }
+            for (int j = 0; j < 8; ++j)
+                w[j] = __uint_as_float(wv[i][j >> 2][j & 3]);
+        } else {
+            unpack8<FP16>(wv[i][0], w);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -192,24 +217,15 @@ __global__ __launch_bounds__(64 * ROW_WAVES *ROWS) void add_rms_norm_kernel(cons
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 t[i][j] *= rms;
-            if (col < p.H)
-                store16(y + col, pack8<FP16>(t[i]), p.H - col);
+            store8(y + col, pack8<FP16>(t[i]), p.H - col);
         }
     } else if constexpr (QUANT == QUANT_INT8_TOKEN) {
-        int8_t *y = reinterpret_cast<int8_t *>(p.y) + row * p.H;
+        uint8_t *y = reinterpret_cast<uint8_t *>(p.y) + row * p.H;
         const float a = fmaxf(am, NORM_TINY), inv = 127.0f / a;
 #pragma unroll
         for (int i = 0; i < NIT; ++i) {
-            const int col = (i * RT + tid) * 8, n = p.H - col;
-            const u32x2 v = {int8x4(t[i], inv), int8x4(t[i] + 4, inv)};
-            if (n >= 8) {
-                __builtin_memcpy(y + col, &v, 8);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 7; ++j)
-                    if (j < n)
-                        y[col + j] = (int8_t)(v[j >> 2] >> (8 * (j & 3)));
-            }
+            const int col = (i * RT + tid) * 8;
+            store8(y + col, u32x2{int8x4(t[i], inv), int8x4(t[i] + 4, inv)}, p.H - col);
         }
         if (tid == 0)
             p.scales[row] = a / 127.0f * rms;
@@ -227,13 +243,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES *ROWS) void add_rms_norm_kernel(cons
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 t[i][j] *= inv;
-            if (col < p.H) {
-                const u32x2 v = {f32x4_to_e4m3(t[i][0], t[i][1], t[i][2], t[i][3]),
-                                 f32x4_to_e4m3(t[i][4], t[i][5], t[i][6], t[i][7])};
-                __builtin_memcpy(y + col, &v, 8);
-                if ((tid & 15) == 0)
-                    p.scales[(int64_t)(col / 128) * p.T + row] = a / 448.0f * rms;
-            }
+            store8(y + col, u32x2{f32x4_to_e4m3(t[i][0], t[i][1], t[i][2], t[i][3]),
+                                  f32x4_to_e4m3(t[i][4], t[i][5], t[i][6], t[i][7])}, p.H - col);
+            if (col < p.H && (tid & 15) == 0)
+                p.scales[(int64_t)(col / 128) * p.T + row] = a / 448.0f * rms;
         }
     }
 }

@@ -10,7 +10,8 @@ and can be captured in a HIP graph.  Rows past recv_count[-1] are unused.
 import torch
 
 from . import _lib
-from .ops import QUANT_FP8_BLOCK, QUANT_FP8_BLOCK_KMAJOR, QUANT_INT8_TOKEN, QUANT_NONE
+from .ops import (_DTYPE, _GROUP_SCORE, _SCORE, QUANT_FP8_BLOCK, QUANT_FP8_BLOCK_KMAJOR, QUANT_INT8_TOKEN,
+                  QUANT_NONE)
 
 
 class MoePrefillPlan:
@@ -60,6 +61,16 @@ class MoePrefillPlan:
         _lib.launch("camhipMoeRoute", logits.data_ptr(), None if bias is None else bias.data_ptr(), self.T, self.E,
                     self.K, self.topk_idx.data_ptr(), self.topk_w.data_ptr(), self.topk_idx64.data_ptr(),
                     stream=stream, device=self.device)
+
+    def route_grouped(self, logits, bias=None, n_group=1, topk_group=1, score_func="softmax", group_score="top2",
+                      renormalize=True, routed_scaling=1.0, stream=None):
+        """route() by groups of experts (ops.moe_route_grouped) over E_route experts; logits [T, E_route] float32, bfloat16
+        or float16, rows contiguous.  layout(), dispatch() and combine() take its ids and weights as they take route()'s."""
+        _lib.launch("camhipMoeRouteGrouped", logits.data_ptr(), None if bias is None else bias.data_ptr(), self.T,
+                    self.E_route, self.K, _DTYPE[logits.dtype], logits.stride(0) if self.T > 1 else self.E_route, n_group,
+                    topk_group, _SCORE[score_func], _GROUP_SCORE[group_score], 1 if renormalize else 0, routed_scaling,
+                    self.topk_idx.data_ptr(), self.topk_w.data_ptr(), self.topk_idx64.data_ptr(), stream=stream,
+                    device=self.device)
 
     def layout(self, stream=None):
         _lib.launch("camhipDispatchLayout", self.topk_idx64.data_ptr(), self.T, 1, self.E, self.K, None,
@@ -210,9 +221,13 @@ class MoeLayerPlan(MoePrefillPlan):
         self.experts(w1, w1_scale, w2, w2_scale, stream)
         return self.combine_step(self.y, stream)
 
-    def forward_op_chain(self, x, logits, bias, w1, w1_scale, w2, w2_scale, stream=None):
-        """The same layer through the reference-shaped calls (route, layout, count exchange, dispatch, ..., combine)."""
-        self.route(logits, bias, stream)
+    def forward_op_chain(self, x, logits, bias, w1, w1_scale, w2, w2_scale, stream=None, gating=None):
+        """The same layer through the reference-shaped calls (route, layout, count exchange, dispatch, ..., combine).
+        gating: route_grouped()'s arguments by name, to route by groups of experts."""
+        if gating is None:
+            self.route(logits, bias, stream)
+        else:
+            self.route_grouped(logits, bias, stream=stream, **gating)
         self.layout(stream)
         self.dispatch(x, stream)
         self.experts(w1, w1_scale, w2, w2_scale, stream)
