@@ -53,8 +53,8 @@ def test_many_rows(m, n, k):
 
 # (a size for each of the kernels' shapes, which the launcher takes by what a product costs with them; edges in m, n and k)
 @pytest.mark.parametrize("m,n,k", [(7, 4093, 1040), (13, 4001, 1200), (27, 4093, 1232), (61, 4099, 400), (95, 4091, 848),
-                                   (127, 4097, 976), (250, 4001, 528), (70, 12005, 720), (70, 8235, 272), (129, 8445, 272),
-                                   (385, 8929, 144), (769, 7091, 144), (780, 8263, 144), (1, 28672, 272), (3071, 1, 144)])
+                                   (9, 4567, 144), (250, 4001, 6416), (9, 8697, 272), (70, 8235, 272), (131, 8361, 272),
+                                   (389, 8711, 144), (769, 7021, 656), (1042, 7209, 144), (1, 28672, 272), (3071, 1, 144)])
 def test_every_shape_of_block(m, n, k):
     check(m, n, k, m + n, ALL[(m + n) % 3:] + ALL[:(m + n) % 3], full=True)
 
