@@ -68,6 +68,9 @@ def data(T, E, seed, dtype=torch.float32, spread=1.5):
     (33, 1, 1, 1, 1, "top2"), (17, 7, 7, 7, 7, "max"), (4097, 256, 8, 8, 4, "top2"), (5000, 160, 6, 8, 3, "max"),
     (4100, 512, 16, 1, 1, "top2"), (4099, 60, 6, 5, 2, "top2"), (6001, 33, 9, 11, 4, "top2"), (4111, 8, 8, 1, 1, "max"),
     (4500, 480, 8, 5, 2, "top2"), (4097, 320, 8, 1, 1, "max"), (4097, 384, 6, 4, 2, "max"),
+    # 8 lanes a token, with as many experts a lane as its kernels take, and 16 or 64 beside them
+    (6, 64, 8, 8, 4, "top2"), (8195, 160, 6, 8, 3, "max"), (8193, 100, 5, 5, 2, "top2"), (24577, 256, 8, 8, 4, "top2"),
+    (24580, 192, 7, 1, 1, "max"), (24579, 250, 6, 2, 1, "top2"), (24581, 256, 4, 4, 2, "top2"), (24578, 256, 9, 8, 3, "max"),
 ])
 def test_against_the_definition(T, E, K, G, KG, group, score):
     for i, (dtype, with_bias, renorm) in enumerate([(torch.float32, True, True), (torch.bfloat16, False, False),

@@ -13,7 +13,7 @@
 // a bias s orders as l does, and the keys are the logits themselves (exact: a float leaves 29 bits of a double free):
 // no exponential then, but for the picks and the denominator.
 //
-// A token is handled by LANES (16 or 64) adjacent lanes, each holding PER consecutive experts of one group; a group
+// A token is handled by LANES (8, 16 or 64) adjacent lanes, each holding PER consecutive experts of one group; a group
 // has LANES / (number of groups, rounded up to a power of two) lanes.  So the best two of a group are found by a scan of
 // the lane's own experts and log2 of those lanes' steps, all groups at once.
 #include "cam_device.h"
@@ -95,14 +95,18 @@ template <int STEP> __device__ __forceinline__ double sum_step(double v)
 }
 template <int LANES> __device__ __forceinline__ double row_max(double v)
 {
-    v = max_step<8>(max_step<4>(max_step<2>(max_step<1>(v))));
+    v = max_step<4>(max_step<2>(max_step<1>(v)));
+    if constexpr (LANES >= 16)
+        v = max_step<8>(v);
     if constexpr (LANES == 64)
         v = max_step<32>(max_step<16>(v));
     return v;
 }
 template <int LANES> __device__ __forceinline__ double row_sum(double v)
 {
-    v = sum_step<8>(sum_step<4>(sum_step<2>(sum_step<1>(v))));
+    v = sum_step<4>(sum_step<2>(sum_step<1>(v)));
+    if constexpr (LANES >= 16)
+        v = sum_step<8>(v);
     if constexpr (LANES == 64)
         v = sum_step<32>(sum_step<16>(v));
     return v;
@@ -403,8 +407,10 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
             top2_step<2>(m1, m2);
         if (p.lpg > 4)
             top2_step<4>(m1, m2);
-        if (p.lpg > 8)
-            top2_step<8>(m1, m2);
+        if constexpr (LANES >= 16) {
+            if (p.lpg > 8)
+                top2_step<8>(m1, m2);
+        }
         if constexpr (LANES == 64) {
             if (p.lpg > 16)
                 top2_step<16>(m1, m2);
@@ -429,7 +435,8 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         merge_step<1>(key);
         merge_step<2>(key);
         merge_step<4>(key);
-        merge_step<8>(key);
+        if constexpr (LANES >= 16)
+            merge_step<8>(key);
         if constexpr (LANES == 64) {
             merge_step<16>(key);
             merge_step<32>(key);
@@ -502,7 +509,13 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     // lanes while there are few tokens: 512 experts, 128 tokens 5.5 against 7.6 us, 2048 6.7 against 7.8, 4096 9.4
     // against 8.1.
     const int per16 = g2 <= 16 ? (a.gs + 16 / g2 - 1) / (16 / g2) : 64;
-    const int lanes = per16 <= 16 || (per16 <= 32 && a.T > 3000) ? 16 : 64;
+    const int per8 = g2 <= 8 ? (a.gs + 8 / g2 - 1) / (8 / g2) : 64;
+    int lanes = per16 <= 16 || (per16 <= 32 && a.T > 3000) ? 16 : 64;
+    // 8 lanes for 5 to 8 picks (on sorted lists, a merge step less for half the lanes) where a lane has 8 experts, or where
+    // the tokens fill the GPU: 64 experts 128 tokens 3.6 against 3.9 us, 65536 9.4 against 12.3; 160 in 8 groups, 8192
+    // tokens 5.8 against 7.3, 128 5.6 against 5.1; 256 experts, 65536 tokens 36.1 against 38.6, 8192 8.2 against 7.7.
+    if (a.K > 4 && a.K <= 8 && (per8 <= 8 || (per8 <= 20 && a.T >= 8192) || (per8 <= 32 && a.T >= 24576)))
+        lanes = 8;
     a.lpg = lanes / g2;
     const int per = (a.gs + a.lpg - 1) / a.lpg;
     const uintptr_t bases = (uintptr_t)a.logits | (uintptr_t)a.bias | (uintptr_t)a.row_bytes;
@@ -522,6 +535,11 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
 #define RG_SORT(L, P)                                                                                               \
     if (lanes == L && per <= P && a.K > 4 && a.K <= 8)                                                              \
     RG_LAUNCH(L, P, true)
+    RG_SORT(8, 8);
+    RG_SORT(8, 16);
+    RG_SORT(8, 20);
+    RG_SORT(8, 24);
+    RG_SORT(8, 32);
     RG_CASE(64, 1);
     RG_CASE(64, 2);
     RG_CASE(64, 4);
