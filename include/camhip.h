@@ -81,7 +81,7 @@ CAMHIP_API camhipStatus camhipMoeRoute(void *workspace, uint64_t workspaceSize, 
  * the experts form numGroups groups of numExperts / numGroups consecutive ids; a group's score is its largest c
  * (CAMHIP_ROUTE_GROUP_MAX) or the sum of its two largest (CAMHIP_ROUTE_GROUP_TOP2; of one, if it has no second); the
  * topkGroups best groups are kept (ties -> lower group).  topkIdx[t,k]: the k-th largest c within them (ties -> lower
- * expert id; scores nearer than 2^-43 of their size are ties).  topkWeights[t,k] = s at topkIdx[t,k] (without the bias),
+ * expert id; scores nearer than 2^-42 of their size are ties).  topkWeights[t,k] = s at topkIdx[t,k] (without the bias),
  * if renormalize over (the sum of the K picks' + 1e-20), times routedScaling.
  * An expert whose logit or bias is -inf or NaN is not picked (nor counted in the softmax, if its logit is); a group with
  * none to pick is not kept; slots left without an expert hold id -1 (the calls below skip it) and weight 0.

@@ -36,8 +36,9 @@ struct RouteGroupedArgs {
     int32_t *topk_idx;
     float *topk_w;
     int64_t *topk_idx64;  // or nullptr
-    // set by the launcher: experts per group, lanes per group, whether the keys are the logits, vector loads
-    int gs, lpg, by_logit, vec;
+    // set by the launcher: experts per group, lanes per group and their logarithm, whether the keys are the logits, whether
+    // every lane holds as many experts as it can, vector loads
+    int gs, lpg, lpg_log, by_logit, full, vec;
 };
 hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s);
 

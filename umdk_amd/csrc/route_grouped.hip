@@ -8,8 +8,9 @@
 //
 // Which of two experts comes first may hang on the last bits of their scores, so c is computed in 64 bits (the
 // vector unit runs 64-bit FMAs at the rate of single 32-bit ones) and its order does not depend on how an fp32
-// exponential rounds.  The low 9 mantissa bits of c then hold the expert's id, so that one v_max_f64 reduction gives
-// both the score and the id, with ties to the lower id; scores nearer than 2^-43 of their size count as equal.  Without
+// exponential rounds.  The low 10 mantissa bits of c then hold the expert's place among the lanes (which rises with its
+// id), so that one v_max_f64 reduction gives both the score and the expert, with ties to the lower id; scores nearer than
+// 2^-42 of their size count as equal.  Without
 // a bias s orders as l does, and the keys are the logits themselves (exact: a float leaves 29 bits of a double free):
 // no exponential then, but for the picks and the denominator.
 //
@@ -169,7 +170,7 @@ template <int STEP> __device__ __forceinline__ void merge_step(double *k)
 }
 
 // exp(x) in 64 bits for x in [-700, 700]: x log2 e = n + f, |f| <= 1/2, and the polynomial of degree 9 that meets 2^f in the
-// ten Chebyshev nodes of that interval, within 1.9e-14 of it: below the 2^-43 that count as equal.  n comes out of the
+// ten Chebyshev nodes of that interval, within 1.9e-14 of it: below the 2^-42 that count as equal.  n comes out of the
 // low bits of x log2 e + 1.5 2^52 and goes into the exponent by an integer addition (rounding, conversion and ldexp
 // are slow in 64 bits).  The constants sit in scalar registers: as literals each costs two moves to the FMA that uses it.
 struct Exp64 {
@@ -217,12 +218,12 @@ __device__ __forceinline__ double exp_rel(const Exp64 &exp64, float l, float mx)
     return l > -INFINITY ? e : 0.0;
 }
 
-// c with `id` in its low BITS bits, the lower id the larger of two equal c
-template <int BITS> __device__ __forceinline__ double tag(double c, int id)
+// c with `id` in its low BITS bits, the lower id the larger of two equal c.  flip: all ones of BITS bits ^ id
+template <int BITS> __device__ __forceinline__ double tag(double c, uint32_t flip)
 {
     constexpr uint32_t M = (1u << BITS) - 1;
     const uint64_t u = __builtin_bit_cast(uint64_t, fmin(c, 0x1p1023));  // (an infinity would turn into a NaN)
-    const uint32_t hi = (uint32_t)(u >> 32), low = (M ^ (uint32_t)id) ^ (uint32_t)((int32_t)hi >> 31);
+    const uint32_t hi = (uint32_t)(u >> 32), low = flip ^ (uint32_t)((int32_t)hi >> 31);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | (((uint32_t)u & ~M) | (low & M)));
 }
 template <int BITS> __device__ __forceinline__ int untag(double key)
@@ -231,6 +232,8 @@ template <int BITS> __device__ __forceinline__ int untag(double key)
     const uint64_t u = __builtin_bit_cast(uint64_t, key);
     return (int)(((uint32_t)u ^ M ^ (uint32_t)((int64_t)u >> 63)) & M);
 }
+constexpr int RG_PLACE = 10;  // bits of an expert's place: its lane of the token, then its place in the lane
+constexpr int place_bits(int per) { return per <= 1 ? 0 : 1 + place_bits((per + 1) / 2); }
 // a key (a group) that is out: the value below RG_NONE_MAX, whatever its low word
 __device__ __forceinline__ double none_if(bool out, double key)
 {
@@ -302,8 +305,15 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
     const bool live = t < p.T;  // dead rows run along (they read row 0)
     const char *row = reinterpret_cast<const char *>(p.logits) + (size_t)(live ? t : 0) * (size_t)p.row_bytes;
     // (lanes past the last group look at expert 0's, so that their loads stay inside the row, and hold none)
-    const int g = rl / p.lpg, pos0 = (rl % p.lpg) * PER, e0 = g < p.G ? g * p.gs + pos0 : 0;
+    const int g = rl >> p.lpg_log, pos0 = (rl & (p.lpg - 1)) * PER, e0 = g < p.G ? g * p.gs + pos0 : 0;
     const int have = g < p.G ? min(max(p.gs - pos0, 0), PER) : 0;
+    constexpr int LOG = place_bits(PER);
+    static_assert((LANES << LOG) <= (1 << RG_PLACE), "places fit their bits");
+    const uint32_t flip = ((1u << RG_PLACE) - 1) ^ (uint32_t)(rl << LOG);
+    const auto expert_of = [&](double key) {
+        const int at = untag<RG_PLACE>(key), l = at >> LOG;
+        return (l >> p.lpg_log) * p.gs + (l & (p.lpg - 1)) * PER + (at & ((1 << LOG) - 1));
+    };
 
     float lg[PER], bs[PER];
     load_logits<PER>(row, p, e0, lg);
@@ -326,18 +336,22 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         for (int j = 0; j < PER; ++j)
             bs[j] = 0.0f;
     }
-    float mx = -INFINITY;
+    if (!p.full) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        lg[j] = j < have ? lg[j] : -INFINITY;
-        mx = fmaxf(mx, lg[j]);
+        for (int j = 0; j < PER; ++j)
+            lg[j] = j < have ? lg[j] : -INFINITY;
     }
     const Exp64 exp64;
     const bool softmax = p.score == ROUTE_SOFTMAX;
     const bool by_logit = p.by_logit != 0;
     double denom = 0.0;
-    if (softmax)
+    float mx = -INFINITY;
+    if (softmax) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            mx = fmaxf(mx, lg[j]);
         mx = (float)row_max<LANES>((double)mx);  // (exact)
+    }
 
     double key[SORTED && PER < 8 ? 8 : PER];
     if (by_logit) {
@@ -349,7 +363,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         }
 #pragma unroll
         for (int j = 0; j < PER; ++j)  // (+ 0: the zeros of both signs are equal)
-            key[j] = none_if(!(lg[j] > -INFINITY), tag<9>((double)lg[j] + 0.0, e0 + j));
+            key[j] = none_if(!(lg[j] > -INFINITY), tag<RG_PLACE>((double)lg[j] + 0.0, flip ^ (uint32_t)j));
     } else {
         if (softmax) {
 #pragma unroll
@@ -370,7 +384,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const double c = key[j] + (double)bs[j];
-            key[j] = none_if(!(lg[j] > -INFINITY) | !(bs[j] > -INFINITY), tag<9>(c, e0 + j));
+            key[j] = none_if(!(lg[j] > -INFINITY) | !(bs[j] > -INFINITY), tag<RG_PLACE>(c, flip ^ (uint32_t)j));
         }
     }
 
@@ -415,9 +429,9 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
             if (p.lpg > 16)
                 top2_step<16>(m1, m2);
         }
-        // (the ids in the low bits change a score by 2^-43 of itself at most)
+        // (the places in the low bits change a score by 2^-42 of itself at most)
         const double two = p.group_top2 && m2 > RG_NONE_MAX ? m1 + m2 : m1;
-        double gk = none_if(!(m1 > RG_NONE_MAX), tag<6>(two, g));
+        double gk = none_if(!(m1 > RG_NONE_MAX), tag<6>(two, 63u ^ (uint32_t)g));
         bool kept = false;
         for (int i = 0; i < p.KG; ++i) {
             const double win = row_max<LANES>(gk);
@@ -446,7 +460,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         for (int j = 1; j < 8; ++j)
             mine = rl == j ? key[j] : mine;
         if (rl < p.K && mine > RG_NONE_MAX)
-            my_idx = untag<9>(mine);
+            my_idx = expert_of(mine);
     } else {
 #pragma unroll 1
         for (int k = 0; k < p.K; ++k) {
@@ -459,7 +473,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
             for (int j = 0; j < PER; ++j)
                 key[j] = none_if(same_id(key[j], best), key[j]);
             if (rl == k)
-                my_idx = best > RG_NONE_MAX ? untag<9>(best) : -1;
+                my_idx = best > RG_NONE_MAX ? expert_of(best) : -1;
         }
     }
 
@@ -517,6 +531,7 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     if (a.K > 4 && a.K <= 8 && (per8 <= 8 || (per8 <= 20 && a.T >= 8192) || (per8 <= 32 && a.T >= 24576)))
         lanes = 8;
     a.lpg = lanes / g2;
+    a.lpg_log = __builtin_ctz((unsigned)a.lpg);
     const int per = (a.gs + a.lpg - 1) / a.lpg;
     const uintptr_t bases = (uintptr_t)a.logits | (uintptr_t)a.bias | (uintptr_t)a.row_bytes;
     const int tokens = RG_WAVES * (64 / lanes);
@@ -525,7 +540,8 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     // about 3 PER + 25: from 5 picks of 8 experts a lane on the lists are ahead (16 lanes, PER = 16, K = 8: 300 and 520).
 #define RG_LAUNCH(L, P, S)                                                                                          \
     do {                                                                                                            \
-        a.vec = P % 4 == 0 && a.gs == a.lpg * P && bases % 16 == 0; /* every lane's experts in whole vectors */      \
+        a.full = a.gs == a.lpg * P && a.G == g2;                    /* every lane holds P experts */                \
+        a.vec = P % 4 == 0 && a.gs == a.lpg * P && bases % 16 == 0; /* every lane's experts in whole vectors */     \
         hipLaunchKernelGGL((route_grouped_kernel<L, P, S>), grid, block, 0, s, a);                                  \
         return hipGetLastError();                                                                                   \
     } while (0)
