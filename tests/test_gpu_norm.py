@@ -126,6 +126,21 @@ def test_rows_with_infinities_and_nans_say_so(bad, H):
             assert torch.isnan(y[2, H - 3])
 
 
+def test_offsets_past_32_bits():
+    T, H = 262400, 8192   # 4.3 GB a tensor
+    x = torch.zeros(T, H, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = rows(3, H, 3, torch.bfloat16)
+    w = weights(H, torch.bfloat16)
+    for quant in (0, 2, 3):
+        y, scale, new = umdk_amd.add_rms_norm(x, x, w, 1e-6, quant)
+        ys, ss, ns = umdk_amd.add_rms_norm(x[-3:], x[-3:], w, 1e-6, quant)
+        bits = lambda t: t.contiguous().view(torch.uint8)  # noqa: E731
+        assert torch.equal(bits(y[-3:]), bits(ys)) and torch.equal(new[-3:], ns)
+        assert not quant or torch.equal(scale[-3:], ss)
+        assert (y[T // 2].float() == 0).all()   # (zeros of both signs: a weight below zero turns them)
+        del y, scale, new
+
+
 def test_results_do_not_hang_on_the_batch():
     x, res, w = rows(300, 7168, 3, torch.bfloat16), rows(300, 7168, 4, torch.bfloat16), weights(7168, torch.bfloat16)
     y, _, _ = umdk_amd.add_rms_norm(x, res, w)

@@ -96,6 +96,20 @@ def test_nothing_is_written_behind_the_output():
         assert (room[:32] == 7).all() and (room[32 + m * n:] == 7).all()
 
 
+@pytest.mark.parametrize("m,n,k", [(270000, 24, 16400), (70000, 33001, 48), (5, 270001, 16400)])
+def test_offsets_past_32_bits(m, n, k):
+    # x, the output and W past 4 GiB: the last rows and columns against a product of their own
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randint(-127, 128, (m, k), generator=g, dtype=torch.int8, device=DEV)
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8, device=DEV)
+    xs, ws = torch.rand(m, generator=g, device=DEV), torch.rand(n, generator=g, device=DEV)
+    y = umdk_amd.quant_matmul(x, xs, w, ws)
+    for rows in (slice(0, 3), slice(m // 2, m // 2 + 3), slice(m - 3, m)):
+        for cols in (slice(0, 19), slice(n - 19, n)):
+            want = reference(x[rows].cpu(), xs[rows].cpu(), w[cols].cpu(), ws[cols].cpu(), None, torch.bfloat16)
+            assert torch.equal(y[rows, cols].cpu(), want)
+
+
 def test_agrees_with_the_grouped_product():
     x, xs, w, ws, _ = (t.to(DEV) for t in operands(77, 512, 1024, 9))
     groups = torch.tensor([77], device=DEV)

@@ -138,6 +138,16 @@ def test_rows_with_a_stride_and_no_rows():
     assert ids.shape == (0, 4) and w.shape == (0, 4)
 
 
+def test_offsets_past_32_bits():
+    wide = torch.empty(40000, 30000, dtype=torch.float32, device=DEV)   # 4.8 GB
+    part = wide[:, 29000:29064]
+    fresh, bias = data(40000, 64, 9)
+    part.copy_(fresh)
+    ids, w = umdk_amd.moe_route_grouped(part, bias, 6, score_func="sigmoid")
+    rids, rw = umdk_amd.moe_route_grouped(fresh, bias, 6, score_func="sigmoid")
+    assert torch.equal(ids, rids) and torch.equal(w, rw)
+
+
 def test_same_as_moe_route_where_they_agree():
     logits, _ = data(300, 128, 2)
     ids, w = umdk_amd.moe_route_grouped(logits, None, 6)

@@ -93,7 +93,7 @@ camhipStatus camhipMoeRouteGroupedGetWorkspaceSize(const void *logits, const flo
     CHECK_PARAM(renormalize == 0 || renormalize == 1, "%s: renormalize must be 0 or 1", op);
     CHECK_PARAM(logitsRowStride >= numExperts, "%s: logitsRowStride %lld is below numExperts %lld", op,
                 (ll)logitsRowStride, (ll)numExperts);
-    CHECK_PARAM(logitsRowStride <= (int64_t)1 << 40, "%s: logitsRowStride %lld is out of range", op,
+    CHECK_PARAM(logitsRowStride <= (int64_t)1 << 31, "%s: logitsRowStride %lld is out of range", op,
                 (ll)logitsRowStride);
     if (numTokens > 0) {
         CHECK_PTR(op, logits);
@@ -151,7 +151,7 @@ camhipStatus camhipAddRmsNormGetWorkspaceSize(const void *x, const void *residua
                 "%s: outQuant %lld not supported (0, 2 or 5)", op, (ll)outQuant);
     CHECK_PARAM(outQuant != CAMHIP_QUANT_FP8_BLOCK_KMAJOR || hidden % 128 == 0,
                 "%s: fp8 rows need hidden to be a multiple of 128 (got %lld)", op, (ll)hidden);
-    CHECK_PARAM(xRowStride >= hidden && xRowStride <= (int64_t)1 << 40, "%s: xRowStride %lld is below hidden %lld", op,
+    CHECK_PARAM(xRowStride >= hidden && xRowStride <= (int64_t)1 << 31, "%s: xRowStride %lld out of [hidden %lld,2^31]", op,
                 (ll)xRowStride, (ll)hidden);
     CHECK_PARAM(eps >= 0.0 && eps <= 1.0, "%s: eps %g out of [0,1]", op, eps);
     if (numTokens > 0) {
