@@ -390,10 +390,12 @@ def _norm_check(x, residual, weight, out_quant):
 
 
 def _norm_outputs(x, shape, residual, out_quant):
+    """(y, y_scale, residual_out); residual: contiguous, or None."""
     T, H = shape
-    new = x.new_empty(shape if residual is not None else 0)
+    new = torch.empty_like(residual) if residual is not None else x.new_empty(0)
     if out_quant == QUANT_NONE:
-        return x.new_empty(shape), x.new_empty(0, dtype=torch.float32), new
+        y = torch.empty_like(residual) if residual is not None else x.new_empty(shape)
+        return y, x.new_empty(0, dtype=torch.float32), new
     if out_quant == QUANT_INT8_TOKEN:
         return x.new_empty(shape, dtype=torch.int8), x.new_empty(T, dtype=torch.float32), new
     return (x.new_empty(shape, dtype=torch.float8_e4m3fn), x.new_empty((H // 128, T), dtype=torch.float32).t(), new)
@@ -418,7 +420,7 @@ def add_rms_norm(x, residual, weight, eps=1e-6, out_quant=0):
         x, step = x.contiguous(), H
     r = None if residual is None else residual.contiguous()
     w = weight.contiguous()
-    y, scale, new = _norm_outputs(x, shape, residual, out_quant)
+    y, scale, new = _norm_outputs(x, shape, r, out_quant)
     _run("camhipAddRmsNorm", index, x.data_ptr(), None if r is None else r.data_ptr(), w.data_ptr(), T, H,
          step if T > 1 else H, _DTYPE[x.dtype], _DTYPE[w.dtype],
          QUANT_FP8_BLOCK_KMAJOR if out_quant == QUANT_FP8_BLOCK else out_quant, eps, y.data_ptr(), scale.data_ptr(),
@@ -470,7 +472,8 @@ def moe_route_grouped_meta(logits, bias, topk, n_group=1, topk_group=1, score_fu
 
 
 def add_rms_norm_meta(x, residual, weight, eps=1e-6, out_quant=0):
-    return _norm_outputs(x, _norm_check(x, residual, weight, out_quant), residual, out_quant)
+    r = None if residual is None else residual.contiguous()
+    return _norm_outputs(x, _norm_check(x, residual, weight, out_quant), r, out_quant)
 
 
 def quant_matmul_meta(x, x_scale, weight, weight_scale, bias=None, out_dtype=None):
