@@ -127,6 +127,36 @@ def test_extreme_logits_and_biases():
     assert (ids[:, 0] == 3).all() and (ids[:, 1] == 5).all()
 
 
+def test_a_pick_leaves_the_mirrored_expert_below_zero():
+    # 34 groups of 15 experts, 16 places each: those of (group 32, expert 1) and (group 31, expert 14) add up to 1023, the
+    # places being turned over in keys below zero
+    logits = torch.full((3, 510), -5.0, device=DEV)
+    logits[:, 32 * 15 + 1] = 1.0
+    logits[:, 31 * 15 + 14] = -1.0
+    check(logits, None, 2, G=34, KG=34, renorm=False)
+    # 40 groups of 12: groups 30 and 33, whose ids add up to 63
+    logits = torch.full((3, 480), -5.0, device=DEV)
+    logits[:, 30 * 12] = 1.0
+    logits[:, 33 * 12] = -1.0
+    check(logits, None, 2, G=40, KG=2, group="max", renorm=False)
+
+
+def test_logits_of_infinity_count_as_the_largest_number():
+    logits, bias = data(40, 64, 6)
+    logits[0, 9] = math.inf
+    logits[1, [50, 3]] = math.inf
+    logits[2, :] = math.inf
+    largest = torch.where(logits == math.inf, torch.full_like(logits, torch.finfo(torch.float32).max), logits)
+    for b in (None, bias):
+        for kw in (dict(), dict(group="max"), dict(renorm=False)):
+            own = dict(n_group=8, topk_group=3, score_func="softmax", group_score=kw.get("group", "top2"),
+                       renormalize=kw.get("renorm", True))
+            ids, w = umdk_amd.moe_route_grouped(logits, b, 4, **own)
+            rids, rw = reference(largest, b, 4, G=8, KG=3, **kw)
+            assert torch.equal(ids.cpu(), rids)
+            assert ((w.cpu().double() - rw).abs() <= 2 * U * rw.abs() + 2.0 ** -150).all()
+
+
 def test_rows_with_a_stride_and_no_rows():
     logits, bias = data(50, 200, 8)
     part = logits[:, 20:148]

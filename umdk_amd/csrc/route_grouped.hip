@@ -241,11 +241,9 @@ __device__ __forceinline__ double none_if(bool out, double key)
     return __builtin_bit_cast(double, (uint64_t)(out ? RG_NONE_HI : (uint32_t)(u >> 32)) << 32 | (uint32_t)u);
 }
 __device__ __forceinline__ double none() { return __builtin_bit_cast(double, (uint64_t)RG_NONE_HI << 32); }
-// whether two tagged keys are the same expert's (group's): their low words hold its id
-__device__ __forceinline__ bool same_id(double a, double b)
-{
-    return (uint32_t)__builtin_bit_cast(uint64_t, a) == (uint32_t)__builtin_bit_cast(uint64_t, b);
-}
+// whether two tagged keys are the same expert's (group's).  (The whole keys: a low word alone can be that of another
+// expert's, as the ids in keys below zero are turned over.)
+__device__ __forceinline__ bool same_id(double a, double b) { return a == b; }
 
 __device__ __forceinline__ float half_to_f32(uint32_t h, bool bf16)
 {
@@ -350,7 +348,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             mx = fmaxf(mx, lg[j]);
-        mx = (float)row_max<LANES>((double)mx);  // (exact)
+        mx = fminf((float)row_max<LANES>((double)mx), 0x1.fffffep127f);  // (exact; +inf is taken as the largest number)
     }
 
     double key[SORTED && PER < 8 ? 8 : PER];
