@@ -141,6 +141,19 @@ def test_offsets_past_32_bits():
         del y, scale, new
 
 
+def test_more_rows_than_a_launch_takes_threads_for():
+    T, H = 2 ** 25 + 7, 3   # a wave of 64 threads a row
+    x = torch.ones(T, H, dtype=torch.bfloat16, device=DEV)
+    x[2 ** 25 - 4:] = rows(11, H, 3, torch.bfloat16)
+    w = weights(H, torch.bfloat16)
+    for quant in (0, 2):
+        y, scale, new = umdk_amd.add_rms_norm(x, x, w, 1e-6, quant)
+        ys, ss, ns = umdk_amd.add_rms_norm(x[-12:], x[-12:], w, 1e-6, quant)
+        assert torch.equal(y[-12:], ys) and torch.equal(new[-12:], ns) and (not quant or torch.equal(scale[-12:], ss))
+        assert torch.equal(y[:1], ys[:1]) and bool((y[:2 ** 25 - 4] == y[:1]).all())
+        assert bool((new[:2 ** 25 - 4] == 2).all())
+
+
 def test_results_do_not_hang_on_the_batch():
     x, res, w = rows(300, 7168, 3, torch.bfloat16), rows(300, 7168, 4, torch.bfloat16), weights(7168, torch.bfloat16)
     y, _, _ = umdk_amd.add_rms_norm(x, res, w)

@@ -23,6 +23,9 @@ hipError_t launch_route_hist(const float *logits, const float *bias, int T, int 
                              float *topk_w, int32_t *chunk_counts, int32_t *chunk_pref, int32_t *chunk_rank,
                              hipStream_t s);
 
+// A launch of up to 112 bytes of arguments takes the host 2.75 us, from 120 bytes on 3.5 us.
+constexpr size_t LAUNCH_ARGS = 112;
+
 // ---- routing over groups of experts (route_grouped.hip)
 enum RouteScore { ROUTE_SOFTMAX = 0, ROUTE_SIGMOID = 1 };
 enum RouteDtype { ROUTE_BF16 = 0, ROUTE_FP16 = 1, ROUTE_FP32 = 4 };  // the CAMHIP_DTYPE_* codes
@@ -40,6 +43,7 @@ struct RouteGroupedArgs {
     // every lane holds as many experts as it can, vector loads
     int gs, lpg, lpg_log, by_logit, full, vec;
 };
+static_assert(sizeof(RouteGroupedArgs) <= LAUNCH_ARGS, "a cheap launch");
 hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s);
 
 // ---- residual addition + root-mean-square norm (+ quantisation) (norm.hip)
@@ -49,6 +53,7 @@ struct NormArgs {
     const uint16_t *residual;  // or nullptr; rows of H
     const void *weight;        // [H], x's type or fp32 (weight_fp32)
     int64_t T;
+    int64_t row0;  // the launcher's: the first row of a launch
     int H;
     float eps;
     int fp16, weight_fp32, quant;  // quant: QUANT_NONE, QUANT_INT8_TOKEN, QUANT_FP8_BLOCK (k-major scales)
@@ -56,6 +61,7 @@ struct NormArgs {
     float *scales;                 // [T] (int8), [H/128, T] (fp8)
     uint16_t *residual_out;        // [T, H], with a residual only
 };
+static_assert(sizeof(NormArgs) <= LAUNCH_ARGS, "a cheap launch");
 hipError_t launch_add_rms_norm(const NormArgs &a, hipStream_t s);
 
 // ---- int8 matrix product (qmm.hip)
@@ -68,6 +74,7 @@ struct QmmArgs {
     int N, K, out_dtype;
     void *out;               // [M, N]
 };
+static_assert(sizeof(QmmArgs) + 2 * sizeof(int) <= LAUNCH_ARGS, "a cheap launch");
 hipError_t launch_quant_matmul(const QmmArgs &a, hipStream_t s);
 
 // ---- dispatch layout (layout.hip)

@@ -119,7 +119,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES *ROWS) void add_rms_norm_kernel(cons
 #pragma clang fp contract(off)
     constexpr int RT = 64 * ROW_WAVES;
     static_assert(ROWS == 1 || ROW_WAVES == 1, "a block holds one row, or a row per wave");
-    const int64_t row = (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? (int)(threadIdx.x >> 6) : 0);
+    const int64_t row = p.row0 + (int64_t)blockIdx.x * ROWS + (ROWS > 1 ? (int)(threadIdx.x >> 6) : 0);
     if (ROWS > 1 && row >= p.T)
         return;
     const int tid = ROWS > 1 ? threadIdx.x & 63 : threadIdx.x;
@@ -251,14 +251,22 @@ __global__ __launch_bounds__(64 * ROW_WAVES *ROWS) void add_rms_norm_kernel(cons
     }
 }
 
-template <bool FP16, int QUANT> hipError_t launch_quant(const NormArgs &a, hipStream_t s)
+template <bool FP16, int QUANT> hipError_t launch_quant(NormArgs a, hipStream_t s)
 {
+    // (a launch takes fewer than 2^32 threads: more rows go in several)
 #define NORM_CASE(NIT, RW, ROWS)                                                                                    \
     if (a.H <= NIT * 512 * RW) {                                                                                    \
-        const int64_t grid = (a.T + ROWS - 1) / ROWS;                                                               \
-        hipLaunchKernelGGL((add_rms_norm_kernel<FP16, QUANT, NIT, RW, ROWS>), dim3((uint32_t)grid),                 \
-                           dim3(64 * RW * ROWS), 0, s, a);                                                          \
-        return hipGetLastError();                                                                                   \
+        constexpr int THREADS = 64 * RW * ROWS;                                                                     \
+        constexpr int64_t MOST = ((int64_t)1 << 31) / THREADS * ROWS;                                               \
+        for (; a.row0 < a.T; a.row0 += MOST) {                                                                      \
+            const int64_t rows = a.T - a.row0 < MOST ? a.T - a.row0 : MOST;                                         \
+            hipLaunchKernelGGL((add_rms_norm_kernel<FP16, QUANT, NIT, RW, ROWS>),                                   \
+                               dim3((uint32_t)((rows + ROWS - 1) / ROWS)), dim3(THREADS), 0, s, a);                 \
+            const hipError_t e = hipGetLastError();                                                                 \
+            if (e != hipSuccess)                                                                                    \
+                return e;                                                                                           \
+        }                                                                                                           \
+        return hipSuccess;                                                                                          \
     }
     NORM_CASE(1, 1, 4)
     NORM_CASE(2, 1, 4)
