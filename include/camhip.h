@@ -81,13 +81,14 @@ CAMHIP_API camhipStatus camhipMoeRoute(void *workspace, uint64_t workspaceSize, 
  * the experts form numGroups groups of numExperts / numGroups consecutive ids; a group's score is its largest c
  * (CAMHIP_ROUTE_GROUP_MAX) or the sum of its two largest (CAMHIP_ROUTE_GROUP_TOP2; of one, if it has no second); the
  * topkGroups best groups are kept (ties -> lower group).  topkIdx[t,k]: the k-th largest c within them (ties -> lower
- * expert id; scores nearer than 2^-42 of their size are ties).  topkWeights[t,k] = s at topkIdx[t,k] (without the bias),
- * if renormalize over (the sum of the K picks' + 1e-20), times routedScaling.
+ * expert id; scores nearer than 2^-42 of their size are ties, but where no bias and no sum takes part the order is the
+ * logits').  topkWeights[t,k] = s at topkIdx[t,k] (without the bias), if renormalize over (the sum of the K picks' +
+ * 1e-20), times routedScaling.  A logit of +inf has the softmax of the largest number.
  * An expert whose logit or bias is -inf or NaN is not picked (nor counted in the softmax, if its logit is); a group with
  * none to pick is not kept; slots left without an expert hold id -1 (the calls below skip it) and weight 0.
  * topkIdxInt64 (optional, may be NULL): the same ids as int64.
  * Limits: numTokens <= 65536, 1 <= topK <= 16, numExperts <= 512, numGroups <= 64 and a divisor of numExperts,
- * topK <= topkGroups * numExperts / numGroups. */
+ * topK <= topkGroups * numExperts / numGroups, logitsRowStride in [numExperts,2^31]. */
 #define CAMHIP_ROUTE_SOFTMAX 0
 #define CAMHIP_ROUTE_SIGMOID 1
 #define CAMHIP_ROUTE_GROUP_MAX 1
@@ -385,9 +386,10 @@ CAMHIP_API camhipStatus camhipFusedDeepMoe(void *workspace, uint64_t workspaceSi
  * code = rint(t * (127 / a)), scale = a / 127 * r, where t = v * weight, a = max |t| over the row (at least 2^-100) and
  * r the reciprocal root: the rows and scales of camhipQuantMatmul.  CAMHIP_QUANT_FP8_BLOCK_KMAJOR: y fp8 e4m3fn, the same per 1x128
  * block with 448, yScales k-major [hidden/128, numTokens] (xScaleLayout 1 of the grouped GEMMs).  Values are
- * code * scale.  A row with an infinity or a NaN has NaN scales.
- * Limits: hidden in [1,32768] (a multiple of 128 for fp8), eps in [0,1].  Any element alignment is taken; rows that
- * start on 16 bytes are the fast ones. */
+ * code * scale.  The squares are fp32: rows of magnitudes past 2^63 have r = 0.  The scale is NaN of a row (fp8: a
+ * block) with an infinity and of any row (all its blocks) with a NaN.
+ * Limits: numTokens < 2^31, hidden in [1,32768] (a multiple of 128 for fp8), xRowStride in [hidden,2^31], eps in [0,1].
+ * Any element alignment is taken; rows that start on 16 bytes are the fast ones. */
 CAMHIP_API camhipStatus camhipAddRmsNormGetWorkspaceSize(const void *x, const void *residual, const void *weight,
                                                          int64_t numTokens, int64_t hidden, int64_t xRowStride,
                                                          int64_t dtype, int64_t weightDtype, int64_t outQuant,

@@ -38,6 +38,17 @@ def test_route_grouped_rejects(kw, frag):
     assert st == 161001 and frag in msg, msg
 
 
+def test_misaligned_outputs_are_refused():
+    args = (P, None, 4, 64, 4, 4, 64, 8, 4, 0, 2, 1, 1.0)
+    for out in ((P + 2, P, None), (P, P + 1, None), (P, P, P + 4)):
+        st, _, msg = first_phase("camhipMoeRouteGrouped", *args, *out)
+        assert st == 161001 and "aligned" in msg, msg
+    for kw in (dict(y=P + 1), dict(quant=2, scales=P + 2), dict(res=P, out=P + 1)):
+        st, _, msg = norm(**kw)
+        assert st == 161001 and "aligned" in msg, msg
+    assert norm(quant=2, y=P + 1)[0] == 0   # bytes go anywhere
+
+
 @pytest.mark.parametrize("kw", [dict(logits=None), dict(idx=None), dict(w=None)])
 def test_route_grouped_null_pointers(kw):
     assert route(**kw)[0] == 161002

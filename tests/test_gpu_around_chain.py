@@ -137,6 +137,17 @@ def test_plan_routes_by_groups(T):
     assert torch.equal(out.cpu(), want.bfloat16())
 
 
+def test_plan_refuses_other_logits():
+    plan = MoePrefillPlan(8, 1024, 32, 4, quant_mode=0)
+    good, bias = torch.zeros(8, 32, device=DEV), torch.zeros(32, device=DEV)
+    for logits, b, kw in [(good[:7], bias, {}), (good[:, :16], bias[:16], {}), (good.t().contiguous().t(), bias, {}),
+                          (good.cpu(), bias, {}), (good, bias.cpu(), {}), (good, bias.double(), {}), (good, bias[:31], {}),
+                          (good.double(), bias, {}), (good, bias, dict(score_func="relu")), (good, bias, dict(n_group=5))]:
+        with pytest.raises(RuntimeError):
+            plan.route_grouped(logits, b, **kw)
+    plan.route_grouped(torch.zeros(8, 48, device=DEV)[:, :32], bias, n_group=4, topk_group=2)   # rows of a wider tensor
+
+
 def test_layer_plan_takes_the_gating():
     T, H, E, K, I = 130, 1024, 32, 4, 256
     d = make(T, H, E, I)

@@ -102,6 +102,9 @@ camhipStatus camhipMoeRouteGroupedGetWorkspaceSize(const void *logits, const flo
     }
     CHECK_ALIGN(op, logits, dtype_bytes(logitsDtype));
     CHECK_ALIGN(op, bias, 4);
+    CHECK_ALIGN(op, topkIdx, 4);
+    CHECK_ALIGN(op, topkWeights, 4);
+    CHECK_ALIGN(op, topkIdxInt64, 8);
     cam::RouteGroupedArgs a{};
     a.logits = logits;
     a.row_bytes = logitsRowStride * (int64_t)dtype_bytes(logitsDtype);
@@ -167,6 +170,8 @@ camhipStatus camhipAddRmsNormGetWorkspaceSize(const void *x, const void *residua
     CHECK_ALIGN(op, residual, 2);
     CHECK_ALIGN(op, weight, dtype_bytes(weightDtype));
     CHECK_ALIGN(op, residualOut, 2);
+    CHECK_ALIGN(op, y, outQuant == CAMHIP_QUANT_NONE ? 2 : 1);
+    CHECK_ALIGN(op, yScales, 4);
     cam::NormArgs a{};
     a.x = static_cast<const uint16_t *>(x);
     a.x_stride = xRowStride;

@@ -522,7 +522,7 @@ int q_choose(int64_t M, int64_t N, int64_t K)
 template <auto KERNEL, int LDS> hipError_t q_launch(const QmmArgs &a, int bm, int bn, int threads, hipStream_t s)
 {
     const int64_t mt = (a.M + bm - 1) / bm, nt = (a.N + bn - 1) / bn;
-    if (mt * nt > 0x7fffffff)
+    if (mt * nt * threads > 0xffffffff)  // (no output of that size fits the memory)
         return hipErrorInvalidValue;
     const hipError_t e = allow_lds<KERNEL, LDS>();
     if (e != hipSuccess)

@@ -357,7 +357,8 @@ def moe_route_grouped(logits, bias, topk, n_group=1, topk_group=1, score_func="s
     are s at the picks, over their sum (+ 1e-20) if renormalize, times
     routed_scaling.  Experts whose logit or bias is -inf (or NaN) are never
     picked; slots left without an expert hold id -1 and weight 0.  logits:
-    float32, bfloat16 or float16, rows of any stride."""
+    float32, bfloat16 or float16, rows of any stride; T <= 65536.  No
+    backward: inputs that ask for a gradient are refused in grad mode."""
     T, E = _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
     index = _device_index("moe_route_grouped", logits, bias)
     step, one = logits.stride()
@@ -411,7 +412,8 @@ def add_rms_norm(x, residual, weight, eps=1e-6, out_quant=0):
     [tokens], the rows of quant_matmul and of the int8 grouped GEMMs.  3: fp8
     e4m3 y with y_scale [tokens, hidden/128], the transpose of k-major storage
     as grouped_matmul_swiglu reads it.  x may be a column slice of a wider
-    tensor (rows of any stride)."""
+    tensor (rows of any stride).  No backward: inputs that ask for a gradient
+    (the weight among them) are refused in grad mode."""
     shape = _norm_check(x, residual, weight, out_quant)
     index = _device_index("add_rms_norm", x, residual, weight)
     T, H = shape

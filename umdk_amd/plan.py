@@ -10,7 +10,7 @@ and can be captured in a HIP graph.  Rows past recv_count[-1] are unused.
 import torch
 
 from . import _lib
-from .ops import (_DTYPE, _GROUP_SCORE, _SCORE, QUANT_FP8_BLOCK, QUANT_FP8_BLOCK_KMAJOR, QUANT_INT8_TOKEN,
+from .ops import (_DTYPE, _GROUP_SCORE, _SCORE, _check, _route_grouped_check, QUANT_FP8_BLOCK, QUANT_FP8_BLOCK_KMAJOR, QUANT_INT8_TOKEN,
                   QUANT_NONE)
 
 
@@ -66,6 +66,11 @@ class MoePrefillPlan:
                       renormalize=True, routed_scaling=1.0, stream=None):
         """route() by groups of experts (ops.moe_route_grouped) over E_route experts; logits [T, E_route] float32, bfloat16
         or float16, rows contiguous.  layout(), dispatch() and combine() take its ids and weights as they take route()'s."""
+        shape = _route_grouped_check(logits, bias, self.K, n_group, topk_group, score_func, group_score)
+        _check(shape == (self.T, self.E_route) and logits.stride(1) == 1 and (bias is None or bias.is_contiguous()),
+               "route_grouped: logits must be [T, E_route] with contiguous rows, bias contiguous")
+        _check(logits.device == self.topk_w.device and (bias is None or bias.device == logits.device),
+               "route_grouped: logits and bias must be on the plan's device")
         _lib.launch("camhipMoeRouteGrouped", logits.data_ptr(), None if bias is None else bias.data_ptr(), self.T,
                     self.E_route, self.K, _DTYPE[logits.dtype], logits.stride(0) if self.T > 1 else self.E_route, n_group,
                     topk_group, _SCORE[score_func], _GROUP_SCORE[group_score], 1 if renormalize else 0, routed_scaling,
