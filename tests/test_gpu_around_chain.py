@@ -137,6 +137,54 @@ def test_plan_routes_by_groups(T):
     assert torch.equal(out.cpu(), want.bfloat16())
 
 
+def test_the_long_way_gives_the_same():
+    """Calls that the native caller of tensors leaves to Python: numbers of other types, other strides."""
+    d = make(9)
+    logits = torch.randn(9, 64, device=DEV)
+    a = umdk_amd.moe_route_grouped(logits, None, 4, 8, 2, "sigmoid", "max", True, 2.0)
+    for b in (umdk_amd.moe_route_grouped(logits, None, 4, 8, 2, "sigmoid", "max", True, 2),
+              umdk_amd.moe_route_grouped(logits, None, 4, 8, 2, "sigmoid", "max", 1, 2.0),
+              umdk_amd.moe_route_grouped(logits.t().contiguous().t(), None, 4, 8, 2, "sigmoid", "max", True, 2.0),
+              OPS.moe_route_grouped(logits, None, 4, 8, 2, "sigmoid", "max", True, 2.0)):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    for quant in (0, 2, 3):
+        a = umdk_amd.add_rms_norm(d["x"], d["res"], d["g"], 1.0, quant)
+        for b in (umdk_amd.add_rms_norm(d["x"], d["res"], d["g"], 1, quant),
+                  umdk_amd.add_rms_norm(d["x"].t().contiguous().t(), d["res"].t().contiguous().t(), d["g"], 1.0, quant),
+                  umdk_amd.add_rms_norm(d["x"], d["res"], d["g"].repeat_interleave(2)[::2], 1.0, quant)):
+            for p, q in zip(a, b):
+                assert p.dtype == q.dtype and p.shape == q.shape and p.stride() == q.stride()
+                assert torch.equal(p.contiguous().view(torch.uint8), q.contiguous().view(torch.uint8))
+
+
+def test_parameters_without_a_gradient_to_record():
+    d = make(5)
+    g = torch.nn.Parameter(d["g"])
+    q, s, new = umdk_amd.add_rms_norm(d["x"], d["res"], d["g"], 1e-6, 2)
+    for guard in (torch.no_grad, torch.inference_mode):
+        with guard():
+            for a, b in zip(umdk_amd.add_rms_norm(d["x"], d["res"], g, 1e-6, 2), (q, s, new)):
+                assert torch.equal(a, b) and type(a) is torch.Tensor and not a.requires_grad
+    with pytest.raises(RuntimeError, match="no backward"):
+        umdk_amd.add_rms_norm(d["x"], d["res"], g, 1e-6, 2)
+    logits = torch.randn(5, 32, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        umdk_amd.moe_route_grouped(logits, None, 4)
+    assert umdk_amd.moe_route_grouped(logits.detach(), None, 4)[0].shape == (5, 4)
+
+
+def test_negated_views_and_batched_tensors_are_refused():
+    z = torch.randn(4, 32, dtype=torch.complex64, device=DEV)
+    view = torch.conj(z).imag
+    assert view.is_neg()
+    with pytest.raises(RuntimeError, match="negated"):
+        umdk_amd.moe_route_grouped(view, None, 4)
+    ids, _ = umdk_amd.moe_route_grouped(view.resolve_neg(), None, 4)
+    assert torch.equal(ids, (-z.imag).topk(4, dim=1).indices.int())
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda l: umdk_amd.moe_route_grouped(l, None, 4))(torch.randn(3, 4, 32, device=DEV))
+
+
 def test_plan_refuses_other_logits():
     plan = MoePrefillPlan(8, 1024, 32, 4, quant_mode=0)
     good, bias = torch.zeros(8, 32, device=DEV), torch.zeros(32, device=DEV)

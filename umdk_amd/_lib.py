@@ -39,6 +39,7 @@ SIGNATURES = {
 
 _lib = None
 _caller = None
+_tensor_caller = None
 
 
 class CamHipError(RuntimeError):
@@ -87,6 +88,20 @@ def _calls():
         _camcall.bind(L._handle, CamHipError)
         _caller = _camcall
     return _caller
+
+
+def _tensors():
+    """The native caller that takes tensors (pyext/camops.cpp)."""
+    global _tensor_caller
+    if _tensor_caller is None:
+        L = lib()
+        try:
+            from . import _camops
+        except ImportError as e:
+            raise ImportError(f"umdk_amd/_camops.so is not built ({e}); run `python -m umdk_amd.build`") from e
+        _camops.bind(L._handle, CamHipError, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+        _tensor_caller = _camops
+    return _tensor_caller
 
 
 def _stream(device):

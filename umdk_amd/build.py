@@ -1,10 +1,11 @@
 """Builds libcamhip.so (the C-ABI library of HIP kernels for gfx950) in-tree.
 
-    python -m umdk_amd.build              # -> umdk_amd/lib/libcamhip.so, umdk_amd/_camcall.so
+    python -m umdk_amd.build              # -> umdk_amd/lib/libcamhip.so, umdk_amd/_camcall.so, umdk_amd/_camops.so
 
 Every source is compiled by hipcc for gfx950 only; symbols are hidden except
 the extern "C" entry points declared in include/camhip.h.  _camcall.so is the
-Python caller of those entry points (host code, g++); it takes them from the library that _lib has loaded.
+Python caller of those entry points (host code, g++); it takes them from the library that _lib has loaded.  So does
+_camops.so, which calls some of them with torch's tensors (host code, g++ and torch's headers).
 """
 import os
 import subprocess
@@ -19,6 +20,7 @@ BUILD = os.path.join(HERE, "_build")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libcamhip.so")
 CALLER = os.path.join(HERE, "_camcall.so")
+TENSOR_CALLER = os.path.join(HERE, "_camops.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 COMMON = [
@@ -47,15 +49,30 @@ def _compile(src, defines=(), build_dir=BUILD):
     return obj
 
 
-def _build_caller():
-    tmp = CALLER + ".tmp"
+def _build_pyext(out, src, flags=(), libs=()):
+    tmp = out + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
-           "-I" + os.path.join(ROOT, "include"), "-I" + sysconfig.get_paths()["include"],
-           os.path.join(HERE, "pyext", "camcall.cpp"), "-o", tmp, "-ldl"]
+           "-I" + os.path.join(ROOT, "include"), "-I" + sysconfig.get_paths()["include"], *flags,
+           os.path.join(HERE, "pyext", src), "-o", tmp, "-ldl", *libs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError("building _camcall.so failed:\n" + r.stdout + r.stderr)
-    os.replace(tmp, CALLER)
+        raise RuntimeError(f"building {os.path.basename(out)} failed:\n" + r.stdout + r.stderr)
+    os.replace(tmp, out)
+
+
+def _build_caller():
+    _build_pyext(CALLER, "camcall.cpp")
+
+
+def _build_tensor_caller():
+    import torch
+
+    home = os.path.dirname(torch.__file__)
+    # (no run path: torch's libraries are in the process by the time this one is loaded)
+    _build_pyext(TENSOR_CALLER, "camops.cpp",
+                 ["-I" + os.path.join(home, "include"), "-I" + os.path.join(home, "include/torch/csrc/api/include"),
+                  f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"],
+                 ["-L" + os.path.join(home, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"])
 
 
 def build(verbose=True, defines=(), lib=LIB):
@@ -66,15 +83,16 @@ def build(verbose=True, defines=(), lib=LIB):
     os.makedirs(os.path.dirname(lib), exist_ok=True)
     srcs = sources()
     with ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+        callers = [ex.submit(f) for f in (_build_caller, _build_tensor_caller)] if lib == LIB else []
         objs = list(ex.map(lambda f: _compile(f, defines, build_dir), srcs))
+        for c in callers:
+            c.result()
     tmp = lib + ".tmp"
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", tmp] + objs
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
     os.replace(tmp, lib)
-    if lib == LIB:
-        _build_caller()
     if verbose:
         print(f"built {lib}")
     return lib

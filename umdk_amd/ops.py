@@ -301,6 +301,8 @@ def _refuse(op, tensors):
             continue
         if t.device != dev:
             raise RuntimeError(f"{op}: all tensors must be on one device (got {dev} and {t.device})")
+        if t.is_neg():
+            raise RuntimeError(f"{op}: a tensor is a negated view; resolve_neg() it")
         if torch.is_grad_enabled() and t.requires_grad:
             raise RuntimeError(f"{op}: no backward; call it under torch.no_grad() or detach its inputs")
     raise _lib.CamHipError(f"{op} runs on the GPU only; got a tensor on {dev}")
@@ -312,7 +314,7 @@ def _device_index(op, *tensors):
     index = tensors[0].get_device()
     grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is not None and (t.get_device() != index or grad and t.requires_grad):
+        if t is not None and (t.get_device() != index or grad and t.requires_grad or t.is_neg()):
             _refuse(op, tensors)
     if index < 0:
         _refuse(op, tensors)
@@ -320,14 +322,9 @@ def _device_index(op, *tensors):
 
 
 def _run(name, index, *args):
-    """One entry point without a workspace on the current stream of GPU `index`, which need not be the current one.
-    (Straight to the native caller: the smallest calls are bound by the host.)"""
-    entry = getattr(_lib._caller or _lib._calls(), name)
-    if index == torch._C._cuda_getDevice():
-        entry(None, None, 0, torch._C._cuda_getCurrentRawStream(index), *args)
-    else:
-        with torch.cuda.device(index):
-            entry(None, None, 0, torch._C._cuda_getCurrentRawStream(index), *args)
+    """One entry point without a workspace on the current stream of GPU `index`, which need not be the current one."""
+    with torch.cuda.device(index):
+        _lib.launch(name, *args, stream=torch._C._cuda_getCurrentRawStream(index))
 
 
 def _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score):
@@ -359,6 +356,11 @@ def moe_route_grouped(logits, bias, topk, n_group=1, topk_group=1, score_func="s
     picked; slots left without an expert hold id -1 and weight 0.  logits:
     float32, bfloat16 or float16, rows of any stride; T <= 65536.  No
     backward: inputs that ask for a gradient are refused in grad mode."""
+    out = (_lib._tensor_caller or _lib._tensors()).route_grouped(logits, bias, topk, n_group, topk_group, score_func,
+                                                                 group_score, renormalize, routed_scaling)
+    if out is not None:
+        return out
+    # not an ordinary call: to be refused, or other strides, types of numbers or devices
     T, E = _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
     index = _device_index("moe_route_grouped", logits, bias)
     step, one = logits.stride()
@@ -414,6 +416,9 @@ def add_rms_norm(x, residual, weight, eps=1e-6, out_quant=0):
     as grouped_matmul_swiglu reads it.  x may be a column slice of a wider
     tensor (rows of any stride).  No backward: inputs that ask for a gradient
     (the weight among them) are refused in grad mode."""
+    out = (_lib._tensor_caller or _lib._tensors()).add_rms_norm(x, residual, weight, eps, out_quant)
+    if out is not None:
+        return out
     shape = _norm_check(x, residual, weight, out_quant)
     index = _device_index("add_rms_norm", x, residual, weight)
     T, H = shape
@@ -458,6 +463,9 @@ def quant_matmul(x, x_scale, weight, weight_scale, bias=None, out_dtype=None):
     in int32, rounded once to out_dtype (bfloat16 by default, float16,
     float32).  x [m, k] int8 and x_scale [m] as add_rms_norm(out_quant=2) gives
     them, weight [n, k] int8, k a multiple of 16."""
+    out = (_lib._tensor_caller or _lib._tensors()).quant_matmul(x, x_scale, weight, weight_scale, bias, out_dtype)
+    if out is not None:
+        return out
     out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
     m, n, k = _quant_matmul_check(x, x_scale, weight, weight_scale, bias, out_dtype)
     index = _device_index("quant_matmul", x, x_scale, weight, weight_scale, bias)
