@@ -80,6 +80,20 @@ def test_against_the_definition(T, E, K, G, KG, group, score):
               scaling=[1.0, 16.0, 2.5, 0.3][i])
 
 
+@pytest.mark.parametrize("T,E,K,G,KG", [
+    (3, 96, 6, 1, 1), (2049, 96, 6, 1, 1), (8193, 96, 7, 1, 1), (130, 150, 6, 5, 2), (2050, 150, 6, 5, 2), (2300, 512, 8, 16, 4),
+    (2600, 384, 8, 6, 2), (4097, 512, 12, 16, 4), (8200, 192, 8, 1, 1), (2048, 144, 4, 1, 1), (2049, 144, 4, 1, 1),
+    (7, 36, 5, 3, 2), (9, 300, 8, 3, 2), (5, 468, 9, 13, 5), (11, 20, 5, 1, 1), (8192, 20, 5, 1, 1), (6, 44, 3, 11, 4),
+])
+@pytest.mark.parametrize("off", [0, 1, 4])
+def test_lanes_that_are_not_full_and_slices(T, E, K, G, KG, off):
+    for i, dtype in enumerate((torch.float32, torch.bfloat16, torch.float16)):
+        wide, bias = data(T, E + 16, 3 * T + i, dtype)
+        part, b = wide[:, off:off + E], bias[off:off + E]
+        check(part, b, K, G=G, KG=KG, score="sigmoid")
+        check(part, None, K, G=G, KG=KG, score="softmax", group="max", renorm=False)
+
+
 @pytest.mark.parametrize("T", [6, 4200])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_ties_fall_to_the_lower_id(score, T):

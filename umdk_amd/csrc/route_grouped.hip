@@ -255,38 +255,54 @@ __device__ __forceinline__ float logit(const char *row, int dtype, int e)
         return reinterpret_cast<const float *>(row)[e];
     return half_to_f32(reinterpret_cast<const uint16_t *>(row)[e], dtype == ROUTE_BF16);
 }
-// the logits e0 ... e0 + PER - 1 of a row (past the last expert the last one again)
-template <int PER> __device__ __forceinline__ void load_logits(const char *row, const RouteGroupedArgs &p, int e0, float *lg)
+// The logits e0 ... e0 + PER - 1 of a row, or the biases; past the last expert the last ones again.  vec: by fours (a
+// group's size is a multiple of 4 then, and so is e0).  With every lane full nothing needs to be kept inside the row.  (By
+// fours against one by one: 96 experts, 128 tokens 5.1 -> 4.0 us, 320 experts, 65536 tokens 77 -> 48.)
+template <int PER, typename LOAD> __device__ __forceinline__ void fours(const RouteGroupedArgs &p, int e0, LOAD load)
 {
-    if (PER % 4 == 0 && p.vec) {
-        if (p.dtype == ROUTE_FP32) {
-#pragma unroll
-            for (int j = 0; j < PER / 4; ++j) {
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(row + (e0 + 4 * j) * 4);
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    lg[4 * j + q] = v[q];
-            }
-            return;
-        }
-        u32x2 v[PER / 4 ? PER / 4 : 1];
+    if (p.full) {
 #pragma unroll
         for (int j = 0; j < PER / 4; ++j)
-            v[j] = *reinterpret_cast<const u32x2 *>(row + (e0 + 4 * j) * 2);
-        const bool bf16 = p.dtype == ROUTE_BF16;
+            load(j, e0 + 4 * j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j)
+            load(j, min(e0 + 4 * j, p.E - 4));
+    }
+}
+template <int PER> __device__ __forceinline__ void load_f32(const float *row, const RouteGroupedArgs &p, int e0, float *v)
+{
+    if (PER % 4 == 0 && p.vec) {
+        f32x4 q[PER / 4 ? PER / 4 : 1];
+        fours<PER>(p, e0, [&](int j, int e) { q[j] = *reinterpret_cast<const f32x4 *>(row + e); });
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            v[j] = q[j / 4][j & 3];
+    } else {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            v[j] = row[min(e0 + j, p.E - 1)];
+    }
+}
+template <int PER> __device__ __forceinline__ void load_logits(const char *row, const RouteGroupedArgs &p, int e0, float *lg)
+{
+    if (p.dtype == ROUTE_FP32) {
+        load_f32<PER>(reinterpret_cast<const float *>(row), p, e0, lg);
+        return;
+    }
+    const uint16_t *half = reinterpret_cast<const uint16_t *>(row);
+    const bool bf16 = p.dtype == ROUTE_BF16;
+    if (PER % 4 == 0 && p.vec) {
+        u32x2 v[PER / 4 ? PER / 4 : 1];
+        fours<PER>(p, e0, [&](int j, int e) { v[j] = *reinterpret_cast<const u32x2 *>(half + e); });
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             lg[j] = half_to_f32(v[j / 4][(j >> 1) & 1] >> (16 * (j & 1)), bf16);
-    } else if (p.dtype == ROUTE_FP32) {
-#pragma unroll
-        for (int j = 0; j < PER; ++j)
-            lg[j] = reinterpret_cast<const float *>(row)[min(e0 + j, p.E - 1)];
     } else {
         uint32_t h[PER];
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            h[j] = reinterpret_cast<const uint16_t *>(row)[min(e0 + j, p.E - 1)];
-        const bool bf16 = p.dtype == ROUTE_BF16;
+            h[j] = half[min(e0 + j, p.E - 1)];
 #pragma unroll
         for (int j = 0; j < PER; ++j)
             lg[j] = half_to_f32(h[j], bf16);
@@ -316,19 +332,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
     float lg[PER], bs[PER];
     load_logits<PER>(row, p, e0, lg);
     if (p.bias) {
-        if (PER % 4 == 0 && p.vec) {
-#pragma unroll
-            for (int j = 0; j < PER / 4; ++j) {
-                const f32x4 v = *reinterpret_cast<const f32x4 *>(p.bias + e0 + 4 * j);
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    bs[4 * j + q] = v[q];
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < PER; ++j)
-                bs[j] = p.bias[min(e0 + j, p.E - 1)];
-        }
+        load_f32<PER>(p.bias, p, e0, bs);
     } else {
 #pragma unroll
         for (int j = 0; j < PER; ++j)
@@ -516,18 +520,32 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     a.gs = a.E / a.G;
     // without a bias the scores order as the logits do, and so do the groups by their largest one
     a.by_logit = !a.bias && (a.KG == a.G || !a.group_top2);
-    // 16 lanes a token where that leaves a lane 16 experts at most: no slower than 64 lanes for one token (5.4 us), 5.8
-    // against 8.5 us for 4096 of 256 experts.  With up to 32 (over 256 experts, or groups that fill the lanes badly) 64
-    // lanes while there are few tokens: 512 experts, 128 tokens 5.5 against 7.6 us, 2048 6.7 against 7.8, 4096 9.4
-    // against 8.1.
+    // How many lanes a token gets.  More lanes hold fewer experts each (shorter chains: one token), fewer have fewer steps
+    // between lanes to pay for (many tokens); from 64 lanes to 16 a grid has a quarter of the waves.  In us, sigmoid with a
+    // bias, the lanes chosen first:
+    //   5 to 8 picks, on sorted lists:
+    //     5 to 8 experts in one of 8 lanes: 64 experts, 128 tokens 3.7 against 3.9 in 16 lanes, 65536 tokens 12.0 against 15.2.
+    //     up to 24, from 8192 tokens on: 128 experts 4.7 against 5.1, 160 (8 groups) 5.4 against 6.8, 192 5.4 against 5.7
+    //     (below: 128 experts, 128 tokens 4.4 against 3.8).
+    //     up to 32, from 24576 tokens on: 256 experts (8 groups) 14.6 against 15.1, 65536 tokens 34.7 against 37.3 (16384 both
+    //     11.8; 8192 7.7 against 7.0).
+    //     otherwise 16 lanes: 256 experts, 128 tokens 5.1 against 5.6 in 64; 384 5.3 against 5.5, 2048 tokens 5.4 against 6.7.
+    //     With 25 to 32 experts each only past 2500 tokens: 512 experts, 2048 tokens 7.1 against 6.5, 3000 7.4 against 7.8.
+    //   other numbers of picks, and groups that are not read by fours, go to 64 lanes while there are few tokens:
+    //     128 experts, 4 picks, 128 tokens 3.7 against 4.1 in 16 lanes, 2048 both 4.1; 256 (8 groups), 12 picks, 2048 tokens
+    //     7.5 against 7.7, 4096 10.1 against 7.8; 150 (5 groups), 6 picks, 128 tokens 5.1 against 6.2, 2048 6.0 against 6.4.
+    //     With 25 to 32 experts in one of 16 lanes up to 4096 tokens: 512 experts, 16 picks 12.9 against 13.5 (8192 21.6 against
+    //     18.6).  Up to 4 experts 16 lanes are no slower.
     const int per16 = g2 <= 16 ? (a.gs + 16 / g2 - 1) / (16 / g2) : 64;
     const int per8 = g2 <= 8 ? (a.gs + 8 / g2 - 1) / (8 / g2) : 64;
-    int lanes = per16 <= 16 || (per16 <= 32 && a.T > 3000) ? 16 : 64;
-    // 8 lanes for 5 to 8 picks (on sorted lists, a merge step less for half the lanes) where a lane has 8 experts, or where
-    // the tokens fill the GPU: 64 experts 128 tokens 3.6 against 3.9 us, 65536 9.4 against 12.3; 160 in 8 groups, 8192
-    // tokens 5.8 against 7.3, 128 5.6 against 5.1; 256 experts, 65536 tokens 36.1 against 38.6, 8192 8.2 against 7.7.
-    if (a.K > 4 && a.K <= 8 && (per8 <= 8 || (per8 <= 20 && a.T >= 8192) || (per8 <= 32 && a.T >= 24576)))
+    const bool sorted = a.K > 4 && a.K <= 8;
+    int lanes = per16 <= 32 ? 16 : 64;
+    if (sorted && ((per8 > 4 && per8 <= 8) || (per8 <= 24 && a.T >= 8192) || (per8 <= 32 && a.T >= 24576)))
         lanes = 8;
+    else if (sorted && a.gs % 4 == 0)
+        lanes = per16 <= 24 || (per16 <= 32 && a.T > 2500) ? 16 : 64;
+    else if (per16 > 4 && a.T <= (per16 > 24 ? 4096 : 2048))
+        lanes = 64;
     a.lpg = lanes / g2;
     a.lpg_log = __builtin_ctz((unsigned)a.lpg);
     const int per = (a.gs + a.lpg - 1) / a.lpg;
@@ -539,7 +557,7 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
 #define RG_LAUNCH(L, P, S)                                                                                          \
     do {                                                                                                            \
         a.full = a.gs == a.lpg * P && a.G == g2;                    /* every lane holds P experts */                \
-        a.vec = P % 4 == 0 && a.gs == a.lpg * P && bases % 16 == 0; /* every lane's experts in whole vectors */     \
+        a.vec = P % 4 == 0 && a.gs % 4 == 0 && bases % 16 == 0;     /* a lane's experts in whole vectors */         \
         hipLaunchKernelGGL((route_grouped_kernel<L, P, S>), grid, block, 0, s, a);                                  \
         return hipGetLastError();                                                                                   \
     } while (0)
@@ -564,9 +582,10 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     RG_CASE(16, 4);
     RG_SORT(16, 8);
     RG_CASE(16, 8);
-    RG_SORT(16, 10);
-    RG_CASE(16, 10);
+    if (a.by_logit || a.gs % 4)  // (with scores to compute, 12 by fours are ahead of 10: 160 experts, one token 4.8 against 5.0 us)
+        RG_SORT(16, 10);
     RG_SORT(16, 12);
+    RG_CASE(16, 10);
     RG_CASE(16, 12);
     RG_SORT(16, 16);
     RG_CASE(16, 16);
