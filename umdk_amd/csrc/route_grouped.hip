@@ -218,13 +218,18 @@ __device__ __forceinline__ double exp_rel(const Exp64 &exp64, float l, float mx)
     return l > -INFINITY ? e : 0.0;
 }
 
-// c with `id` in its low BITS bits, the lower id the larger of two equal c.  flip: all ones of BITS bits ^ id
-template <int BITS> __device__ __forceinline__ double tag(double c, uint32_t flip)
+// c with `id` in its low BITS bits, the lower id the larger of two equal c.  flip ^ j: all ones of BITS bits ^ id
+// FINITE: c is.  (Otherwise it is limited first: an infinity would turn into a NaN.)
+template <int BITS, bool FINITE = false> __device__ __forceinline__ double tag(double c, uint32_t flip, int j = 0)
 {
     constexpr uint32_t M = (1u << BITS) - 1;
-    const uint64_t u = __builtin_bit_cast(uint64_t, fmin(c, 0x1p1023));  // (an infinity would turn into a NaN)
-    const uint32_t hi = (uint32_t)(u >> 32), low = flip ^ (uint32_t)((int32_t)hi >> 31);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | (((uint32_t)u & ~M) | (low & M)));
+    const uint64_t u = __builtin_bit_cast(uint64_t, FINITE ? c : fmin(c, 0x1p1023));
+    const uint32_t hi = (uint32_t)(u >> 32);
+    uint32_t sign = (uint32_t)((int32_t)hi >> 31);
+    asm("" : "+v"(sign));  // (a comparison of 64 bits and a selection otherwise)
+    const uint32_t id = __builtin_amdgcn_bitop3_b32(flip, sign, (uint32_t)j, 0x96);       // flip ^ sign ^ j
+    const uint32_t low = __builtin_amdgcn_bitop3_b32(M, id, (uint32_t)u, 0xCA);  // (M & id) | (~M & u)
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | low);
 }
 template <int BITS> __device__ __forceinline__ int untag(double key)
 {
@@ -310,6 +315,7 @@ template <int PER> __device__ __forceinline__ void load_logits(const char *row, 
 }
 
 // SORTED (K <= 8): the lanes sort their experts and merge their lists, in place of a reduction for each pick.
+// (32 experts a lane take 166 registers, three waves of a SIMD; held to 128 they spill: 64 against 33 us at 65536 tokens.)
 template <int LANES, int PER, bool SORTED>
 __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const RouteGroupedArgs p)
 {
@@ -365,7 +371,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         }
 #pragma unroll
         for (int j = 0; j < PER; ++j)  // (+ 0: the zeros of both signs are equal)
-            key[j] = none_if(!(lg[j] > -INFINITY), tag<RG_PLACE>((double)lg[j] + 0.0, flip ^ (uint32_t)j));
+            key[j] = none_if(!(lg[j] > -INFINITY), tag<RG_PLACE>((double)lg[j] + 0.0, flip, j));
     } else {
         if (softmax) {
 #pragma unroll
@@ -384,10 +390,23 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
                 key[j] = sigmoid64(exp64, lg[j]);
         }
 #pragma unroll
-        for (int j = 0; j < PER; ++j) {
-            const double c = key[j] + (double)bs[j];
-            key[j] = none_if(!(lg[j] > -INFINITY) | !(bs[j] > -INFINITY), tag<RG_PLACE>(c, flip ^ (uint32_t)j));
+        for (int j = 0; j < PER; ++j)
+            key[j] += (double)bs[j];
+        // infinities and NaN among the wave's logits and biases: seldom, so that none is looked for one by one
+        float far = 0.0f;
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            far = __builtin_elementwise_maximum(__builtin_elementwise_maximum(far, fabsf(lg[j])), fabsf(bs[j]));
+        if (__any(!(far < INFINITY))) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const bool out = !(lg[j] > -INFINITY) | !(bs[j] > -INFINITY);
+                key[j] = out ? none() : fmin(key[j], 0x1p1023);
+            }
         }
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+            key[j] = tag<RG_PLACE, true>(key[j], flip, j);
     }
 
     // the lane's 8 best, sorted
