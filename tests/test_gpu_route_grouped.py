@@ -94,6 +94,35 @@ def test_lanes_that_are_not_full_and_slices(T, E, K, G, KG, off):
         check(part, None, K, G=G, KG=KG, score="softmax", group="max", renorm=False)
 
 
+@pytest.mark.parametrize("T,E,G,KG", [
+    (5, 256, 1, 1), (5, 256, 8, 4), (1025, 256, 8, 4), (7, 512, 16, 4), (3001, 512, 1, 1), (3, 510, 34, 3), (9, 64, 4, 2),
+    (9, 128, 1, 1), (1030, 160, 8, 3), (1026, 384, 1, 1), (1, 384, 6, 2), (8200, 40, 5, 4), (300, 17, 1, 1), (4, 450, 5, 3),
+])
+def test_many_picks_and_few_experts_left(T, E, G, KG):
+    for K in (9, 12, 16):
+        logits, bias = data(T, E, T + K)
+        logits[0, 5:] = -math.inf                      # fewer experts than picks
+        logits[-1, ::3] = math.nan
+        logits[T // 2, :] = -1.0                       # ties throughout
+        bias[E // 2] = -math.inf
+        check(logits, bias, K, G=G, KG=KG, score="sigmoid")
+        check(logits, bias - 3.0, K, G=G, KG=KG, score="softmax", group="max", renorm=False)
+        check(logits, None, K, G=G, KG=KG, score="softmax", group="max")
+        # the best ones all in one lane: every pick from one list
+        logits[0] = torch.arange(E, device=DEV) * -1e-3
+        check(logits, None, K, G=G, KG=KG, score="sigmoid")
+
+
+@pytest.mark.parametrize("K", [5, 8])
+@pytest.mark.parametrize("T,E,G,KG", [(3, 512, 1, 1), (3, 512, 16, 4), (1000, 384, 1, 1), (1025, 384, 1, 1), (3, 450, 5, 3),
+                                      (3, 510, 34, 3), (3002, 512, 16, 4), (2, 352, 1, 1)])
+def test_five_to_eight_picks_of_many_experts(T, E, G, KG, K):
+    logits, bias = data(T, E, T + K)
+    logits[0, 3:] = -math.inf
+    check(logits, bias, K, G=G, KG=KG, score="sigmoid")
+    check(logits, None, K, G=G, KG=KG, score="softmax", group="max", renorm=False)
+
+
 @pytest.mark.parametrize("T", [6, 4200])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_ties_fall_to_the_lower_id(score, T):

@@ -153,6 +153,25 @@ __device__ __forceinline__ void merge8(double *k, const double *o)
         k[i] = kmax(k[i], o[7 - i]);
     sort_bitonic8(k);
 }
+// k rising and then falling, sorted
+__device__ __forceinline__ void sort_bitonic16(double *k)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        order(k[i], k[i + 8]);
+    sort_bitonic8(k);
+    sort_bitonic8(k + 8);
+}
+__device__ __forceinline__ void sort16(double *k)
+{
+    sort8(k);
+    sort8(k + 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        order(k[i], k[15 - i]);
+    sort_bitonic8(k);
+    sort_bitonic8(k + 8);
+}
 template <int STEP> __device__ __forceinline__ void merge_step(double *k)
 {
     double a[8], b[8];
@@ -318,12 +337,34 @@ template <int PER> __device__ __forceinline__ void load_logits(const char *row, 
     }
 }
 
-// SORTED (K <= 8): the lanes sort their experts and merge their lists, in place of a reduction for each pick.
+// How the picks are found.  RG_EACH: each by a reduction over all of a lane's experts and the lanes.  RG_MERGE (K <= 8): the
+// lanes sort their experts and merge their lists of 8.  RG_POP: the lanes sort their experts, each pick is the largest of the
+// lists' heads, and its lane's list moves up.
+enum { RG_EACH, RG_MERGE, RG_POP };
 // (32 experts a lane take 166 registers, three waves of a SIMD; held to 128 they spill: 64 against 33 us at 65536 tokens.)
-template <int LANES, int PER, bool SORTED>
+// Pick FROM and those behind it, K in all: lane k of a token gets the k-th.
+template <int LANES, int LIST, int FROM> __device__ __forceinline__ void pop_picks(double *key, int K, int rl, double &pick)
+{
+    if constexpr (FROM < 16) {
+        const double best = row_max<LANES>(key[0]);
+        pick = rl == FROM ? best : pick;
+        if (FROM + 1 == K)
+            return;
+        const bool mine = same_id(key[0], best);
+        constexpr int MOVES = LIST - 1 < 15 - FROM ? LIST - 1 : 15 - FROM;  // (what the picks to come may need)
+#pragma unroll
+        for (int j = 0; j < MOVES; ++j)
+            key[j] = mine ? key[j + 1] : key[j];
+        if constexpr (LIST == 8)
+            key[7] = none_if(mine, key[7]);
+        pop_picks<LANES, LIST, FROM + 1>(key, K, rl, pick);
+    }
+}
+template <int LANES, int PER, int PICK>
 __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const RouteGroupedArgs p)
 {
     constexpr int TPW = 64 / LANES;  // tokens per wave
+    constexpr bool SORTED = PICK != RG_EACH;
     const int lane = threadIdx.x & 63, rl = lane & (LANES - 1);
     const int t = ((int)blockIdx.x * RG_WAVES + (int)(threadIdx.x >> 6)) * TPW + lane / LANES;
     const bool live = t < p.T;  // dead rows run along (they read row 0)
@@ -365,7 +406,8 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         mx = fminf((float)row_max<LANES>((double)mx), 0x1.fffffep127f);  // (exact; +inf is taken as the largest number)
     }
 
-    double key[SORTED && PER < 8 ? 8 : PER];
+    constexpr int LIST = PICK == RG_EACH ? PER : PICK == RG_POP && PER > 8 ? 16 : 8;
+    double key[LIST > PER ? LIST : PER];
     if (by_logit) {
         if (softmax && !p.renorm) {
 #pragma unroll
@@ -413,27 +455,43 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
             key[j] = tag<RG_PLACE, true>(key[j], flip, j);
     }
 
-    // the lane's 8 best, sorted
-    constexpr int LIST = SORTED ? 8 : PER, PADDED = (PER + 7) & ~7;
+    // the lane's best, sorted
     if constexpr (SORTED) {
+        constexpr int PADDED = (PER + 7) & ~7;
         double pad[PADDED];
 #pragma unroll
         for (int j = 0; j < PADDED; ++j)
             pad[j] = j < PER ? key[j < PER ? j : 0] : none();
+        if constexpr (LIST == 8) {
 #pragma unroll
-        for (int j = 0; j < PADDED; j += 8) {
-            sort8(pad + j);
-            if (j > 0)
-                merge8(pad, pad + j);
+            for (int j = 0; j < PADDED; j += 8) {
+                sort8(pad + j);
+                if (j > 0)
+                    merge8(pad, pad + j);
+            }
+        } else {
+            sort16(pad);
+            if constexpr (PADDED == 24)
+                sort8(pad + 16);
+            if constexpr (PADDED == 32)
+                sort16(pad + 16);
+            if constexpr (PADDED > 16) {
+#pragma unroll
+                for (int j = 16; j < PADDED; ++j)
+                    pad[31 - j] = kmax(pad[31 - j], pad[j]);
+                sort_bitonic16(pad);
+            }
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < LIST; ++j)
             key[j] = pad[j];
     }
 
     if (p.KG < p.G) {
-        double m1 = key[0], m2 = SORTED ? key[1] : none();
-        if constexpr (!SORTED) {
+        double m1 = key[0], m2 = none();
+        if constexpr (SORTED) {
+            m2 = key[1];
+        } else {
 #pragma unroll
             for (int j = 1; j < PER; ++j) {
                 m2 = kmax(m2, kmin(m1, key[j]));
@@ -470,7 +528,12 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
     }
 
     int my_idx = -1;
-    if constexpr (SORTED) {
+    if constexpr (PICK == RG_POP) {
+        double pick = none();
+        pop_picks<LANES, LIST, 0>(key, p.K, rl, pick);
+        if (pick > RG_NONE_MAX)
+            my_idx = expert_of(pick);
+    } else if constexpr (SORTED) {
         merge_step<1>(key);
         merge_step<2>(key);
         merge_step<4>(key);
@@ -546,36 +609,43 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     // How many lanes a token gets.  More lanes hold fewer experts each (shorter chains: one token), fewer have fewer steps
     // between lanes to pay for (many tokens); from 64 lanes to 16 a grid has a quarter of the waves.  In us, sigmoid with a
     // bias, the lanes chosen first:
-    //   5 to 8 picks, on sorted lists:
+    //   5 to 8 picks, 8 lanes:
     //     5 to 8 experts in one of 8 lanes: 64 experts, 128 tokens 3.7 against 3.9 in 16 lanes, 65536 tokens 12.0 against 15.2.
     //     up to 24, from 8192 tokens on: 128 experts 4.7 against 5.1, 160 (8 groups) 5.4 against 6.8, 192 5.4 against 5.7
     //     (below: 128 experts, 128 tokens 4.4 against 3.8).
     //     up to 32, from 24576 tokens on: 256 experts (8 groups) 14.6 against 15.1, 65536 tokens 34.7 against 37.3 (16384 both
     //     11.8; 8192 7.7 against 7.0).
-    //     otherwise 16 lanes: 256 experts, 128 tokens 5.1 against 5.6 in 64; 384 5.3 against 5.5, 2048 tokens 5.4 against 6.7.
-    //     With 25 to 32 experts each only past 2500 tokens: 512 experts, 2048 tokens 7.1 against 6.5, 3000 7.4 against 7.8.
-    //   other numbers of picks, and groups that are not read by fours, go to 64 lanes while there are few tokens:
-    //     128 experts, 4 picks, 128 tokens 3.7 against 4.1 in 16 lanes, 2048 both 4.1; 256 (8 groups), 12 picks, 2048 tokens
-    //     7.5 against 7.7, 4096 10.1 against 7.8; 150 (5 groups), 6 picks, 128 tokens 5.1 against 6.2, 2048 6.0 against 6.4.
-    //     With 25 to 32 experts in one of 16 lanes up to 4096 tokens: 512 experts, 16 picks 12.9 against 13.5 (8192 21.6 against
-    //     18.6).  Up to 4 experts 16 lanes are no slower.
+    //   64 lanes while there are few tokens, 16 otherwise:
+    //     25 to 32 experts in one of 16 lanes: 512 experts, 8 picks, 2048 tokens 5.5 against 6.8, 3000 6.4 against 6.8, 4096 7.4
+    //     against 6.8; 16 picks 3000 8.5 and 8.5; 4 picks 4096 7.2 against 8.2, 8192 12.0 against 12.2.
+    //     17 to 24, 5 to 8 picks: 384 experts, 1024 tokens 4.9 against 5.1, 2048 6.0 against 5.1.  (256, one token: 4.9 against 4.6.)
+    //     9 to 24, more picks: 256 experts, 16 picks, 1024 tokens 5.6 against 5.9, 2048 6.5 against 5.9.  (128, 10 picks, one
+    //     token 4.6 against 4.0.)
+    //     5 to 24, fewer picks: 128 experts, 4 picks, 128 tokens 3.7 against 4.1, 2048 both 4.1; 256, 2 picks, 2048 4.0 against 4.5.
+    //     groups that are not read by fours: 150 (5 groups), 6 picks, 128 tokens 4.8 against 6.3, 2048 5.7 against 6.5.
     const int per16 = g2 <= 16 ? (a.gs + 16 / g2 - 1) / (16 / g2) : 64;
     const int per8 = g2 <= 8 ? (a.gs + 8 / g2 - 1) / (8 / g2) : 64;
-    const bool sorted = a.K > 4 && a.K <= 8;
-    int lanes = per16 <= 32 ? 16 : 64;
-    if (sorted && ((per8 > 4 && per8 <= 8) || (per8 <= 24 && a.T >= 8192) || (per8 <= 32 && a.T >= 24576)))
+    const bool merged = a.K > 4 && a.K <= 8;
+    int few = 0;
+    if (per16 > 24)
+        few = a.K > 4 ? 3000 : 4096;
+    else if (per16 > 4 && (a.K <= 4 || a.gs % 4))
+        few = 2048;
+    else if (per16 > (merged ? 16 : 8))
+        few = 1024;
+    int lanes = per16 > 32 || a.T <= few ? 64 : 16;
+    if (merged && ((per8 > 4 && per8 <= 8) || (per8 <= 24 && a.T >= 8192) || (per8 <= 32 && a.T >= 24576)))
         lanes = 8;
-    else if (sorted && a.gs % 4 == 0)
-        lanes = per16 <= 24 || (per16 <= 32 && a.T > 2500) ? 16 : 64;
-    else if (per16 > 4 && a.T <= (per16 > 24 ? 4096 : 2048))
-        lanes = 64;
     a.lpg = lanes / g2;
     a.lpg_log = __builtin_ctz((unsigned)a.lpg);
     const int per = (a.gs + a.lpg - 1) / a.lpg;
     const int tokens = RG_WAVES * (64 / lanes);
     const dim3 grid((a.T + tokens - 1) / tokens), block(RG_WAVES * 64);
-    // Sorted lists cost about 100 instructions for 16 experts of a lane and 50 for each of 4 merges, a pick by reduction
-    // about 3 PER + 25: from 5 picks of 8 experts a lane on the lists are ahead (16 lanes, PER = 16, K = 8: 300 and 520).
+    // A pick by a reduction over everything takes about 3 PER + 25 instructions, of a sorted list's heads 45 to 15 (fewer as
+    // fewer are left to move up), a merge of two lists 90; sorting 16 experts 140 (8 of them kept: 100).  So: up to 4 picks by
+    // reductions, 5 to 8 by merges (16 lanes, PER = 16, K = 8: 460 against 520), more from the heads (256 experts, 12 picks,
+    // 4096 tokens 7.5 -> 6.2 us, 512 experts, 16 picks, 65536 tokens 101 -> 78), and from the heads too where 64 lanes would
+    // need six merges (512 experts, 8 picks, one token 5.0 -> 4.2).
 #define RG_LAUNCH(L, P, S)                                                                                          \
     do {                                                                                                            \
         a.full = a.gs == a.lpg * P && a.G == g2;                    /* every lane holds P experts */                \
@@ -585,10 +655,13 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     } while (0)
 #define RG_CASE(L, P)                                                                                               \
     if (lanes == L && per <= P)                                                                                     \
-    RG_LAUNCH(L, P, false)
+    RG_LAUNCH(L, P, RG_EACH)
 #define RG_SORT(L, P)                                                                                               \
     if (lanes == L && per <= P && a.K > 4 && a.K <= 8)                                                              \
-    RG_LAUNCH(L, P, true)
+    RG_LAUNCH(L, P, RG_MERGE)
+#define RG_POPS(L, P)                                                                                               \
+    if (lanes == L && per <= P && a.K > (L == 64 ? 4 : 8))                                                          \
+    RG_LAUNCH(L, P, RG_POP)
     RG_SORT(8, 8);
     RG_SORT(8, 16);
     RG_SORT(8, 20);
@@ -596,12 +669,21 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     RG_SORT(8, 32);
     RG_CASE(64, 1);
     RG_CASE(64, 2);
+    RG_POPS(64, 4);
     RG_CASE(64, 4);
+    RG_POPS(64, 8);
     RG_CASE(64, 8);
+    RG_POPS(64, 16);
     RG_CASE(64, 16);
     RG_CASE(16, 1);
     RG_CASE(16, 2);
+    RG_POPS(16, 4);
     RG_CASE(16, 4);
+    RG_POPS(16, 8);
+    RG_POPS(16, 12);
+    RG_POPS(16, 16);
+    RG_POPS(16, 24);
+    RG_POPS(16, 32);
     RG_SORT(16, 8);
     RG_CASE(16, 8);
     if (a.by_logit || a.gs % 4)  // (with scores to compute, 12 by fours are ahead of 10: 160 experts, one token 4.8 against 5.0 us)
@@ -616,6 +698,7 @@ hipError_t launch_route_grouped(RouteGroupedArgs a, hipStream_t s)
     RG_SORT(16, 32);
     RG_CASE(16, 32);
 #undef RG_SORT
+#undef RG_POPS
 #undef RG_LAUNCH
 #undef RG_CASE
     return hipErrorInvalidValue;
