@@ -81,9 +81,11 @@ CAMHIP_API camhipStatus camhipMoeRoute(void *workspace, uint64_t workspaceSize, 
  * the experts form numGroups groups of numExperts / numGroups consecutive ids; a group's score is its largest c
  * (CAMHIP_ROUTE_GROUP_MAX) or the sum of its two largest (CAMHIP_ROUTE_GROUP_TOP2; of one, if it has no second); the
  * topkGroups best groups are kept (ties -> lower group).  topkIdx[t,k]: the k-th largest c within them (ties -> lower
- * expert id; scores nearer than 2^-42 of their size are ties, but where no bias and no sum takes part the order is the
- * logits').  topkWeights[t,k] = s at topkIdx[t,k] (without the bias), if renormalize over (the sum of the K picks' +
- * 1e-20), times routedScaling.  A logit of +inf has the softmax of the largest number.
+ * expert id).  Where no bias and no sum takes part the order is the logits'.  Otherwise the choice rounds s to 42 fraction
+ * bits (an s below e^-700 counts as that) and computes c and the sums in 64 bits; two c nearer than 2^-42, two sums
+ * nearer than 2^-46 of their size may count as ties.  topkWeights[t,k] = s at topkIdx[t,k] (without the bias), if
+ * renormalize over (the sum of the K picks' + 1e-20), times routedScaling.  A logit of +inf has the softmax of the largest
+ * number.
  * An expert whose logit or bias is -inf or NaN is not picked (nor counted in the softmax, if its logit is); a group with
  * none to pick is not kept; slots left without an expert hold id -1 (the calls below skip it) and weight 0.
  * topkIdxInt64 (optional, may be NULL): the same ids as int64.

@@ -173,3 +173,32 @@ def test_captured_and_replayed():
         for a, b in zip(held, umdk_amd.add_rms_norm(x, res, w, 1e-6, 2)):
             torch.cuda.synchronize()
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("H", [256, 513, 7168])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_infinities_under_a_weight_of_zero_and_bad_weights_say_so(bad, H):
+    x, res, w = rows(5, H, 3, torch.bfloat16), rows(5, H, 4, torch.bfloat16), weights(H, torch.bfloat16)
+    w[7] = 0
+    x[2, 7] = bad                     # 0 times it is NaN in the formula
+    for quant in (0, 2, 3):
+        if quant == 3 and H % 128:
+            continue
+        y, scale, _ = umdk_amd.add_rms_norm(x, res, w, 1e-6, quant)
+        if quant == 0:
+            assert torch.isnan(y[2, 7])
+            continue
+        by_row = torch.isnan(scale) if quant == 2 else torch.isnan(scale[:, 0])
+        assert by_row.tolist() == [False, False, True, False, False]
+    x[2, 7] = 1.0
+    w[7] = bad                        # every row has it
+    for quant in (0, 2, 3):
+        if quant == 3 and H % 128:
+            continue
+        y, scale, _ = umdk_amd.add_rms_norm(x, res, w, 1e-6, quant)
+        if quant == 0:
+            assert not torch.isfinite(y[:, 7]).any() and torch.isfinite(y[:, 8:]).all()
+        elif quant == 2:
+            assert not torch.isfinite(scale).any()
+        else:
+            assert not torch.isfinite(scale[:, 0]).any() and torch.isfinite(scale[:, 1:]).all()

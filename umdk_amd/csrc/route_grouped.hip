@@ -8,10 +8,12 @@
 //
 // Which of two experts comes first may hang on the last bits of their scores, so c is computed in 64 bits (the
 // vector unit runs 64-bit FMAs at the rate of single 32-bit ones) and its order does not depend on how an fp32
-// exponential rounds.  The low 10 mantissa bits of c then hold the expert's place among the lanes (which rises with its
-// id), so that one v_max_f64 reduction gives both the score and the expert, with ties to the lower id; scores nearer than
-// 2^-42 of their size count as equal.  Without a bias s orders as l does, and the keys are the logits themselves (exact: a
-// float leaves 29 bits of a double free): no exponential then, but for the picks and the denominator.
+// exponential rounds.  For the choice s is rounded to 42 fraction bits: what is left of the exponential's error goes (1/2
+// is 1/2), and s + b and the sum of two such are exact in 64 bits for most biases, so that sums of different parts that
+// are equal are found equal.  The low 10 mantissa bits of c then give way to the expert's place among the lanes (which
+// rises with its id), so that one v_max_f64 reduction gives both the score and the expert, with ties to the lower id; a
+// group's sum is taken before that, of the whole c.  Without a bias s orders as l does, and the keys are the logits
+// themselves (exact: a float leaves 29 bits of a double free): no exponential then, but for the picks and the denominator.
 //
 // A token is handled by LANES (8, 16 or 64) adjacent lanes, each holding PER consecutive experts of one group; a group
 // has LANES / (number of groups, rounded up to a power of two) lanes.  So the best two of a group are found by a scan of
@@ -191,7 +193,7 @@ template <int STEP> __device__ __forceinline__ void merge_step(double *k)
 }
 
 // exp(x) in 64 bits for x in [-700, 700]: x log2 e = n + f, |f| <= 1/2, and the polynomial of degree 9 that meets 2^f in the
-// ten Chebyshev nodes of that interval, within 1.9e-14 of it: below the 2^-42 that count as equal.  n comes out of the
+// ten Chebyshev nodes of that interval, within 1.9e-14 of it: a twelfth of the last of the 42 bits that count.  n comes out of the
 // low bits of x log2 e + 1.5 2^52 and goes into the exponent by an integer addition (rounding, conversion and ldexp
 // are slow in 64 bits).  The constants sit in scalar registers: as literals each costs two moves to the FMA that uses it.
 struct Exp64 {
@@ -237,6 +239,13 @@ __device__ __forceinline__ double exp_rel(const Exp64 &exp64, float l, float mx)
 {
     const double e = exp64(fmin(fmax((double)l - (double)mx, -700.0), 0.0));
     return l > -INFINITY ? e : 0.0;
+}
+
+// s >= 0 to 42 fraction bits, the nearest.  (A carry goes on into the exponent, as it should.)
+__device__ __forceinline__ double round42(double s)
+{
+    const uint64_t u = __builtin_bit_cast(uint64_t, s) + 0x200;
+    return __builtin_bit_cast(double, (u >> 32) << 32 | ((uint32_t)u & ~0x3FFu));
 }
 
 // c with `id` in its low BITS bits, the lower id the larger of two equal c.  flip ^ j: all ones of BITS bits ^ id
@@ -362,6 +371,49 @@ template <int LANES, int LIST, int FROM> __device__ __forceinline__ void pop_pic
         pop_picks<LANES, LIST, FROM + 1>(key, K, rl, pick);
     }
 }
+
+// the two largest of a group, from those of its lanes
+template <int LANES> __device__ __forceinline__ void best_two_of_group(int lpg, double &m1, double &m2)
+{
+    if (lpg > 1)
+        top2_step<1>(m1, m2);
+    if (lpg > 2)
+        top2_step<2>(m1, m2);
+    if (lpg > 4)
+        top2_step<4>(m1, m2);
+    if constexpr (LANES >= 16) {
+        if (lpg > 8)
+            top2_step<8>(m1, m2);
+    }
+    if constexpr (LANES == 64) {
+        if (lpg > 16)
+            top2_step<16>(m1, m2);
+    }
+}
+// the two largest of a lane
+template <int N> __device__ __forceinline__ void best_two(const double *k, double &m1, double &m2)
+{
+    m1 = k[0];
+    m2 = none();
+#pragma unroll
+    for (int j = 1; j < N; ++j) {
+        m2 = kmax(m2, kmin(m1, k[j]));
+        m1 = kmax(m1, k[j]);
+    }
+}
+// whether this lane's group g, of that score, is among the KG best (some: there is an expert to pick in it)
+template <int LANES> __device__ __forceinline__ bool keep_group(int KG, int g, double score, bool some)
+{
+    double gk = none_if(!some, tag<6>(score, 63u ^ (uint32_t)g));
+    bool kept = false;
+    for (int i = 0; i < KG; ++i) {
+        const double win = row_max<LANES>(gk);
+        const bool mine = same_id(gk, win) && win > RG_NONE_MAX;
+        kept |= mine;
+        gk = none_if(mine, gk);
+    }
+    return kept;
+}
 template <int LANES, int PER, int PICK>
 __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const RouteGroupedArgs p)
 {
@@ -398,7 +450,8 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
     }
     const Exp64 exp64;
     const bool softmax = p.score == ROUTE_SOFTMAX;
-    const bool by_logit = p.by_logit != 0;
+    const bool by_logit = p.by_logit != 0, choose = p.KG < p.G;
+    bool kept = true;
     double denom = 0.0;
     float mx = -INFINITY;
     if (softmax) {
@@ -439,7 +492,7 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
         }
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            key[j] += (double)bs[j];
+            key[j] = round42(key[j]) + (double)bs[j];
         // infinities and NaN among the wave's logits and biases: seldom, so that none is looked for one by one
         float far = 0.0f;
 #pragma unroll
@@ -451,6 +504,15 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
                 const bool out = !(lg[j] > -INFINITY) | !(bs[j] > -INFINITY);
                 key[j] = out ? none() : fmin(key[j], 0x1p1023);
             }
+        }
+        // sums of whole scores: with the places in their low bits, which weigh by each one's exponent, those would decide
+        // between equal sums of different parts.  (The sorted keys' two first would be free: 512 experts, 65536 tokens 61.5
+        // us against 65.8; 256 36.8 and 36.0, one token 4.9 and 4.9.)
+        if (choose && p.group_top2) {
+            double m1, m2;
+            best_two<PER>(key, m1, m2);
+            best_two_of_group<LANES>(p.lpg, m1, m2);
+            kept = keep_group<LANES>(p.KG, g, m2 > RG_NONE_MAX ? m1 + m2 : m1, m1 > RG_NONE_MAX);
         }
 #pragma unroll
         for (int j = 0; j < PER; ++j)
@@ -489,40 +551,13 @@ __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const Rout
             key[j] = pad[j];
     }
 
-    if (p.KG < p.G) {
-        double m1 = key[0], m2 = none();
-        if constexpr (SORTED) {
-            m2 = key[1];
-        } else {
-#pragma unroll
-            for (int j = 1; j < PER; ++j) {
-                m2 = kmax(m2, kmin(m1, key[j]));
-                m1 = kmax(m1, key[j]);
-            }
-        }
-        if (p.lpg > 1)
-            top2_step<1>(m1, m2);
-        if (p.lpg > 2)
-            top2_step<2>(m1, m2);
-        if (p.lpg > 4)
-            top2_step<4>(m1, m2);
-        if constexpr (LANES >= 16) {
-            if (p.lpg > 8)
-                top2_step<8>(m1, m2);
-        }
-        if constexpr (LANES == 64) {
-            if (p.lpg > 16)
-                top2_step<16>(m1, m2);
-        }
-        // (the places in the low bits change a score by 2^-42 of itself at most)
-        const double two = p.group_top2 && m2 > RG_NONE_MAX ? m1 + m2 : m1;
-        double gk = none_if(!(m1 > RG_NONE_MAX), tag<6>(two, 63u ^ (uint32_t)g));
-        bool kept = false;
-        for (int i = 0; i < p.KG; ++i) {
-            const double win = row_max<LANES>(gk);
-            const bool mine = same_id(gk, win) && win > RG_NONE_MAX;
-            kept |= mine;
-            gk = none_if(mine, gk);
+    if (choose) {
+        if (!p.group_top2) {  // (the places give equal ones to the lower group, as its tag does)
+            double m1 = key[0], m2 = none();
+            if constexpr (!SORTED)
+                best_two<PER>(key, m1, m2);
+            best_two_of_group<LANES>(p.lpg, m1, m2);
+            kept = keep_group<LANES>(p.KG, g, m1, m1 > RG_NONE_MAX);
         }
 #pragma unroll
         for (int j = 0; j < LIST; ++j)
