@@ -389,7 +389,8 @@ CAMHIP_API camhipStatus camhipFusedDeepMoe(void *workspace, uint64_t workspaceSi
  * r the reciprocal root: the rows and scales of camhipQuantMatmul.  CAMHIP_QUANT_FP8_BLOCK_KMAJOR: y fp8 e4m3fn, the same per 1x128
  * block with 448, yScales k-major [hidden/128, numTokens] (xScaleLayout 1 of the grouped GEMMs).  Values are
  * code * scale.  The squares are fp32: rows of magnitudes past 2^63 have r = 0.  The scale is NaN of a row (fp8: a
- * block) with an infinity and of any row (all its blocks) with a NaN.
+ * block) with an infinity and of any row (all its blocks) with a NaN, whatever the weight there, and not finite where the
+ * weight is not.
  * Limits: numTokens < 2^31, hidden in [1,32768] (a multiple of 128 for fp8), xRowStride in [hidden,2^31], eps in [0,1].
  * Any element alignment is taken; rows that start on 16 bytes are the fast ones. */
 CAMHIP_API camhipStatus camhipAddRmsNormGetWorkspaceSize(const void *x, const void *residual, const void *weight,
