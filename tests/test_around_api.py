@@ -6,6 +6,7 @@ import torch
 
 import umdk_amd
 from umdk_amd import _lib
+from umdk_amd.plan import MoePrefillPlan
 
 P = 0x1000  # a non-NULL stand-in pointer: never dereferenced by the first phase
 
@@ -153,3 +154,13 @@ def test_shape_functions():
     out = ops.quant_matmul(m(5, 32, dtype=i8), m(5), m(7, 32, dtype=i8), m(7), None, torch.float16)
     assert out.shape == (5, 7) and out.dtype == torch.float16
     assert ops.quant_matmul(m(5, 32, dtype=i8), m(5), m(7, 32, dtype=i8), m(7)).dtype == bf
+
+
+def test_the_plan_refuses_gradients_and_negated_views():
+    plan = MoePrefillPlan(4, 1024, 8, 2, quant_mode=0, device="cpu")   # (its host side: nothing is launched)
+    good = z(4, 8)
+    for logits, bias, why in [(good.requires_grad_(), z(8), "no backward"), (z(4, 8), z(8).requires_grad_(), "no backward"),
+                              (torch._neg_view(z(4, 8)), z(8), "negated"), (z(4, 8), torch._neg_view(z(8)), "negated"),
+                              (z(4, 8), z(8), "GPU only")]:
+        with pytest.raises(RuntimeError, match=why):
+            plan.route_grouped(logits, bias)

@@ -10,8 +10,8 @@ and can be captured in a HIP graph.  Rows past recv_count[-1] are unused.
 import torch
 
 from . import _lib
-from .ops import (_DTYPE, _GROUP_SCORE, _SCORE, _check, _route_grouped_check, QUANT_FP8_BLOCK, QUANT_FP8_BLOCK_KMAJOR, QUANT_INT8_TOKEN,
-                  QUANT_NONE)
+from .ops import (_DTYPE, _GROUP_SCORE, _SCORE, _check, _device_index, _route_grouped_check, QUANT_FP8_BLOCK,
+                  QUANT_FP8_BLOCK_KMAJOR, QUANT_INT8_TOKEN, QUANT_NONE)
 
 
 class MoePrefillPlan:
@@ -65,12 +65,13 @@ class MoePrefillPlan:
     def route_grouped(self, logits, bias=None, n_group=1, topk_group=1, score_func="softmax", group_score="top2",
                       renormalize=True, routed_scaling=1.0, stream=None):
         """route() by groups of experts (ops.moe_route_grouped) over E_route experts; logits [T, E_route] float32, bfloat16
-        or float16, rows contiguous.  layout(), dispatch() and combine() take its ids and weights as they take route()'s."""
+        or float16, rows contiguous; inputs that ask for a gradient are refused, as by the operator.  layout(), dispatch() and
+        combine() take its ids and weights as they take route()'s."""
         shape = _route_grouped_check(logits, bias, self.K, n_group, topk_group, score_func, group_score)
         _check(shape == (self.T, self.E_route) and logits.stride(1) == 1 and (bias is None or bias.is_contiguous()),
                "route_grouped: logits must be [T, E_route] with contiguous rows, bias contiguous")
-        _check(logits.device == self.topk_w.device and (bias is None or bias.device == logits.device),
-               "route_grouped: logits and bias must be on the plan's device")
+        index = _device_index("route_grouped", logits, bias)
+        _check(index == self.topk_w.get_device(), "route_grouped: logits and bias must be on the plan's device")
         _lib.launch("camhipMoeRouteGrouped", logits.data_ptr(), None if bias is None else bias.data_ptr(), self.T,
                     self.E_route, self.K, _DTYPE[logits.dtype], logits.stride(0) if self.T > 1 else self.E_route, n_group,
                     topk_group, _SCORE[score_func], _GROUP_SCORE[group_score], 1 if renormalize else 0, routed_scaling,
