@@ -3,6 +3,7 @@ import ctypes
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import umdk_amd
 from umdk_amd import _lib
@@ -164,3 +165,20 @@ def test_the_plan_refuses_gradients_and_negated_views():
                               (z(4, 8), z(8), "GPU only")]:
         with pytest.raises(RuntimeError, match=why):
             plan.route_grouped(logits, bias)
+
+
+def test_forward_mode_gradients_are_refused_not_dropped():
+    dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+    plan = MoePrefillPlan(4, 1024, 8, 2, quant_mode=0, device="cpu")
+    with fwd.dual_level():
+        for call in (lambda: umdk_amd.moe_route_grouped(dual(z(4, 8)), None, 2),
+                     lambda: umdk_amd.moe_route_grouped(z(4, 8), dual(z(8)), 2),
+                     lambda: plan.route_grouped(dual(z(4, 8)), None),
+                     lambda: umdk_amd.add_rms_norm(dual(z(4, 8, dtype=bf)), None, z(8)),
+                     lambda: umdk_amd.add_rms_norm(z(4, 8, dtype=bf), None, dual(z(8))),
+                     lambda: umdk_amd.quant_matmul(z(4, 32, dtype=i8), dual(z(4)), z(8, 32, dtype=i8), z(8))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        x = dual(z(4, 8))
+        with torch.inference_mode(), pytest.raises(RuntimeError, match="GPU only"):
+            umdk_amd.moe_route_grouped(x, None, 2)   # nothing is asked for there

@@ -209,3 +209,28 @@ def test_layer_plan_takes_the_gating():
     h, hs = umdk_amd.grouped_matmul_swiglu(ex, sc, n, d["w1"], d["s1"], 2)
     y = umdk_amd.grouped_matmul(h, hs, n, d["w2"], d["s2"])
     assert torch.equal(out, umdk_amd.moe_combine_prefill(y, idx, w, src, rc, "ep", 0, 1))
+
+
+def test_forward_mode_gradients_are_refused():
+    """The tensors are on the GPU, where the native caller takes the call."""
+    fwd = torch.autograd.forward_ad
+    d = make(5)
+    logits = torch.randn(5, 32, device=DEV)
+    q, s, _ = umdk_amd.add_rms_norm(d["x"], d["res"], d["g"], 1e-6, 2)
+    plan = MoePrefillPlan(5, 1024, 32, 4, quant_mode=0)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: umdk_amd.moe_route_grouped(dual(logits), None, 4),
+                     lambda: umdk_amd.moe_route_grouped(logits, dual(d["bias"]), 4),
+                     lambda: plan.route_grouped(dual(logits), None),
+                     lambda: umdk_amd.add_rms_norm(dual(d["x"]), d["res"], d["g"]),
+                     lambda: umdk_amd.add_rms_norm(d["x"], dual(d["res"]), d["g"]),
+                     lambda: umdk_amd.add_rms_norm(d["x"], d["res"], dual(d["g"])),
+                     lambda: umdk_amd.quant_matmul(q, dual(s), d["wd"], d["sd"]),
+                     lambda: umdk_amd.quant_matmul(q, s, d["wd"], dual(d["sd"]))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        x = dual(logits)
+        with torch.inference_mode():   # none is asked for there
+            ids, _ = umdk_amd.moe_route_grouped(x, None, 4)
+        assert torch.equal(ids, umdk_amd.moe_route_grouped(logits, None, 4)[0])

@@ -22,6 +22,7 @@ Differences, all documented in the op docstrings:
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -293,6 +294,11 @@ _SCORE = {"softmax": 0, "sigmoid": 1}
 _GROUP_SCORE = {"max": 1, "top2": 2}
 
 
+def _has_tangent(t):
+    """Whether a forward-mode gradient of t is asked for (requires_grad says nothing of those)."""
+    return torch._C._is_fwd_grad_enabled() and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _refuse(op, tensors):
     """Why _device_index said no."""
     dev = tensors[0].device
@@ -305,16 +311,18 @@ def _refuse(op, tensors):
             raise RuntimeError(f"{op}: a tensor is a negated view; resolve_neg() it")
         if torch.is_grad_enabled() and t.requires_grad:
             raise RuntimeError(f"{op}: no backward; call it under torch.no_grad() or detach its inputs")
+        if _has_tangent(t):
+            raise RuntimeError(f"{op}: no forward-mode gradient; take the primal of its inputs")
     raise _lib.CamHipError(f"{op} runs on the GPU only; got a tensor on {dev}")
 
 
 def _device_index(op, *tensors):
     """What the operators around the expert layer ask of their tensors: one GPU, whose index this is, and no gradient
-    (they have no backward)."""
+    (they have none, backward or forward)."""
     index = tensors[0].get_device()
     grad = torch.is_grad_enabled()
     for t in tensors:
-        if t is not None and (t.get_device() != index or grad and t.requires_grad or t.is_neg()):
+        if t is not None and (t.get_device() != index or grad and t.requires_grad or t.is_neg() or _has_tangent(t)):
             _refuse(op, tensors)
     if index < 0:
         _refuse(op, tensors)
@@ -355,7 +363,8 @@ def moe_route_grouped(logits, bias, topk, n_group=1, topk_group=1, score_func="s
     routed_scaling.  Experts whose logit or bias is -inf (or NaN) are never
     picked; slots left without an expert hold id -1 and weight 0.  logits:
     float32, bfloat16 or float16, rows of any stride; T <= 65536.  No
-    backward: inputs that ask for a gradient are refused in grad mode."""
+    backward: inputs that ask for a gradient are refused in grad mode, those
+    with a forward-mode tangent too."""
     out = (_lib._tensor_caller or _lib._tensors()).route_grouped(logits, bias, topk, n_group, topk_group, score_func,
                                                                  group_score, renormalize, routed_scaling)
     if out is not None:
@@ -415,7 +424,8 @@ def add_rms_norm(x, residual, weight, eps=1e-6, out_quant=0):
     e4m3 y with y_scale [tokens, hidden/128], the transpose of k-major storage
     as grouped_matmul_swiglu reads it.  x may be a column slice of a wider
     tensor (rows of any stride).  No backward: inputs that ask for a gradient
-    (the weight among them) are refused in grad mode."""
+    (the weight among them) are refused in grad mode, those with a
+    forward-mode tangent too."""
     out = (_lib._tensor_caller or _lib._tensors()).add_rms_norm(x, residual, weight, eps, out_quant)
     if out is not None:
         return out

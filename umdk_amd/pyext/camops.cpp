@@ -13,6 +13,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <dlfcn.h>
 #include <torch/csrc/Dtype.h>
@@ -38,6 +39,8 @@ const at::Tensor *plain(PyObject *o)
         return nullptr;
     const at::Tensor &t = THPVariable_Unpack(o);
     if (!t.is_cuda() || t.layout() != at::kStrided || t.is_neg() || (t.requires_grad() && c10::GradMode::is_enabled()))
+        return nullptr;
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())  // (there is level 0 only)
         return nullptr;
     return &t;
 }
