@@ -10,9 +10,10 @@
 // is above all for a (an infinity under a weight of 0 is one), and other infinities meet r = 0.
 //
 // Bound by memory: x, the residual, its sum and the rows pass once, the row in registers from its load to its last store
-// (T = 4096, H = 7168 with a residual: int8 36.4 us = 5.65 TB/s, fp8 39.4, bf16 41.6; T = 32768 bf16 312 us = 6.03 TB/s,
-// where a large copy reaches 4.7; T = 1 3.9 us).  A block per row of 8 waves with 16 columns a thread (4 waves of 32
-// columns: 37.2 us and 4.6 us for one row; 16 waves of 8: 38.6 and 3.75); up to 1024 columns a wave per row.
+// (T = 4096, H = 7168 with a residual, six sets of rows in turn: int8 36.9 us = 5.6 TB/s, fp8 39.8, bf16 41.6; three sets,
+// part of which the last-level cache holds: fp8 37.6; T = 32768 bf16 305 us = 6.2 TB/s, where a large copy reaches 4.7; T = 1
+// 3.9 us).  A block per row of 8 waves with 16 columns a thread (36.4 us int8 when this was chosen; 4 waves of 32 columns:
+// 37.2, and 4.6 for one row; 16 waves of 8: 38.6 and 3.75); up to 1024 columns a wave per row.
 //
 // The norm reads v before it is rounded to 16 bits (the stored residual stream is the rounded one): one rounding per
 // output.

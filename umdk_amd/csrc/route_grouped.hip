@@ -19,8 +19,11 @@
 // has LANES / (number of groups, rounded up to a power of two) lanes.  So the best two of a group are found by a scan of
 // the lane's own experts and log2 of those lanes' steps, all groups at once.
 //
-// Bound by vector instructions where there are many tokens, 45 an expert (65536 tokens, 256 experts, 8 picks: 30 us, where
-// the logits' stream takes 15), and by one token's chain of steps and the launch where there are few (one token 3.8 us).
+// Bound by vector instructions where there are many tokens, 50 an expert (65536 tokens, 256 experts, 8 picks in 4 of 8
+// groups: 33 us, where the logits' stream takes 15), and by one token's chain of steps and the launch where there are few
+// (one token 4.1 us).  Figures of two sides, below, are those that a choice was made on; the scores' rounding and the group
+// sums of whole scores came after most of them and cost both sides up to 0.3 us at few tokens and -4 to 10% at
+// 65536.
 #include "cam_device.h"
 #include "launchers.h"
 
@@ -352,7 +355,6 @@ template <int PER> __device__ __forceinline__ void load_logits(const char *row, 
 // lanes sort their experts and merge their lists of 8.  RG_POP: the lanes sort their experts, each pick is the largest of the
 // lists' heads, and its lane's list moves up.
 enum { RG_EACH, RG_MERGE, RG_POP };
-// (32 experts a lane take 166 registers, three waves of a SIMD; held to 128 they spill: 64 against 33 us at 65536 tokens.)
 // Pick FROM and those behind it, K in all: lane k of a token gets the k-th.
 template <int LANES, int LIST, int FROM> __device__ __forceinline__ void pop_picks(double *key, int K, int rl, double &pick)
 {
@@ -414,6 +416,8 @@ template <int LANES> __device__ __forceinline__ bool keep_group(int KG, int g, d
     }
     return kept;
 }
+// (PER = 32: 156 registers with merges, 164 with heads, three waves of a SIMD; held to 128 they spill: 64 against 33 us at
+// 65536 tokens.)
 template <int LANES, int PER, int PICK>
 __global__ __launch_bounds__(RG_WAVES * 64) void route_grouped_kernel(const RouteGroupedArgs p)
 {
