@@ -416,6 +416,57 @@ CAMHIP_API camhipStatus camhipQuantMatmulGetWorkspaceSize(const void *x, const f
 CAMHIP_API camhipStatus camhipQuantMatmul(void *workspace, uint64_t workspaceSize, camhipExecutor *executor,
                                           void *stream);
 
+/* ------------------------------------------------------------------ a whole expert layer for a few tokens
+ * Extension: what camhipMoeRouteGrouped and camhipFusedDeepMoe do for a decode batch, the router product before them and
+ * the shared expert's addition behind them, for 1 to 16 tokens, which need neither a permutation nor quantised rows.
+ * x [numTokens, hidden] bf16; router [numExperts, hidden] of routerDtype (bf16 or fp32):
+ *   l = x router^T, summed in 64 bits, rounded to fp32;  topkIdx, topkWeights [numTokens, topK] as camhipMoeRouteGrouped
+ *   gives them for the logits l (bias, groups, scoreFunc, groupScore, renormalize, routedScaling as there)
+ *   E_e(x) = W2_e (silu(g) * u),  (g, u) = the halves of W1_e x
+ *   out[t] = sum_k topkWeights[t, k] E_topkIdx[t, k](x_t) + E_shared(x_t), k ascending, rounded once to bf16
+ * in fp32, of the weights' exact values (code * scale): int8 and fp8 quantise the weights alone, the rows stay in 16 bits
+ * (camhipFusedDeepMoe quantises them too, and its results differ by that), and what is between the two products is held
+ * to 2^-16 of itself.  Weights with the reduction dimension contiguous, as camhipMoeExperts takes them: gmm1Weight [numExperts,
+ * gmm1HiddenSize, hidden] (rows [0,I) gate, [I,2I) up), gmm2Weight [numExperts, hidden, I]; weightDtype
+ * CAMHIP_DTYPE_BF16 (no scales), _INT8 (scales [numExperts, gmm1HiddenSize], [numExperts, hidden]) or _FP8 (128x128
+ * block scales [numExperts, n/128, k/128]).  Shared expert (optional): the same for one expert of shareGmm1HiddenSize / 2
+ * columns, of the same type.  xActiveMask [numTokens] bool (1 byte) or NULL: a token that is not active gets ids -1,
+ * weights 0 and a row of zeros.  Slots without an expert (id -1, see camhipMoeRouteGrouped) add nothing.
+ * A token's results are the same bits in any batch.  Limits: numTokens <= 16, hidden <= 8192 and I, the shared one too,
+ * <= 32768, multiples of 64 (fp8: 128); numExperts <= 512, topK <= 16; x and the weights 16-byte aligned, one expert's
+ * weights below 4 GiB. */
+CAMHIP_API camhipStatus camhipMoeDecodeLayerGetWorkspaceSize(
+    const uint16_t *x, const void *router, const float *bias, const void *gmm1Weight, const float *gmm1WeightScale,
+    const void *gmm2Weight, const float *gmm2WeightScale, const void *shareGmm1Weight,
+    const float *shareGmm1WeightScale, const void *shareGmm2Weight, const float *shareGmm2WeightScale,
+    const uint8_t *xActiveMask, int64_t numTokens, int64_t hidden, int64_t numExperts, int64_t gmm1HiddenSize,
+    int64_t shareGmm1HiddenSize, int64_t topK, int64_t weightDtype, int64_t routerDtype, int64_t numGroups,
+    int64_t topkGroups, int64_t scoreFunc, int64_t groupScore, int64_t renormalize, double routedScaling, uint16_t *out,
+    int32_t *topkIdx, float *topkWeights, uint64_t *workspaceSize, camhipExecutor **executor);
+CAMHIP_API camhipStatus camhipMoeDecodeLayer(void *workspace, uint64_t workspaceSize, camhipExecutor *executor,
+                                             void *stream);
+
+/* ------------------------------------------------------------------ low-rank adapters beside a projection
+ * Extension: what each request's adapter adds to a projection that all requests share (camhipQuantMatmul's, say).
+ *   out[t] = base[t] + scaling[a] * B_a (A_a x_t),  a = adapterIds[t];  out[t] = base[t] where a is not in [0, numAdapters)
+ * base [m, n] of baseDtype (bf16, fp16 or fp32), baseRowStride elements between two rows; x [m, k] of xDtype, xRowStride
+ * elements between two rows: loraDtype's, or int8 with xScale [m] (the rows and scales of camhipAddRmsNorm and
+ * camhipQuantMatmul; values code * scale).  loraA [numAdapters, rank, k], loraB [numAdapters, n, rank] of loraDtype (bf16
+ * or fp16); adapters of a lower rank are padded with zeros.  adapterIds [m] in any order; scaling [numAdapters] fp32 or NULL
+ * (ones).  out [m, n] of outDtype (bf16 or fp16), rows contiguous; it may be base itself, where type and stride agree.
+ * Products are exact, sums fp32, A x in between is held to 2^-16 of itself (fp16: 2^-21 of the row's largest), one rounding
+ * at the end.
+ * Limits: m <= 2^20, n <= 2^20, k a multiple of 16 and at most 131056, rank a multiple of 8 and at most 256, numAdapters
+ * <= 65536; loraA and loraB 16-byte aligned (x may start anywhere; rows on 16 bytes are the fast ones). */
+CAMHIP_API camhipStatus camhipLoraAddGetWorkspaceSize(const void *base, const void *x, const float *xScale,
+                                                      const void *loraA, const void *loraB, const int32_t *adapterIds,
+                                                      const float *scaling, int64_t m, int64_t n, int64_t k,
+                                                      int64_t rank, int64_t numAdapters, int64_t baseRowStride,
+                                                      int64_t xRowStride, int64_t baseDtype, int64_t xDtype,
+                                                      int64_t loraDtype, int64_t outDtype, void *out,
+                                                      uint64_t *workspaceSize, camhipExecutor **executor);
+CAMHIP_API camhipStatus camhipLoraAdd(void *workspace, uint64_t workspaceSize, camhipExecutor *executor, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -35,6 +35,8 @@ SIGNATURES = {
     "camhipMoeRouteGrouped": "pp iiiiiiiiii d ppp",
     "camhipAddRmsNorm": "ppp iiiiii d ppp",
     "camhipQuantMatmul": "ppppp iiii p",
+    "camhipMoeDecodeLayer": "pppppppppppp iiiiiiiiiiiii d ppp",
+    "camhipLoraAdd": "ppppppp iiiiiiiiiii p",
 }
 
 _lib = None

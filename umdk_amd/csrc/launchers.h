@@ -77,6 +77,45 @@ struct QmmArgs {
 static_assert(sizeof(QmmArgs) + 2 * sizeof(int) <= LAUNCH_ARGS, "a cheap launch");
 hipError_t launch_quant_matmul(const QmmArgs &a, hipStream_t s);
 
+// ---- a whole expert layer for a few tokens (moe_decode.hip)
+enum MoeDecodeWeight { MD_BF16 = 0, MD_INT8 = 2, MD_FP8 = 3 };  // the CAMHIP_DTYPE_* codes
+constexpr int MD_MAX_TOKENS = 16, MD_MAX_HIDDEN = 8192, MD_MAX_INTER = 32768;
+struct MoeDecodeArgs {
+    const uint16_t *x;          // [T, H] bf16
+    const void *router;         // [E, H] bf16, or fp32 (router_fp32)
+    const float *bias;          // [E] or nullptr
+    const uint8_t *active;      // [T] or nullptr
+    const void *w1, *w2;        // [E, 2 I, H], [E, H, I]
+    const float *s1, *s2;       // int8: [E, 2 I], [E, H]; fp8: [E, 2 I / 128, H / 128], [E, H / 128, I / 128]
+    const void *sw1, *sw2;      // the shared expert's, or nullptr
+    const float *ss1, *ss2;
+    uint16_t *out;              // [T, H] bf16
+    int32_t *topk_idx;          // [T, K]
+    float *topk_w;
+    int T, H, E, I, Is, K;      // Is: 0 without a shared expert
+    int G, KG, score, group_top2, renorm, router_fp32, wtype;
+    float scaling;
+};
+size_t moe_decode_workspace_bytes(const MoeDecodeArgs &a);
+hipError_t launch_moe_decode(const MoeDecodeArgs &a, void *ws, hipStream_t s);
+
+// ---- low-rank adapters beside a projection (lora.hip)
+enum LoraDtype { LORA_BF16 = 0, LORA_FP16 = 1, LORA_INT8 = 2, LORA_FP32 = 4 };  // the CAMHIP_DTYPE_* codes
+struct LoraArgs {
+    const void *base;           // [M, N], rows base_stride elements apart
+    const void *x;              // [M, K], rows x_stride elements apart
+    const float *xs;            // [M], int8 rows only
+    const void *a, *b;          // [L, R, K], [L, N, R]
+    const int32_t *ids;         // [M]
+    const float *scaling;       // [L] or nullptr
+    void *out;                  // [M, N]
+    int64_t M, base_stride, x_stride;
+    int N, K, R, L;
+    int8_t base_dtype, x_dtype, dtype, out_dtype;
+};
+size_t lora_workspace_bytes(const LoraArgs &a);
+hipError_t launch_lora_add(const LoraArgs &a, void *ws, hipStream_t s);
+
 // ---- dispatch layout (layout.hip)
 struct LayoutPlan {
     int tokens_per_chunk;

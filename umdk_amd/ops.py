@@ -17,7 +17,8 @@ Differences, all documented in the op docstrings:
     FP8 e4m3fn rows with [rows, hidden/128] fp32 block scales.
   * moe_route (routing) and grouped expert GEMM ops are additions with no
     reference counterpart, and so are the operators around the expert layer:
-    moe_route_grouped, add_rms_norm and quant_matmul.
+    moe_route_grouped, add_rms_norm and quant_matmul, and those of a decode
+    step of a few requests: moe_decode_layer and lora_add.
 """
 import weakref
 
@@ -50,6 +51,13 @@ _def.define("add_rms_norm(Tensor x, Tensor? residual, Tensor weight, float eps=1
             "-> (Tensor, Tensor, Tensor)")
 _def.define("quant_matmul(Tensor x, Tensor x_scale, Tensor weight, Tensor weight_scale, Tensor? bias=None, "
             "ScalarType? out_dtype=None) -> Tensor")
+_def.define("moe_decode_layer(Tensor x, Tensor router, Tensor? bias, Tensor gmm1_weight, Tensor? gmm1_weight_scale, "
+            "Tensor gmm2_weight, Tensor? gmm2_weight_scale, int topk, int n_group=1, int topk_group=1, "
+            "str score_func='softmax', str group_score='top2', bool renormalize=True, float routed_scaling=1.0, "
+            "Tensor? share_gmm1_weight=None, Tensor? share_gmm1_weight_scale=None, Tensor? share_gmm2_weight=None, "
+            "Tensor? share_gmm2_weight_scale=None, Tensor? x_active_mask=None) -> (Tensor, Tensor, Tensor)")
+_def.define("lora_add(Tensor base, Tensor x, Tensor lora_a, Tensor lora_b, Tensor adapter_ids, Tensor? scaling=None, "
+            "Tensor? x_scale=None, ScalarType? out_dtype=None) -> Tensor")
 
 _def.define(
     "fused_deep_moe(Tensor x, Tensor expert_ids, Tensor[] gmm1_weight, Tensor[] gmm1_weight_scale, "
@@ -485,6 +493,190 @@ def quant_matmul(x, x_scale, weight, weight_scale, bias=None, out_dtype=None):
     return out
 
 
+def _run_ws(name, index, *args):
+    """_run() of an entry point with a workspace, allocated on GPU `index`."""
+    with torch.cuda.device(index):
+        _lib.call(name, *args, device=torch.device("cuda", index), stream=torch._C._cuda_getCurrentRawStream(index))
+
+
+_WEIGHT_DTYPE = {torch.bfloat16: 0, torch.int8: 2, torch.float8_e4m3fn: 3}  # CAMHIP_DTYPE_*
+MAX_DECODE_TOKENS = 16
+
+
+def _weight_scale_check(scale, weight, what):
+    """A weight [..., n, k] and its scales: none (bf16), [..., n] (int8), [..., n/128, k/128] (fp8)."""
+    if weight.dtype == torch.bfloat16:
+        _check(scale is None, f"moe_decode_layer: bf16 {what} takes no scales")
+        return
+    _check(scale is not None, f"moe_decode_layer: {what}_scale missing")
+    n, k = weight.shape[-2:]
+    want = (n,) if weight.dtype == torch.int8 else (n // 128, k // 128)
+    _check(scale.dtype == torch.float32 and tuple(scale.shape) == tuple(weight.shape[:-2]) + want and scale.is_contiguous(),
+           f"moe_decode_layer: {what}_scale must be float32 {list(weight.shape[:-2]) + list(want)}, contiguous")
+
+
+def _moe_decode_check(x, router, bias, w1, s1, w2, s2, topk, score_func, group_score, sw1, ss1, sw2, ss2, mask):
+    op = "moe_decode_layer"
+    _check(x.dim() == 2 and x.dtype == torch.bfloat16 and x.is_contiguous(),
+           f"{op}: x must be [tokens, hidden] bfloat16, contiguous")
+    T, H = x.shape
+    _check(T <= MAX_DECODE_TOKENS, f"{op}: at most {MAX_DECODE_TOKENS} tokens (got {T}); moe_route_grouped and "
+           "fused_deep_moe take larger batches")
+    _check(router.dim() == 2 and router.dtype in (torch.float32, torch.bfloat16) and router.is_contiguous()
+           and router.shape[1] == H, f"{op}: router must be [experts, hidden] float32 or bfloat16, contiguous")
+    E = router.shape[0]
+    _check(bias is None or bias.dtype == torch.float32 and bias.shape == (E,) and bias.is_contiguous(),
+           f"{op}: bias must be [experts] float32")
+    _check(w1.dtype in _WEIGHT_DTYPE, f"{op}: weights must be bfloat16, int8 or float8_e4m3fn")
+    _check(w1.dim() == 3 and w1.is_contiguous() and w1.shape[0] == E and w1.shape[2] == H and w1.shape[1] % 2 == 0,
+           f"{op}: gmm1_weight must be [experts, 2 I, hidden], contiguous")
+    I = w1.shape[1] // 2
+    _check(w2.dtype == w1.dtype and w2.shape == (E, H, I) and w2.is_contiguous(),
+           f"{op}: gmm2_weight must be [experts, hidden, I] of gmm1_weight's dtype, contiguous")
+    _weight_scale_check(s1, w1, "gmm1_weight")
+    _weight_scale_check(s2, w2, "gmm2_weight")
+    _check((sw1 is None) == (sw2 is None), f"{op}: share_gmm1_weight and share_gmm2_weight come together")
+    Is = 0
+    if sw1 is not None:
+        _check(sw1.dtype == w1.dtype and sw1.dim() == 2 and sw1.is_contiguous() and sw1.shape[1] == H
+               and sw1.shape[0] % 2 == 0 and sw1.shape[0] > 0,
+               f"{op}: share_gmm1_weight must be [2 Is, hidden] of gmm1_weight's dtype, contiguous")
+        Is = sw1.shape[0] // 2
+        _check(sw2.dtype == w1.dtype and sw2.shape == (H, Is) and sw2.is_contiguous(),
+               f"{op}: share_gmm2_weight must be [hidden, Is] of gmm1_weight's dtype, contiguous")
+        _weight_scale_check(ss1, sw1, "share_gmm1_weight")
+        _weight_scale_check(ss2, sw2, "share_gmm2_weight")
+    else:
+        _check(ss1 is None and ss2 is None, f"{op}: share scales without share weights")
+    _check(mask is None or mask.dtype == torch.bool and mask.shape == (T,) and mask.is_contiguous(),
+           f"{op}: x_active_mask must be [tokens] bool")
+    if score_func not in _SCORE:
+        raise RuntimeError(f"{op}: score_func must be 'softmax' or 'sigmoid' (got {score_func!r})")
+    if group_score not in _GROUP_SCORE:
+        raise RuntimeError(f"{op}: group_score must be 'max' or 'top2' (got {group_score!r})")
+    return T, H, E, I, Is
+
+
+def moe_decode_layer(x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weight, gmm2_weight_scale, topk, n_group=1,
+                     topk_group=1, score_func="softmax", group_score="top2", renormalize=True, routed_scaling=1.0,
+                     share_gmm1_weight=None, share_gmm1_weight_scale=None, share_gmm2_weight=None,
+                     share_gmm2_weight_scale=None, x_active_mask=None):
+    """A whole expert layer for 1 to 16 tokens (addition; no reference
+    counterpart): router product, grouped routing, GMM1 + SwiGLU, GMM2,
+    weighted sum and shared expert in two launches.  Returns (out [T,H]
+    bfloat16, topk_idx [T,K] int32, topk_weights [T,K] fp32).
+
+    The logits are x router^T, summed in 64 bits and rounded to fp32, and are
+    routed as moe_route_grouped routes them (bias, n_group, topk_group,
+    score_func, group_score, renormalize, routed_scaling as there).
+    out[t] = sum_k w[t,k] W2_e (silu(g) * u) + the shared expert's, with
+    (g, u) = W1_e x_t, in fp32 and rounded once.  Weights [E, 2I, H] and
+    [E, H, I] (shared: [2Is, H] and [H, Is]) with the reduction dimension
+    contiguous: bfloat16; int8 with scales per channel [E, 2I] and [E, H];
+    float8_e4m3fn with scales for 128x128 blocks.  Unlike fused_deep_moe, the
+    rows stay in 16 bits whatever the weights' type.  x_active_mask [T] bool:
+    tokens that are not active get ids -1, weights 0 and rows of zeros.  A
+    token's results are the same bits in any batch.  No backward: inputs that
+    ask for a gradient are refused in grad mode, those with a forward-mode
+    tangent too."""
+    T, H, E, I, Is = _moe_decode_check(x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weight, gmm2_weight_scale,
+                                       topk, score_func, group_score, share_gmm1_weight, share_gmm1_weight_scale,
+                                       share_gmm2_weight, share_gmm2_weight_scale, x_active_mask)
+    tensors = (x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weight, gmm2_weight_scale, share_gmm1_weight,
+               share_gmm1_weight_scale, share_gmm2_weight, share_gmm2_weight_scale, x_active_mask)
+    index = _device_index("moe_decode_layer", *tensors)
+    out = torch.empty_like(x)
+    idx = x.new_empty((T, topk), dtype=torch.int32)
+    w = x.new_empty((T, topk), dtype=torch.float32)
+    p = [None if t is None else t.data_ptr() for t in tensors]
+    _run_ws("camhipMoeDecodeLayer", index, *p, T, H, E, 2 * I, 2 * Is, topk, _WEIGHT_DTYPE[gmm1_weight.dtype],
+            _DTYPE[router.dtype], n_group, topk_group, _SCORE[score_func], _GROUP_SCORE[group_score],
+            1 if renormalize else 0, routed_scaling, out.data_ptr(), idx.data_ptr(), w.data_ptr())
+    return out, idx, w
+
+
+def _lora_check(base, x, a, b, ids, scaling, x_scale, out_dtype):
+    op = "lora_add"
+    _check(x.dim() == 2 and base.dim() == 2 and base.shape[0] == x.shape[0],
+           f"{op}: base must be [m, n] and x [m, k]")
+    m, k = x.shape
+    n = base.shape[1]
+    _check(base.dtype in _DTYPE, f"{op}: base must be float32, bfloat16 or float16")
+    _check(a.dim() == 3 and a.dtype in (torch.bfloat16, torch.float16) and a.is_contiguous() and a.shape[2] == k,
+           f"{op}: lora_a must be [adapters, rank, k] bfloat16 or float16, contiguous")
+    L, r, _ = a.shape
+    _check(b.dtype == a.dtype and b.shape == (L, n, r) and b.is_contiguous(),
+           f"{op}: lora_b must be [adapters, n, rank] of lora_a's dtype, contiguous")
+    _check(ids.shape == (m,) and ids.dtype in (torch.int32, torch.int64), f"{op}: adapter_ids must be [m] int32 or int64")
+    _check(scaling is None or scaling.dtype == torch.float32 and scaling.shape == (L,),
+           f"{op}: scaling must be [adapters] float32")
+    if x.dtype == torch.int8:
+        _check(x_scale is not None and x_scale.dtype == torch.float32 and x_scale.shape == (m,),
+               f"{op}: int8 x needs x_scale, float32 [m] (per token)")
+    else:
+        _check(x.dtype == a.dtype, f"{op}: x must be int8 or of lora_a's dtype")
+        _check(x_scale is None, f"{op}: x_scale without int8 x")
+    if out_dtype is None:
+        out_dtype = a.dtype if base.dtype == torch.float32 else base.dtype
+    _check(out_dtype in (torch.bfloat16, torch.float16), f"{op}: out_dtype must be bfloat16 or float16")
+    return m, n, k, L, r, out_dtype
+
+
+def lora_add(base, x, lora_a, lora_b, adapter_ids, scaling=None, x_scale=None, out_dtype=None):
+    """The low-rank adapters of many requests beside a projection that they
+    share (addition; no reference counterpart): out[t] = base[t] +
+    scaling[a] * lora_b[a] (lora_a[a] x_t) with a = adapter_ids[t]; rows whose
+    id is outside [0, adapters) (-1, say) keep base[t].
+
+    base [m, n]: the projection's output, float32 (quant_matmul(...,
+    out_dtype=torch.float32): the sum is then rounded once), bfloat16 or
+    float16, rows of any stride.  x [m, k]: the projection's input, of
+    lora_a's dtype (rows of any stride), or int8 with x_scale [m] as
+    add_rms_norm(out_quant=2) gives them.  lora_a [adapters, rank, k], lora_b
+    [adapters, n, rank] bfloat16 or float16, rank a multiple of 8 (lower ranks
+    padded with zeros).  adapter_ids [m] int32 (int64 is cast), any order.
+    out [m, n] in out_dtype (by default base's, lora_a's for a float32 base).
+    No backward: inputs that ask for a gradient are refused in grad mode,
+    those with a forward-mode tangent too."""
+    m, n, k, L, r, out_dtype = _lora_check(base, x, lora_a, lora_b, adapter_ids, scaling, x_scale, out_dtype)
+    index = _device_index("lora_add", base, x, lora_a, lora_b, adapter_ids, scaling, x_scale)
+
+    def rows(t, width):  # rows of contiguous elements, and the elements between two
+        step, one = t.stride()
+        if one != 1 and width > 1 or m > 1 and step < width:
+            return t.contiguous(), width
+        return t, step if m > 1 else width
+
+    bs, b_step = rows(base, n)
+    xr, x_step = rows(x, k)
+    with torch.cuda.device(index):
+        # (ids past 32 bits stay outside [0, adapters))
+        ids = (adapter_ids if adapter_ids.dtype == torch.int32 else adapter_ids.clamp(-1, L).to(torch.int32)).contiguous()
+        sc = None if scaling is None else scaling.contiguous()
+        xs = None if x_scale is None else x_scale.contiguous()
+    out = base.new_empty((m, n), dtype=out_dtype)
+    _run_ws("camhipLoraAdd", index, bs.data_ptr(), xr.data_ptr(), None if xs is None else xs.data_ptr(),
+            lora_a.data_ptr(), lora_b.data_ptr(), ids.data_ptr(), None if sc is None else sc.data_ptr(), m, n, k, r, L,
+            b_step, x_step, _DTYPE[base.dtype], 2 if x.dtype == torch.int8 else _DTYPE[x.dtype], _DTYPE[lora_a.dtype],
+            _DTYPE[out_dtype], out.data_ptr())
+    return out
+
+
+def moe_decode_layer_meta(x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weight, gmm2_weight_scale, topk,
+                          n_group=1, topk_group=1, score_func="softmax", group_score="top2", renormalize=True,
+                          routed_scaling=1.0, share_gmm1_weight=None, share_gmm1_weight_scale=None,
+                          share_gmm2_weight=None, share_gmm2_weight_scale=None, x_active_mask=None):
+    T = _moe_decode_check(x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weight, gmm2_weight_scale, topk,
+                          score_func, group_score, share_gmm1_weight, share_gmm1_weight_scale, share_gmm2_weight,
+                          share_gmm2_weight_scale, x_active_mask)[0]
+    return torch.empty_like(x), x.new_empty((T, topk), dtype=torch.int32), x.new_empty((T, topk), dtype=torch.float32)
+
+
+def lora_add_meta(base, x, lora_a, lora_b, adapter_ids, scaling=None, x_scale=None, out_dtype=None):
+    m, n, _, _, _, out_dtype = _lora_check(base, x, lora_a, lora_b, adapter_ids, scaling, x_scale, out_dtype)
+    return base.new_empty((m, n), dtype=out_dtype)
+
+
 def moe_route_grouped_meta(logits, bias, topk, n_group=1, topk_group=1, score_func="softmax", group_score="top2",
                            renormalize=True, routed_scaling=1.0):
     T, _ = _route_grouped_check(logits, bias, topk, n_group, topk_group, score_func, group_score)
@@ -781,6 +973,10 @@ _impl.impl("moe_route", moe_route)
 _impl.impl("moe_route_grouped", moe_route_grouped)
 _impl.impl("add_rms_norm", add_rms_norm)
 _impl.impl("quant_matmul", quant_matmul)
+_impl.impl("moe_decode_layer", moe_decode_layer)
+_impl.impl("lora_add", lora_add)
 _meta.impl("moe_route_grouped", moe_route_grouped_meta)
 _meta.impl("add_rms_norm", add_rms_norm_meta)
 _meta.impl("quant_matmul", quant_matmul_meta)
+_meta.impl("moe_decode_layer", moe_decode_layer_meta)
+_meta.impl("lora_add", lora_add_meta)

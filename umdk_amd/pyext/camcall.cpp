@@ -131,7 +131,9 @@ PyObject *entry(const char *name, camhipStatus (*get)(P...), RunFn run, PyObject
     X(camhipMoeExperts)                                                                                              \
     X(camhipMoeRouteGrouped)                                                                                         \
     X(camhipAddRmsNorm)                                                                                              \
-    X(camhipQuantMatmul)
+    X(camhipQuantMatmul)                                                                                             \
+    X(camhipMoeDecodeLayer)                                                                                          \
+    X(camhipLoraAdd)
 
 #define DEFINE(f)                                                                                                    \
     decltype(&f##GetWorkspaceSize) get_##f = nullptr;                                                                \
