@@ -1,155 +1,838 @@
-// A whole expert layer for 1 to 16 tokens.  With x the tokens' rows, R the router, b the balance bias:
+// A whole expert layer for 1 to 16 tokens, in two launches.  With x the tokens' rows, R the router, b the balance bias:
 //   l = x R^T;  ids, gates = grouped routing of l (route_grouped.hip)
 //   E_e(x) = W2_e (silu(g) * u),  (g, u) = halves of W1_e x
 //   out[t] = sum_k gates[t, k] E_ids[t, k](x_t) + E_shared(x_t)
-// Products of the weights' exact values, fp32 sums, one rounding at the end.
-#include "cam_device.h"
-#include "launchers.h"
+// The first kernel computes the logits.  In the second every block routes all tokens for itself (16 tokens are two a wave),
+// and then streams weights.
+//
+// What bounds it is the stream of the weights of the experts that any token picked, each read once.  So the layout serves
+// that stream: a wave multiplies 16 weight rows by all tokens at once (the tokens are the 16 columns of one matrix
+// instruction: no permutation, no gathered rows; columns of tokens that did not pick the expert are never looked at), and
+// what it multiplies them by stays in registers: the wave's share of x for all experts, of h = silu(g) * u for one.  The 8 waves
+// of a block share a sum's products by units of 128 bytes of a weight row, each with a ring of 8 units in registers that is
+// refilled, unit by unit, as it is used, past the ends of tiles and work items.  So some 128 KB are in flight on a CU all the
+// time; matrix and vector instructions are a tenth of what they could be.
+//
+// Work items are numbered, those of the first product (16 gate rows and their 16 up rows) before those of the second (some
+// 16-row tiles of one expert), and blocks take them in that order from a counter.  An item of the second product waits until
+// the expert's h is whole.  That cannot lock: what it waits for are items with lower numbers, taken by blocks that run and
+// never wait themselves, however many blocks the GPU holds at once and whatever else it runs.
+//
+// Sums are fp32 in an order that hangs on the shapes alone: a token's results are the same bits in any batch, on any
+// schedule.  Each (token, pick) gets its own row of partial results; whoever adds the last one to a tile of the output sums
+// them up, picks ascending.  h is held as two bf16 numbers, of which the second is what the first leaves out (2^-16 in
+// all): one would add 2^-8 roundings of I values to the result's own, and the matrix instructions for the second are free.
+#include <atomic>
+#include <type_traits>
+
+#include "route_dev.h"
 
 namespace cam {
 
 namespace {
 
-// ---------------------------------------------------------------- the router product
-// Logits in 64 bits, rounded to fp32: which expert is picked must not hang on the order of a sum.  A block per expert, its
-// waves take turns at runs of 512 columns; products of 16-bit values (and of those with fp32) are exact in 64 bits.
-constexpr int MD_ROUTER_WAVES = 4;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
-__global__ __launch_bounds__(MD_ROUTER_WAVES * 64) void moe_decode_router_kernel(const MoeDecodeArgs p, float *logits)
+// ---------------------------------------------------------------- sizes
+constexpr int MD_WAVES = 8, MD_RING = 7, MD_BLOCKS = 256;
+constexpr int MD_SLOT = 2048;  // bytes of a slot of the ring: 16 rows by 128 bytes
+constexpr int MD_BATCH = 4;    // tiles of a wave between two meetings of the waves
+constexpr int MD_MAX_PICKS = 16, MD_MAX_EXPERTS = 512, MD_MAX_ENTRIES = MD_MAX_TOKENS * MD_MAX_PICKS + 1;
+// The longest run of h that a work item of the second product multiplies by: what 128 registers hold of it (both numbers).
+constexpr int MD_CHUNK = 4096;
+// Counters in the workspace, 64 bytes apart: the queue, the experts' h (finished pairs of tiles), the output's tiles.
+constexpr int MD_CTR = 16, MD_CTR_READY = 1, MD_CTR_DONE = MD_CTR_READY + MD_MAX_ENTRIES;
+constexpr int MD_COUNTERS = MD_CTR_DONE + MD_MAX_HIDDEN / 16;
+constexpr uint32_t MD_OUT = 0x80000000u;  // an offset past every buffer here: loads give 0, stores nothing
+constexpr int AUX_NT = 2, AUX_AGENT = 16;
+
+struct Ws {
+    int *ctr;
+    float *logits;           // [T, E]
+    uint16_t *h, *h_low;     // [T, K + 1, width]
+    float *part;             // [T, K + 1, chunks, H]
+    uint32_t h_bytes, part_bytes;
+};
+struct Layout {
+    size_t logits, h, h_low, part, total;
+    uint32_t h_bytes, part_bytes;
+    int width, chunks;
+};
+int md_chunks(int I) { return (I + MD_CHUNK - 1) / MD_CHUNK; }
+Layout md_layout(const MoeDecodeArgs &a)
+{
+    const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    Layout l;
+    l.width = a.I > a.Is ? a.I : a.Is;
+    l.chunks = md_chunks(l.width);
+    l.h_bytes = (uint32_t)((size_t)a.T * (a.K + 1) * l.width * 2);
+    l.part_bytes = (uint32_t)((size_t)a.T * (a.K + 1) * l.chunks * a.H * 4);
+    l.logits = up((size_t)MD_COUNTERS * MD_CTR * 4);
+    l.h = l.logits + up((size_t)a.T * a.E * 4);
+    l.h_low = l.h + up(l.h_bytes);
+    l.part = l.h_low + up(l.h_bytes);
+    l.total = l.part + up(l.part_bytes);
+    return l;
+}
+
+// ---------------------------------------------------------------- the router product
+// Logits in 64 bits, rounded to fp32: which expert is picked must not hang on the order of a sum.  A block per expert, 16
+// columns a thread, so that all loads are on their way at once; products of 16-bit values (and of those with fp32) are
+// exact in 64 bits.  The kernel also clears the counters of the next one.
+constexpr int MD_ROUTER_WAVES = 8, MD_ROUTER_RUNS = MD_MAX_HIDDEN / (MD_ROUTER_WAVES * 512);
+
+struct RouterArgs {
+    const uint16_t *x;
+    const void *router;
+    const uint8_t *active;
+    float *logits;
+    int *ctr;
+    int T, E, H, router_fp32;
+};
+
+__global__ __launch_bounds__(MD_ROUTER_WAVES * 64) void moe_decode_router_kernel(const RouterArgs p)
 {
     const int e = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     __shared__ double part[MD_ROUTER_WAVES][MD_MAX_TOKENS];
-    for (int t = 0; t < p.T; ++t) {
-        double sum = 0.0;
-        for (int k = (w * 64 + lane) * 8; k < p.H; k += MD_ROUTER_WAVES * 512) {
-            float xf[8], rf[8];
-            unpack_bf16x8(*reinterpret_cast<const u32x4 *>(p.x + (size_t)t * p.H + k), xf);
+    float r[MD_ROUTER_RUNS][8];
+    const int k0 = threadIdx.x * 8;
+#pragma unroll
+    for (int i = 0; i < MD_ROUTER_RUNS; ++i) {
+        const int k = k0 + i * MD_ROUTER_WAVES * 512;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            r[i][j] = 0.0f;
+        if (k < p.H) {
             if (p.router_fp32) {
-                const float *r = reinterpret_cast<const float *>(p.router) + (size_t)e * p.H + k;
+                const f32x4 *v = reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(p.router) + (size_t)e * p.H + k);
+                const f32x4 a = v[0], b = v[1];
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    rf[j] = r[j];
+                    r[i][j] = j < 4 ? a[j & 3] : b[j & 3];
             } else {
-                unpack_bf16x8(*reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(p.router) + (size_t)e * p.H + k), rf);
+                unpack_bf16x8(*reinterpret_cast<const u32x4 *>(reinterpret_cast<const uint16_t *>(p.router) + (size_t)e * p.H + k), r[i]);
             }
+        }
+    }
+    for (int i = e * MD_ROUTER_WAVES * 64 + threadIdx.x; i < MD_COUNTERS; i += p.E * MD_ROUTER_WAVES * 64)
+        p.ctr[i * MD_CTR] = 0;
+    for (int t = 0; t < p.T; ++t) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < MD_ROUTER_RUNS; ++i) {
+            const int k = k0 + i * MD_ROUTER_WAVES * 512;
+            u32x4 v = u32x4{0, 0, 0, 0};
+            if (k < p.H)
+                v = *reinterpret_cast<const u32x4 *>(p.x + (size_t)t * p.H + k);
+            float x[8];
+            unpack_bf16x8(v, x);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                sum = __builtin_fma((double)xf[j], (double)rf[j], sum);
+                sum = __builtin_fma((double)x[j], (double)r[i][j], sum);
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            sum += __shfl_xor(sum, o, 64);
+        sum = row_sum<64>(sum);
         if (lane == 0)
             part[w][t] = sum;
     }
     __syncthreads();
-    if (threadIdx.x < p.T) {
+    if ((int)threadIdx.x < p.T) {
         double sum = 0.0;
+#pragma unroll
         for (int v = 0; v < MD_ROUTER_WAVES; ++v)
             sum += part[v][threadIdx.x];
-        const bool on = !p.active || p.active[threadIdx.x];
-        logits[(size_t)threadIdx.x * p.E + e] = on ? (float)sum : __builtin_nanf("");
+        const bool on = !p.active || p.active[threadIdx.x];  // (a token without a logit has no experts)
+        p.logits[(size_t)threadIdx.x * p.E + e] = on ? (float)sum : __builtin_nanf("");
     }
 }
 
-// ---------------------------------------------------------------- the experts, one output at a time
-template <int WT> __device__ __forceinline__ float weight(const void *w, size_t at)
+// ---------------------------------------------------------------- the experts
+// A weight type: bytes of a value, values of a unit, matrix instructions (32 values deep) of a unit.
+template <int WT> struct Weight {
+    static constexpr int SIZE = WT == MD_BF16 ? 2 : 1, UNIT = 128 / SIZE, STEPS = UNIT / 32;
+};
+// the s-th 8 values (s < STEPS / 2) of 16 bytes, as bf16: exact
+template <int WT> __device__ __forceinline__ bf16x8 values(const u32x4 v, int s)
 {
-    if constexpr (WT == MD_BF16)
-        return bf16_to_f32(reinterpret_cast<const uint16_t *>(w)[at]);
-    else if constexpr (WT == MD_INT8)
-        return (float)reinterpret_cast<const int8_t *>(w)[at];
-    else
-        return __builtin_amdgcn_cvt_f32_fp8((int)reinterpret_cast<const uint8_t *>(w)[at], 0);
-}
-// row n of a matrix of rows of k: the dot product with v, in this wave
-template <int WT, typename V>
-__device__ __forceinline__ float row_dot(const void *w, const float *s, size_t n, int k, int blocks_k, V v)
-{
-    const int lane = threadIdx.x & 63;
-    float sum = 0.0f;
-    for (int j = lane; j < k; j += 64) {
-        float q = weight<WT>(w, n * k + j);
-        if constexpr (WT == MD_FP8)
-            q *= s[n / 128 * blocks_k + j / 128];
-        sum = __builtin_fmaf(q, v(j), sum);
-    }
+    if constexpr (WT == MD_BF16) {
+        return __builtin_bit_cast(bf16x8, v);
+    } else {
+        u32x4 r;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        sum += __shfl_xor(sum, o, 64);
-    if constexpr (WT == MD_INT8)
-        sum *= s[n];
-    return sum;
-}
-
-template <int WT> __global__ __launch_bounds__(256) void moe_decode_gmm1_kernel(const MoeDecodeArgs p, float *h, int width)
-{
-    const int slots = p.K + (p.Is > 0), t = blockIdx.y / slots, k = blockIdx.y % slots;
-    const bool shared = k == p.K;
-    const int I = shared ? p.Is : p.I, i = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int e = shared ? 0 : p.topk_idx[t * p.K + k];
-    if (i >= I || e < 0)
-        return;
-    const size_t per = (size_t)2 * I * p.H * (WT == MD_BF16 ? 2 : 1);
-    const size_t per_s = WT == MD_INT8 ? 2 * I : (size_t)(2 * I / 128) * (p.H / 128);
-    const void *w = shared ? p.sw1 : (const char *)p.w1 + e * per;
-    const float *s = WT == MD_BF16 ? nullptr : shared ? p.ss1 : p.s1 + e * per_s;
-    const auto x = [&](int j) { return bf16_to_f32(p.x[(size_t)t * p.H + j]); };
-    const float g = row_dot<WT>(w, s, i, p.H, p.H / 128, x), u = row_dot<WT>(w, s, I + i, p.H, p.H / 128, x);
-    if ((threadIdx.x & 63) == 0)
-        h[(size_t)blockIdx.y * width + i] = g / (1.0f + __expf(-g)) * u;
-}
-
-template <int WT> __global__ __launch_bounds__(256) void moe_decode_gmm2_kernel(const MoeDecodeArgs p, const float *h, int width)
-{
-    const int slots = p.K + (p.Is > 0), t = blockIdx.y, n = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= p.H)
-        return;
-    float sum = 0.0f;
-    for (int k = 0; k < slots; ++k) {
-        const bool shared = k == p.K;
-        const int I = shared ? p.Is : p.I, e = shared ? 0 : p.topk_idx[t * p.K + k];
-        if (e < 0 || (shared && p.active && !p.active[t]))
-            continue;
-        const size_t per = (size_t)I * p.H * (WT == MD_BF16 ? 2 : 1);
-        const size_t per_s = WT == MD_INT8 ? p.H : (size_t)(I / 128) * (p.H / 128);
-        const void *w = shared ? p.sw2 : (const char *)p.w2 + e * per;
-        const float *s = WT == MD_BF16 ? nullptr : shared ? p.ss2 : p.s2 + e * per_s;
-        const float *row = h + (size_t)(t * slots + k) * width;
-        const float y = row_dot<WT>(w, s, n, I, I / 128, [&](int j) { return row[j]; });
-        sum = shared ? sum + y : __builtin_fmaf(p.topk_w[t * p.K + k], y, sum);
+        for (int q = 0; q < 2; ++q) {
+            const uint32_t d = v[2 * s + q];
+            if constexpr (WT == MD_FP8) {
+                r[2 * q] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, false));
+                r[2 * q + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(d, 1.0f, true));
+            } else {
+                r[2 * q] = f32x2_to_bf16x2((float)(int8_t)d, (float)(int8_t)(d >> 8));
+                r[2 * q + 1] = f32x2_to_bf16x2((float)(int8_t)(d >> 16), (float)(int8_t)(d >> 24));
+            }
+        }
+        return __builtin_bit_cast(bf16x8, r);
     }
-    if ((threadIdx.x & 63) == 0)
-        p.out[(size_t)t * p.H + n] = (uint16_t)(f32x2_to_bf16x2(sum, 0.0f) & 0xffffu);
 }
 
-size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
-
-template <int WT> hipError_t run(const MoeDecodeArgs &a, float *h, int width, hipStream_t s)
+__device__ __forceinline__ rsrc_t rsrc(const void *p, uint32_t bytes)
 {
-    const int slots = a.K + (a.Is > 0);
-    hipLaunchKernelGGL(moe_decode_gmm1_kernel<WT>, dim3((width + 3) / 4, a.T * slots), dim3(256), 0, s, a, h, width);
-    hipLaunchKernelGGL(moe_decode_gmm2_kernel<WT>, dim3((a.H + 3) / 4, a.T), dim3(256), 0, s, a, (const float *)h, width);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)bytes, 0x00020000);
+}
+// 16 bytes for each lane from r + off + at, into LDS at lds + 16 lane, past the caches: weights are read once
+__device__ __forceinline__ void dma(rsrc_t r, uint32_t off, uint32_t at, uint8_t *lds)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, off, at, 0, AUX_NT);
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+template <typename T> __device__ __forceinline__ T *uniform(T *p)
+{
+    const uint64_t u = (uint64_t)p;
+    return (T *)((uint64_t)(uint32_t)uniform((int)(u >> 32)) << 32 | (uint32_t)uniform((int)(uint32_t)u));
+}
+template <typename T> __device__ __forceinline__ __attribute__((address_space(1))) T *gp(T *p)
+{
+    return (__attribute__((address_space(1))) T *)p;
+}
+__device__ __forceinline__ int ctr_add(int *p, int v)
+{
+    return __hip_atomic_fetch_add(gp(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ int ctr_load(int *p)
+{
+    return __hip_atomic_load(gp(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void lds_barrier()  // a barrier that leaves loads in flight
+{
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+struct DecodeArgs {
+    MoeDecodeArgs p;
+    RouteGroupedArgs r;  // one token's routing by a wave
+    int route_per, width, chunks;
+    Ws ws;
+};
+
+// A work item.  phase 1: a pair of 16-row tiles (gate, up) of an entry's first matrix; 2: `count` tiles of a chunk of its
+// second; 0: none.
+struct Item {
+    int phase, entry, tile, count;
+    int lkw, k0, units, chunk;  // log2 of the waves that share a tile's sum; the chunk's first unit, its units
+    uint32_t row_bytes, step;   // step: rows from a gate tile to its up tile, or from a wave's tile to its next one
+    const char *w;
+    const float *s;             // the matrix's scales
+};
+
+// What the streams need of the arguments, in LDS: in scalar registers it would crowd out what they work with.
+struct Late {
+    const void *w1, *w2, *sw1, *sw2;
+    const float *s1, *s2, *ss1, *ss2;
+    uint16_t *out, *h, *h_low;
+    float *part;
+    int *ctr;
+    int I, Is, K, width, chunks;
+    uint32_t h_bytes, part_bytes;
+};
+
+// LDS.  red: what the waves have summed up of their tiles.
+struct Shared {
+    uint8_t ring[MD_WAVES][MD_RING][MD_SLOT];
+    f32x4 red[MD_WAVES][MD_BATCH][64];
+    uint32_t expert_mask[MD_MAX_EXPERTS];
+    int16_t expert_entry[MD_MAX_EXPERTS];
+    int16_t ids[MD_MAX_TOKENS][MD_MAX_PICKS];
+    float gates[MD_MAX_TOKENS][MD_MAX_PICKS];
+    int16_t entry_expert[MD_MAX_ENTRIES];
+    uint16_t entry_mask[MD_MAX_ENTRIES];
+    uint8_t entry_pick[MD_MAX_ENTRIES][MD_MAX_TOKENS];
+    int wave_count[MD_WAVES], known;
+    Item item[2];
+    Late a;
+};
+static_assert(sizeof(Shared) <= 160 * 1024, "a CU's LDS");
+
+// at most N of this wave's memory operations are in flight
+template <int N> __device__ __forceinline__ void wait_loads()
+{
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | 0xF70);
+    asm volatile("" ::: "memory");
+}
+// the oldest of `ahead` slots' loads, two each, has arrived
+template <int MOST> __device__ __forceinline__ void wait_slot(int ahead)
+{
+    if constexpr (MOST <= 1) {
+        wait_loads<0>();
+    } else {
+        if (ahead >= MOST)
+            wait_loads<2 * (MOST - 1)>();
+        else
+            wait_slot<MOST - 1>(ahead);
+    }
+}
+
+template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_kernel(const DecodeArgs args)
+{
+    using W = Weight<WT>;
+    constexpr int PIECES = 16 / W::SIZE / 8;               // steps of 16 bytes
+    constexpr int U1 = MD_MAX_HIDDEN / W::UNIT / MD_WAVES;  // a wave's units of a row of the first matrix at most
+    constexpr int U2 = MD_CHUNK / W::UNIT / MD_WAVES;       // and of a chunk of the second
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    Shared &sh = *reinterpret_cast<Shared *>(smem);
+    const Late &a = sh.a;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4;
+    const int w = uniform((int)threadIdx.x >> 6);
+    const int T = args.p.T, H = args.p.H;
+    const bool nshared = args.p.Is > 0;
+
+    // The last wave is the block's clerk: it takes the tickets and says what their items are.  (The first two are on their way
+    // while the tokens are routed, by other waves where there are few.)
+    const bool clerk = w == MD_WAVES - 1;
+    int ticket = 0, ticket2 = 0;
+    if (clerk && lane == 0) {
+        ticket = ctr_add(args.ws.ctr, 1);
+        ticket2 = ctr_add(args.ws.ctr, 1);
+    }
+    int entries;
+    uint32_t on;  // the tokens that are active
+    {
+        const MoeDecodeArgs &p = args.p;
+        const int K = p.K;
+        // ---- routing
+        for (int i = threadIdx.x; i < MD_MAX_EXPERTS; i += MD_WAVES * 64)
+            sh.expert_mask[i] = 0;
+        for (int t = w; t < T; t += MD_WAVES) {
+            int idx = -1;
+            double gate = 0.0;
+            const char *row = reinterpret_cast<const char *>(args.ws.logits + (size_t)t * p.E);
+            if (args.route_per == 4)
+                route_token<64, 4, RG_EACH>(args.r, row, lane, idx, gate);
+            else
+                route_token<64, 16, RG_EACH>(args.r, row, lane, idx, gate);
+            if (lane < K) {
+                const float g = (float)(gate * (double)p.scaling);
+                sh.ids[t][lane] = (int16_t)idx;
+                sh.gates[t][lane] = g;
+                if (blockIdx.x == 0) {
+                    p.topk_idx[t * K + lane] = idx;
+                    p.topk_w[t * K + lane] = g;
+                }
+            }
+        }
+        if (threadIdx.x == MD_WAVES * 64 - 1)
+            sh.a = Late{p.w1,  p.w2, p.sw1, p.sw2, p.s1, p.s2,       p.ss1,       p.ss2,          p.out,          args.ws.h, args.ws.h_low,
+                        args.ws.part, args.ws.ctr, p.I, p.Is, p.K, args.width, args.chunks, args.ws.h_bytes, args.ws.part_bytes};
+        __syncthreads();
+        if ((int)threadIdx.x < T * K) {
+            const int t = threadIdx.x / K, e = sh.ids[t][threadIdx.x % K];
+            if (e >= 0)
+                atomicOr(&sh.expert_mask[e], 1u << t);
+        }
+        __syncthreads();
+        // the entries: the shared expert, then the experts that any token picked, ascending
+        const uint32_t mask = sh.expert_mask[threadIdx.x];  // (as many threads as experts at most)
+        const uint64_t some = __ballot(mask != 0);
+        if (lane == 0)
+            sh.wave_count[w] = __popcll(some);
+        __syncthreads();
+        int before = nshared, all = nshared;
+#pragma unroll
+        for (int v = 0; v < MD_WAVES; ++v) {
+            before += v < w ? sh.wave_count[v] : 0;
+            all += sh.wave_count[v];
+        }
+        if (mask) {
+            const int d = before + __popcll(some & lanemask_lt());
+            sh.entry_expert[d] = (int16_t)threadIdx.x;
+            sh.entry_mask[d] = (uint16_t)mask;
+            sh.expert_entry[threadIdx.x] = (int16_t)d;
+        }
+        on = (1u << T) - 1;
+        if (p.active)
+            on = (uint32_t)__ballot(lane < T && p.active[min(lane, T - 1)]);
+        if (nshared && threadIdx.x == 0)
+            sh.entry_mask[0] = (uint16_t)on;
+        __syncthreads();
+        if ((int)threadIdx.x < T * K) {
+            const int t = threadIdx.x / K, k = threadIdx.x % K, e = sh.ids[t][k];
+            if (e >= 0)
+                sh.entry_pick[sh.expert_entry[e]][t] = (uint8_t)k;
+        }
+        if (nshared && (int)threadIdx.x < T)
+            sh.entry_pick[0][threadIdx.x] = (uint8_t)K;
+        entries = uniform(all);
+        if (entries == 0) {  // nobody has an expert
+            for (int i = blockIdx.x * MD_WAVES * 64 + threadIdx.x; i < T * H / 4; i += gridDim.x * MD_WAVES * 64)
+                reinterpret_cast<u32x2 *>(p.out)[i] = u32x2{0, 0};
+            return;
+        }
+    }
+
+    // ---- the items
+    const uint32_t row1 = (uint32_t)(H * W::SIZE);  // bytes of a row of the first matrix
+    const auto chunks_of = [](int I) { return (I + MD_CHUNK - 1) / MD_CHUNK; };
+    // the item of the clerk's ticket, for all to read
+    const auto describe = [&](int slot) {
+        const int q = uniform(ticket), I0 = uniform(a.I), Is = uniform(a.Is);
+        const int per1 = I0 / 16, per1s = nshared ? Is / 16 : 0, N1 = per1s + (entries - nshared) * per1;
+        Item it{};
+        if (q < N1) {
+            const bool shared = q < per1s;
+            const int I = shared ? Is : I0, at = q - per1s, d = shared ? 0 : nshared + at / per1;
+            const int e = shared ? 0 : uniform(sh.entry_expert[d]);
+            it.phase = 1;
+            it.entry = d;
+            it.tile = shared ? q : at % per1;
+            it.count = 2;
+            it.lkw = 3;
+            it.units = ((int)row1 + 127) / 128;
+            it.row_bytes = row1;
+            it.step = (uint32_t)I;
+            it.w = reinterpret_cast<const char *>(shared ? a.sw1 : a.w1) + (size_t)e * (size_t)(2 * I) * row1;
+            if constexpr (WT == MD_FP8)
+                it.s = (shared ? a.ss1 : a.s1) + (size_t)e * (2 * I / 128) * (H / 128);
+            if constexpr (WT == MD_INT8)
+                it.s = (shared ? a.ss1 : a.s1) + (size_t)e * 2 * I;
+        } else {
+            const int C0 = chunks_of(I0), Cs = nshared ? chunks_of(Is) : 0, parts = Cs + (entries - nshared) * C0;
+            int run = H / 16 * parts / (MD_BLOCKS + MD_BLOCKS / 2);  // tiles of an item: some items for every block
+            run = run >= 8 ? 8 : run >= 4 ? 4 : run >= 2 ? 2 : 1;
+            const int runs = (H / 16 + run - 1) / run, c = (q - N1) / runs;
+            if (c < parts) {
+                const bool shared = c < Cs;
+                const int I = shared ? Is : I0, C = shared ? Cs : C0, d = shared ? 0 : nshared + (c - Cs) / C0;
+                const int e = shared ? 0 : uniform(sh.entry_expert[d]);
+                const int units = (I * W::SIZE + 127) / 128, cu = (units + C - 1) / C;
+                it.phase = 2;
+                it.entry = d;
+                it.chunk = shared ? c : (c - Cs) % C0;
+                it.tile = (q - N1) % runs * run;
+                it.count = min(run, H / 16 - it.tile);
+                it.lkw = cu > 4 ? 3 : cu > 2 ? 2 : cu > 1 ? 1 : 0;
+                it.k0 = it.chunk * cu;
+                it.units = min(cu, units - it.k0);
+                it.row_bytes = (uint32_t)(I * W::SIZE);
+                it.step = 128u >> it.lkw;
+                it.w = reinterpret_cast<const char *>(shared ? a.sw2 : a.w2) + (size_t)e * (size_t)H * it.row_bytes;
+                if constexpr (WT == MD_FP8)
+                    it.s = (shared ? a.ss2 : a.s2) + (size_t)e * (H / 128) * (I / 128);
+                if constexpr (WT == MD_INT8)
+                    it.s = (shared ? a.ss2 : a.s2) + (size_t)e * H;
+            }
+        }
+        if (lane == 0)
+            sh.item[slot] = it;
+    };
+    const auto read_item = [&](int slot) -> Item {
+        const Item &v = sh.item[slot];
+        Item it;
+        it.phase = uniform(v.phase);
+        it.entry = uniform(v.entry);
+        it.tile = uniform(v.tile);
+        it.count = uniform(v.count);
+        it.lkw = uniform(v.lkw);
+        it.k0 = uniform(v.k0);
+        it.units = uniform(v.units);
+        it.chunk = uniform(v.chunk);
+        it.row_bytes = (uint32_t)uniform((int)v.row_bytes);
+        it.step = (uint32_t)uniform((int)v.step);
+        it.w = uniform(v.w);
+        it.s = uniform(v.s);
+        return it;
+    };
+    const auto take = [&] {
+        if (clerk && lane == 0)
+            ticket = ctr_add(a.ctr, 1);
+    };
+    // this wave's share of an item: units of a tile, tiles
+    const auto units_of = [&](const Item &it) { return (it.units - (w & ((1 << it.lkw) - 1)) + (1 << it.lkw) - 1) >> it.lkw; };
+    const auto tiles_of = [&](const Item &it) {
+        const int wr = w >> it.lkw, at_once = 8 >> it.lkw;
+        return it.phase == 0 ? 0 : (it.count - wr + at_once - 1) >> (3 - it.lkw);
+    };
+
+    // ---- the ring.  A load instruction brings 8 rows by 128 bytes (whole cache lines): lane l 16 bytes of row l / 8, into
+    // the l-th 16 bytes of half a slot.  Which 16 of the row's 128: l mod 8, turned by (row / 2) mod 8, so that the 16 rows of
+    // an operand fall on different banks.
+    uint8_t *const my_ring = sh.ring[w][0];
+    const int turned = (lane & 7) ^ (lane >> 4), frag = l16 * 128 + ((lq ^ (l16 >> 1)) << 4);
+    int ahead = 0, in_slot = 0, out_slot = 0;  // slots filled or being filled; the next to fill, to use
+    struct {                                   // what the next slot to fill holds
+        const char *w;
+        uint32_t off, first, tile_step, unit_step, row_bytes;
+        int units, unit, tiles;                // tiles: left, with this one
+        uint32_t lane_off;
+        int which;                             // 0: of the current item, 1: of the next, 2: of one not yet known
+    } in;
+    const auto stream = [&](const Item &it) {
+        in.units = units_of(it);
+        in.tiles = in.units > 0 ? tiles_of(it) : 0;
+        in.unit = 0;
+        in.row_bytes = it.row_bytes;
+        in.w = it.w;
+        in.unit_step = 128u << it.lkw;
+        in.first = (uint32_t)(it.k0 + (w & ((1 << it.lkw) - 1))) * 128u;
+        in.off = (uint32_t)(it.tile * 16 + (it.phase == 2 ? (w >> it.lkw) * 16 : 0)) * it.row_bytes + in.first;
+        in.tile_step = it.step * it.row_bytes;
+        in.lane_off = (uint32_t)(lane >> 3) * it.row_bytes;
+    };
+    Item cur, nxt;
+    const auto fill = [&] {  // (in.tiles > 0, ahead < MD_RING)
+        const rsrc_t r = rsrc(in.w, 0xffffffffu);
+        uint8_t *lds = my_ring + in_slot * MD_SLOT;
+        int c0 = turned, c1 = turned ^ 4;
+        if (WT == MD_INT8 && in.first + in.unit * in.unit_step + 64 >= in.row_bytes) {  // (a row may end within a unit)
+            c0 &= 3;
+            c1 &= 3;
+        }
+        const uint32_t at = in.off + in.unit * in.unit_step;
+        dma(r, in.lane_off + c0 * 16, at, lds);
+        dma(r, in.lane_off + 8 * in.row_bytes + c1 * 16, at, lds + 1024);
+        in_slot = in_slot == MD_RING - 1 ? 0 : in_slot + 1;
+        ++ahead;
+        if (++in.unit == in.units) {
+            in.unit = 0;
+            in.off += in.tile_step;
+            if (--in.tiles == 0 && in.which == 0) {
+                in.which = 1;
+                stream(nxt);
+            }
+        }
+    };
+    const auto top_up = [&] {
+        while (ahead < MD_RING && in.tiles > 0)
+            fill();
+    };
+    // the next slot's products with x, or with both numbers of h, added to acc; the slot is filled again
+    const auto use = [&](const u32x4 *x, const u32x4 *x_low, float s, bool half, f32x4 &acc) {
+        wait_slot<MD_RING>(ahead);
+        const uint8_t *at = my_ring + out_slot * MD_SLOT;
+        u32x4 v[2];
+        v[0] = *reinterpret_cast<const u32x4 *>(at + frag);
+        v[1] = *reinterpret_cast<const u32x4 *>(at + (frag ^ 64));
+        asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(v[0]), "+v"(v[1])::"memory");  // (the slot has been read)
+        out_slot = out_slot == MD_RING - 1 ? 0 : out_slot + 1;
+        --ahead;
+        if (in.tiles > 0)
+            fill();
+        if (WT == MD_INT8 && half)
+            v[1] = u32x4{0, 0, 0, 0};
+        f32x4 sum = WT == MD_FP8 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc;
+#pragma unroll
+        for (int i = 0; i < W::STEPS; ++i) {
+            const bf16x8 b = values<WT>(v[i / PIECES], i % PIECES);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, __builtin_bit_cast(bf16x8, x[i]), sum, 0, 0, 0);
+            if (x_low)
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, __builtin_bit_cast(bf16x8, x_low[i]), sum, 0, 0, 0);
+        }
+        if constexpr (WT == MD_FP8) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                acc[q] = __builtin_fmaf(s, sum[q], acc[q]);
+        } else {
+            acc = sum;
+        }
+    };
+    const auto scale = [&](const float *s, int at) {  // (by a scalar load)
+        return reinterpret_cast<const __attribute__((address_space(4))) float *>((uintptr_t)s)[at];
+    };
+
+    if (clerk) {
+        describe(0);
+        ticket = ticket2;
+        describe(1);
+    }
+    __syncthreads();
+    cur = read_item(0);
+    nxt = read_item(1);
+    int turn = 0;  // the place of the current item, where the one after the next goes
+    in.which = 0;
+    stream(cur);
+    if (in.tiles == 0) {
+        in.which = 1;
+        stream(nxt);
+    }
+    const auto advance = [&] {
+        cur = nxt;
+        nxt = read_item(turn);
+        turn ^= 1;
+        in.which = in.which == 0 ? 0 : in.which - 1;
+        if (in.tiles == 0) {  // (all of the item that is now the current one has been asked for)
+            in.which = 1;
+            stream(nxt);
+        }
+        top_up();
+    };
+
+    // ---- the first product
+    if (cur.phase == 1) {
+        const int units = units_of(cur);  // the same for all of these items
+        top_up();
+        // the wave's share of x: 32 columns each
+        u32x4 x[U1 * W::STEPS];
+        {
+            const rsrc_t rx = rsrc(args.p.x, (uint32_t)(T * H * 2));
+#pragma unroll
+            for (int i = 0; i < U1 * W::STEPS; ++i)
+                x[i] = u32x4{0, 0, 0, 0};
+            if (l16 < T) {  // (lanes that ask for nothing cost nothing)
+#pragma unroll
+                for (int i = 0; i < U1 * W::STEPS; ++i) {
+                    const int st = i % W::STEPS, col = (w + i / W::STEPS * 8) * W::UNIT + (16 / W::SIZE) * (4 * (st / PIECES) + lq) + 8 * (st % PIECES);
+                    x[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, col < H ? (l16 * H + col) * 2 : MD_OUT, 0, 0);
+                }
+            }
+        }
+        wait_loads<0>();
+        while (cur.phase == 1) {
+            take();
+            float s[2][U1];  // the scales of the gate rows and of the up rows
+            if constexpr (WT == MD_FP8) {
+#pragma unroll
+                for (int u = 0; u < U1; ++u) {
+                    const int at = min(w + 8 * u, H / 128 - 1);
+                    s[0][u] = scale(cur.s, (cur.tile >> 3) * (H / 128) + at);
+                    s[1][u] = scale(cur.s, ((cur.tile + (int)cur.step / 16) >> 3) * (H / 128) + at);
+                }
+            }
+            f32x4 acc[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < U1; ++u)
+                    if (u < units)
+                        use(x + u * W::STEPS, nullptr, WT == MD_FP8 ? s[j][u] : 0.f, (uint32_t)(w + 8 * u) * 128 + 64 >= row1, acc[j]);
+            }
+            if (clerk)
+                describe(turn);
+            lds_barrier();  // (the last sums have been read)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                sh.red[w][j][lane] = acc[j];
+            lds_barrier();
+            if (w == (cur.tile & 7)) {  // another one each time
+                f32x4 g = f32x4{0.f, 0.f, 0.f, 0.f}, u = g;
+#pragma unroll
+                for (int v = 0; v < MD_WAVES; ++v) {
+                    g += sh.red[v][0][lane];
+                    u += sh.red[v][1][lane];
+                }
+                const int i0 = cur.tile * 16 + lq * 4;
+                if constexpr (WT == MD_INT8) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        g[q] *= cur.s[i0 + q];
+                        u[q] *= cur.s[cur.step + i0 + q];
+                    }
+                }
+                f32x4 h, low;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    h[q] = g[q] / (1.0f + __expf(-g[q])) * u[q];
+                const u32x2 hi = u32x2{f32x2_to_bf16x2(h[0], h[1]), f32x2_to_bf16x2(h[2], h[3])};
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    low[q] = h[q] - bf16_to_f32((hi[q >> 1] >> (16 * (q & 1))) & 0xffffu);
+                const u32x2 lo = u32x2{f32x2_to_bf16x2(low[0], low[1]), f32x2_to_bf16x2(low[2], low[3])};
+                if (l16 < T && (sh.entry_mask[cur.entry] >> l16 & 1)) {
+                    const size_t at = (size_t)(l16 * (a.K + 1) + sh.entry_pick[cur.entry][l16]) * a.width + i0;
+                    __hip_atomic_store(gp(reinterpret_cast<uint64_t *>(a.h + at)), __builtin_bit_cast(uint64_t, hi), __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(gp(reinterpret_cast<uint64_t *>(a.h_low + at)), __builtin_bit_cast(uint64_t, lo),
+                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                wait_loads<0>();
+                if (lane == 0)
+                    ctr_add(a.ctr + (MD_CTR_READY + cur.entry) * MD_CTR, 1);
+            }
+            advance();
+        }
+    }
+
+    // ---- the second product
+    top_up();
+    bool gave_up = false;
+    int known = 0;  // the entries below have their h
+    while (cur.phase == 2) {
+        take();
+        const int slots = uniform(a.K) + 1, per_tile = 8 >> cur.lkw;  // tiles at once, by the waves' shares
+        const int units = units_of(cur), wk = w & ((1 << cur.lkw) - 1);
+        const uint32_t mask = sh.entry_mask[cur.entry];
+        const int pick = sh.entry_pick[cur.entry][l16];
+        const bool mine = mask >> l16 & 1;  // this lane's token has the expert
+        float s[U2];
+        if constexpr (WT == MD_FP8) {  // (an item's tiles are of one block of rows)
+#pragma unroll
+            for (int u = 0; u < U2; ++u)
+                s[u] = scale(cur.s, (cur.tile >> 3) * (int)(cur.row_bytes / 128) + min(cur.k0 + wk + 8 * u, (int)(cur.row_bytes / 128) - 1));
+        }
+        // h of the entry, once all of it has been written.  One wave looks, at 64 entries at once.
+        if (cur.entry >= known) {
+            if (w == 0) {
+                const uint64_t t0 = wall_clock64();
+                const int d = min(known + lane, entries - 1), want = (nshared && d == 0 ? a.Is : a.I) / 16;
+                int to;
+                for (;;) {
+                    const uint64_t not_yet = __ballot(ctr_load(a.ctr + (MD_CTR_READY + d) * MD_CTR) < want);
+                    to = known + (not_yet ? __builtin_ctzll(not_yet) : 64);
+                    if (to > cur.entry)
+                        break;
+                    if (wall_clock64() - t0 > 200000000ull) {  // 2 s: no launch that has the workspace to itself waits so long
+                        to = -1;
+                        break;
+                    }
+                    __builtin_amdgcn_s_sleep(4);
+                }
+                if (lane == 0)
+                    sh.known = to;
+            }
+            lds_barrier();
+            known = uniform(sh.known);
+            if (known < 0) {
+                gave_up = true;
+                known = MD_MAX_ENTRIES + 64;
+            }
+        }
+        asm volatile("" ::: "memory");
+        u32x4 h[U2 * W::STEPS], low[U2 * W::STEPS];
+        {
+            const rsrc_t rh = rsrc(uniform(a.h), uniform((int)a.h_bytes)), rl = rsrc(uniform(a.h_low), uniform((int)a.h_bytes));
+            const uint32_t row = (uint32_t)((l16 * slots + pick) * a.width);
+            const int limit = (int)(cur.row_bytes / W::SIZE);
+#pragma unroll
+            for (int u = 0; u < U2 * W::STEPS; ++u)
+                h[u] = low[u] = u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < U2; ++u)
+                if (u < units && mine) {
+#pragma unroll
+                    for (int st = 0; st < W::STEPS; ++st) {
+                        const int col = (cur.k0 + wk + u * 8) * W::UNIT + (16 / W::SIZE) * (4 * (st / PIECES) + lq) + 8 * (st % PIECES);
+                        const uint32_t off = col < limit ? (row + col) * 2 : MD_OUT;
+                        h[u * W::STEPS + st] = __builtin_amdgcn_raw_buffer_load_b128(rh, off, 0, AUX_AGENT);
+                        low[u * W::STEPS + st] = __builtin_amdgcn_raw_buffer_load_b128(rl, off, 0, AUX_AGENT);
+                    }
+                }
+            wait_loads<0>();  // (once here, not for every use below)
+        }
+        const rsrc_t rp = rsrc(uniform(a.part), uniform((int)a.part_bytes));
+        const int chunks = uniform(a.chunks), C0 = chunks_of(uniform(a.I)), Cs = nshared ? chunks_of(uniform(a.Is)) : 0;
+        const int tiles = units > 0 ? tiles_of(cur) : 0;
+        for (int t0 = 0; t0 < cur.count; t0 += MD_BATCH * per_tile) {  // t0: the batch's first tile
+            const int j0 = t0 >> (3 - cur.lkw);
+            const bool last_batch = t0 + MD_BATCH * per_tile >= cur.count;
+            f32x4 acc[MD_BATCH];
+#pragma unroll
+            for (int j = 0; j < MD_BATCH; ++j) {
+                acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (j0 + j < tiles) {
+#pragma unroll
+                    for (int u = 0; u < U2; ++u)
+                        if (u < units)
+                            use(h + u * W::STEPS, low + u * W::STEPS, WT == MD_FP8 ? s[u] : 0.f,
+                                (uint32_t)(cur.k0 + wk + 8 * u) * 128 + 64 >= cur.row_bytes, acc[j]);
+                }
+            }
+            lds_barrier();  // (the last sums have been read)
+#pragma unroll
+            for (int j = 0; j < MD_BATCH; ++j)
+                sh.red[w][j][lane] = acc[j];
+            if (clerk && last_batch)
+                describe(turn);
+            lds_barrier();
+            // tile v of the batch is the (v / per_tile)-th of the 2^lkw waves from (v mod per_tile) 2^lkw on; another wave each
+            // time adds them up
+            for (int v = (w + cur.tile) & 7; v < min(MD_BATCH * per_tile, cur.count - t0); v += MD_WAVES) {
+                const int from = (v & (per_tile - 1)) << cur.lkw, j = v >> (3 - cur.lkw);
+                f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int k = 0; k < min(1 << cur.lkw, cur.units); ++k)
+                    y += sh.red[from + k][j][lane];
+                const int tile = cur.tile + t0 + v, n = tile * 16 + lq * 4;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    if constexpr (WT == MD_INT8)
+                        y[q] *= cur.s[n + q];
+                    if (gave_up)
+                        y[q] = __builtin_nanf("");
+                }
+                const uint32_t at = (uint32_t)(((l16 * slots + pick) * chunks + cur.chunk) * H + n) * 4u;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rp, mine ? at : MD_OUT, 0, AUX_AGENT);
+                wait_loads<0>();
+                int before = 0;
+                if (lane == 0)
+                    before = ctr_add(a.ctr + (MD_CTR_DONE + tile) * MD_CTR, 1);
+                before = uniform(before);
+                asm volatile("" ::: "memory");
+                if (before + 1 == Cs + (entries - nshared) * C0) {  // every part of this tile of the output is there
+                    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+                    const int t = min(l16, T - 1);
+                    for (int k = 0; k < slots; ++k) {
+                        const bool shared = k + 1 == slots;
+                        if (shared && !nshared)
+                            break;
+                        const bool have = shared ? on >> t & 1 : sh.ids[t][k] >= 0;
+                        const float gate = shared ? 1.0f : sh.gates[t][k];
+                        const int C = shared ? Cs : C0;
+                        f32x4 e = f32x4{0.f, 0.f, 0.f, 0.f};
+                        for (int c = 0; c < C; ++c)
+                            e += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                     rp, have ? (uint32_t)(((t * slots + k) * chunks + c) * H + n) * 4u : MD_OUT, 0, AUX_AGENT));
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            o[q] = have ? __builtin_fmaf(gate, e[q], o[q]) : o[q];
+                    }
+                    if (l16 < T)
+                        *reinterpret_cast<u32x2 *>(a.out + (size_t)t * H + n) =
+                            u32x2{f32x2_to_bf16x2(o[0], o[1]), f32x2_to_bf16x2(o[2], o[3])};
+                }
+            }
+        }
+        advance();
+    }
+}
+
+constexpr int MD_MAX_DEVICES = 64;
+
+template <int WT> hipError_t run(const DecodeArgs &a, hipStream_t s)
+{
+    static std::atomic<bool> done[MD_MAX_DEVICES];  // the kernel's dynamic LDS limit is raised once per device
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && !(dev < MD_MAX_DEVICES && done[dev].load(std::memory_order_acquire))) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&moe_decode_kernel<WT>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                (int)sizeof(Shared));
+        if (e == hipSuccess && dev < MD_MAX_DEVICES)
+            done[dev].store(true, std::memory_order_release);
+    }
+    if (e != hipSuccess)
+        return e;
+    hipLaunchKernelGGL(moe_decode_kernel<WT>, dim3(MD_BLOCKS), dim3(MD_WAVES * 64), sizeof(Shared), s, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t moe_decode_workspace_bytes(const MoeDecodeArgs &a)
-{
-    const size_t width = a.I > a.Is ? a.I : a.Is;
-    return align256((size_t)a.T * a.E * 4) + align256((size_t)a.T * (a.K + 1) * width * 4);
-}
+size_t moe_decode_workspace_bytes(const MoeDecodeArgs &a) { return md_layout(a).total; }
 
 hipError_t launch_moe_decode(const MoeDecodeArgs &a, void *ws, hipStream_t s)
 {
     if (a.T == 0)
         return hipSuccess;
-    float *logits = reinterpret_cast<float *>(ws);
-    float *h = reinterpret_cast<float *>((char *)ws + align256((size_t)a.T * a.E * 4));
-    hipLaunchKernelGGL(moe_decode_router_kernel, dim3(a.E), dim3(MD_ROUTER_WAVES * 64), 0, s, a, logits);
-    RouteGroupedArgs r{};
-    r.logits = logits;
+    const Layout l = md_layout(a);
+    DecodeArgs d{};
+    d.p = a;
+    d.width = l.width;
+    d.chunks = l.chunks;
+    d.ws.ctr = reinterpret_cast<int *>(ws);
+    d.ws.logits = reinterpret_cast<float *>((char *)ws + l.logits);
+    d.ws.h = reinterpret_cast<uint16_t *>((char *)ws + l.h);
+    d.ws.h_low = reinterpret_cast<uint16_t *>((char *)ws + l.h_low);
+    d.ws.part = reinterpret_cast<float *>((char *)ws + l.part);
+    d.ws.h_bytes = l.h_bytes;
+    d.ws.part_bytes = l.part_bytes;
+    RouteGroupedArgs &r = d.r;
     r.row_bytes = (int64_t)a.E * 4;
     r.bias = a.bias;
     r.T = a.T;
@@ -161,20 +844,20 @@ hipError_t launch_moe_decode(const MoeDecodeArgs &a, void *ws, hipStream_t s)
     r.group_top2 = a.group_top2;
     r.renorm = a.renorm;
     r.dtype = ROUTE_FP32;
-    r.scaling = a.scaling;
-    r.topk_idx = a.topk_idx;
-    r.topk_w = a.topk_w;
-    hipError_t e = launch_route_grouped(r, s);
-    if (e != hipSuccess)
-        return e;
-    const int width = a.I > a.Is ? a.I : a.Is;
+    const int per = route_shares(r, 64);
+    d.route_per = per <= 4 ? 4 : 16;
+    if (per > 16)
+        return hipErrorInvalidValue;
+    route_places(r, 64, d.route_per);
+    const RouterArgs ra{a.x, a.router, a.active, d.ws.logits, d.ws.ctr, a.T, a.E, a.H, a.router_fp32};
+    hipLaunchKernelGGL(moe_decode_router_kernel, dim3(a.E), dim3(MD_ROUTER_WAVES * 64), 0, s, ra);
     switch (a.wtype) {
     case MD_BF16:
-        return run<MD_BF16>(a, h, width, s);
+        return run<MD_BF16>(d, s);
     case MD_INT8:
-        return run<MD_INT8>(a, h, width, s);
+        return run<MD_INT8>(d, s);
     case MD_FP8:
-        return run<MD_FP8>(a, h, width, s);
+        return run<MD_FP8>(d, s);
     }
     return hipErrorInvalidValue;
 }
