@@ -117,23 +117,35 @@ __global__ __launch_bounds__(MD_ROUTER_WAVES * 64) void moe_decode_router_kernel
     }
     for (int i = e * MD_ROUTER_WAVES * 64 + threadIdx.x; i < MD_COUNTERS; i += p.E * MD_ROUTER_WAVES * 64)
         p.ctr[i * MD_CTR] = 0;
-    for (int t = 0; t < p.T; ++t) {
-        double sum = 0.0;
+    constexpr int AT_ONCE = 4;
+    for (int t0 = 0; t0 < p.T; t0 += AT_ONCE) {
+        u32x4 v[AT_ONCE][MD_ROUTER_RUNS];
 #pragma unroll
-        for (int i = 0; i < MD_ROUTER_RUNS; ++i) {
-            const int k = k0 + i * MD_ROUTER_WAVES * 512;
-            u32x4 v = u32x4{0, 0, 0, 0};
-            if (k < p.H)
-                v = *reinterpret_cast<const u32x4 *>(p.x + (size_t)t * p.H + k);
-            float x[8];
-            unpack_bf16x8(v, x);
+        for (int t = 0; t < AT_ONCE; ++t)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                sum = __builtin_fma((double)x[j], (double)r[i][j], sum);
+            for (int i = 0; i < MD_ROUTER_RUNS; ++i) {
+                const int k = k0 + i * MD_ROUTER_WAVES * 512;
+                v[t][i] = u32x4{0, 0, 0, 0};
+                if (t0 + t < p.T && k < p.H)
+                    v[t][i] = *reinterpret_cast<const u32x4 *>(p.x + (size_t)(t0 + t) * p.H + k);
+            }
+#pragma unroll
+        for (int t = 0; t < AT_ONCE; ++t) {
+            if (t0 + t < p.T) {
+                double sum = 0.0;
+#pragma unroll
+                for (int i = 0; i < MD_ROUTER_RUNS; ++i) {
+                    float x[8];
+                    unpack_bf16x8(v[t][i], x);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        sum = __builtin_fma((double)x[j], (double)r[i][j], sum);
+                }
+                sum = row_sum<64>(sum);
+                if (lane == 0)
+                    part[w][t0 + t] = sum;
+            }
         }
-        sum = row_sum<64>(sum);
-        if (lane == 0)
-            part[w][t] = sum;
     }
     __syncthreads();
     if ((int)threadIdx.x < p.T) {
@@ -252,6 +264,17 @@ struct Shared {
 };
 static_assert(sizeof(Shared) <= 160 * 1024, "a CU's LDS");
 
+// f(0), f(1), ... f(n - 1) with constants, n <= N.  (One jump past the rest: code that is only skipped costs its fetch.)
+template <int N, int I = 0, typename F> __device__ __forceinline__ void upto(int n, F &&f)
+{
+    if constexpr (I < N) {
+        if (I < n) {
+            f(std::integral_constant<int, I>{});
+            upto<N, I + 1>(n, f);
+        }
+    }
+}
+
 // at most N of this wave's memory operations are in flight
 template <int N> __device__ __forceinline__ void wait_loads()
 {
@@ -306,7 +329,9 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
             int idx = -1;
             double gate = 0.0;
             const char *row = reinterpret_cast<const char *>(args.ws.logits + (size_t)t * p.E);
-            if (args.route_per == 4)
+            if (args.route_per == 1)
+                route_token<64, 1, RG_EACH>(args.r, row, lane, idx, gate);
+            else if (args.route_per == 4)
                 route_token<64, 4, RG_EACH>(args.r, row, lane, idx, gate);
             else
                 route_token<64, 16, RG_EACH>(args.r, row, lane, idx, gate);
@@ -396,9 +421,21 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 it.s = (shared ? a.ss1 : a.s1) + (size_t)e * 2 * I;
         } else {
             const int C0 = chunks_of(I0), Cs = nshared ? chunks_of(Is) : 0, parts = Cs + (entries - nshared) * C0;
-            int run = H / 16 * parts / (MD_BLOCKS + MD_BLOCKS / 2);  // tiles of an item: some items for every block
+            // tiles of an item: about two items for every block, and small ones for the last quarter of the parts, which the
+            // blocks share out to end together
+            int run = H / 16 * parts / (MD_BLOCKS + MD_BLOCKS / 2);
             run = run >= 8 ? 8 : run >= 4 ? 4 : run >= 2 ? 2 : 1;
-            const int runs = (H / 16 + run - 1) / run, c = (q - N1) / runs;
+            const int big = parts - parts / 4, runs0 = (H / 16 + run - 1) / run;
+            int at = q - N1, c = at / runs0;
+            if (c < big) {
+                at %= runs0;
+            } else {
+                at -= big * runs0;
+                run = max(run / 2, 1);
+                const int runs = (H / 16 + run - 1) / run;
+                c = big + at / runs;
+                at %= runs;
+            }
             if (c < parts) {
                 const bool shared = c < Cs;
                 const int I = shared ? Is : I0, C = shared ? Cs : C0, d = shared ? 0 : nshared + (c - Cs) / C0;
@@ -407,9 +444,9 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 it.phase = 2;
                 it.entry = d;
                 it.chunk = shared ? c : (c - Cs) % C0;
-                it.tile = (q - N1) % runs * run;
+                it.tile = at * run;
                 it.count = min(run, H / 16 - it.tile);
-                it.lkw = cu > 4 ? 3 : cu > 2 ? 2 : cu > 1 ? 1 : 0;
+                it.lkw = cu > 4 * U2 ? 3 : cu > 2 * U2 ? 2 : cu > U2 ? 1 : 0;  // (the fewer, the more tiles are done at once)
                 it.k0 = it.chunk * cu;
                 it.units = min(cu, units - it.k0);
                 it.row_bytes = (uint32_t)(I * W::SIZE);
@@ -538,17 +575,25 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
         return reinterpret_cast<const __attribute__((address_space(4))) float *>((uintptr_t)s)[at];
     };
 
-    if (clerk) {
+    if (clerk)
         describe(0);
-        ticket = ticket2;
-        describe(1);
-    }
     __syncthreads();
     cur = read_item(0);
-    nxt = read_item(1);
     int turn = 0;  // the place of the current item, where the one after the next goes
     in.which = 0;
     stream(cur);
+    nxt.phase = 0;
+    nxt.w = cur.w;
+    nxt.s = cur.s;
+    nxt.entry = nxt.tile = nxt.count = nxt.lkw = nxt.k0 = nxt.units = nxt.chunk = 0;
+    nxt.row_bytes = nxt.step = 0;
+    top_up();  // (all there is of it: the next item is not known yet)
+    if (clerk) {
+        ticket = ticket2;
+        describe(1);
+    }
+    lds_barrier();
+    nxt = read_item(1);
     if (in.tiles == 0) {
         in.which = 1;
         stream(nxt);
@@ -568,7 +613,6 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
     // ---- the first product
     if (cur.phase == 1) {
         const int units = units_of(cur);  // the same for all of these items
-        top_up();
         // the wave's share of x: 32 columns each
         u32x4 x[U1 * W::STEPS];
         {
@@ -577,11 +621,14 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
             for (int i = 0; i < U1 * W::STEPS; ++i)
                 x[i] = u32x4{0, 0, 0, 0};
             if (l16 < T) {  // (lanes that ask for nothing cost nothing)
+                upto<U1>(units, [&](auto c) {
+                    constexpr int u = decltype(c)::value;
 #pragma unroll
-                for (int i = 0; i < U1 * W::STEPS; ++i) {
-                    const int st = i % W::STEPS, col = (w + i / W::STEPS * 8) * W::UNIT + (16 / W::SIZE) * (4 * (st / PIECES) + lq) + 8 * (st % PIECES);
-                    x[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, col < H ? (l16 * H + col) * 2 : MD_OUT, 0, 0);
-                }
+                    for (int st = 0; st < W::STEPS; ++st) {
+                        const int col = (w + u * 8) * W::UNIT + (16 / W::SIZE) * (4 * (st / PIECES) + lq) + 8 * (st % PIECES);
+                        x[u * W::STEPS + st] = __builtin_amdgcn_raw_buffer_load_b128(rx, col < H ? (l16 * H + col) * 2 : MD_OUT, 0, 0);
+                    }
+                });
             }
         }
         wait_loads<0>();
@@ -596,14 +643,20 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                     s[1][u] = scale(cur.s, ((cur.tile + (int)cur.step / 16) >> 3) * (H / 128) + at);
                 }
             }
-            f32x4 acc[2];
-#pragma unroll
+            f32x4 acc[2];  // (the loops' code is kept short: what runs for the first time comes from memory)
+#pragma unroll 1
             for (int j = 0; j < 2; ++j) {
-                acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                acc[0] = acc[1];
+                acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                upto<U1>(units, [&](auto c) {
+                    constexpr int u = decltype(c)::value;
+                    use(x + u * W::STEPS, nullptr, WT == MD_FP8 ? s[0][u] : 0.f, (uint32_t)(w + 8 * u) * 128 + 64 >= row1, acc[1]);
+                });
+                if constexpr (WT == MD_FP8) {
 #pragma unroll
-                for (int u = 0; u < U1; ++u)
-                    if (u < units)
-                        use(x + u * W::STEPS, nullptr, WT == MD_FP8 ? s[j][u] : 0.f, (uint32_t)(w + 8 * u) * 128 + 64 >= row1, acc[j]);
+                    for (int u = 0; u < U1; ++u)
+                        s[0][u] = s[1][u];
+                }
             }
             if (clerk)
                 describe(turn);
@@ -666,7 +719,7 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
         if constexpr (WT == MD_FP8) {  // (an item's tiles are of one block of rows)
 #pragma unroll
             for (int u = 0; u < U2; ++u)
-                s[u] = scale(cur.s, (cur.tile >> 3) * (int)(cur.row_bytes / 128) + min(cur.k0 + wk + 8 * u, (int)(cur.row_bytes / 128) - 1));
+                s[u] = scale(cur.s, (cur.tile >> 3) * (int)(cur.row_bytes / 128) + min(cur.k0 + wk + (u << cur.lkw), (int)(cur.row_bytes / 128) - 1));
         }
         // h of the entry, once all of it has been written.  One wave looks, at 64 entries at once.
         if (cur.entry >= known) {
@@ -704,17 +757,18 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
 #pragma unroll
             for (int u = 0; u < U2 * W::STEPS; ++u)
                 h[u] = low[u] = u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int u = 0; u < U2; ++u)
-                if (u < units && mine) {
+            upto<U2>(units, [&](auto c) {
+                constexpr int u = decltype(c)::value;
+                if (mine) {
 #pragma unroll
                     for (int st = 0; st < W::STEPS; ++st) {
-                        const int col = (cur.k0 + wk + u * 8) * W::UNIT + (16 / W::SIZE) * (4 * (st / PIECES) + lq) + 8 * (st % PIECES);
+                        const int col = (cur.k0 + wk + (u << cur.lkw)) * W::UNIT + (16 / W::SIZE) * (4 * (st / PIECES) + lq) + 8 * (st % PIECES);
                         const uint32_t off = col < limit ? (row + col) * 2 : MD_OUT;
                         h[u * W::STEPS + st] = __builtin_amdgcn_raw_buffer_load_b128(rh, off, 0, AUX_AGENT);
                         low[u * W::STEPS + st] = __builtin_amdgcn_raw_buffer_load_b128(rl, off, 0, AUX_AGENT);
                     }
                 }
+            });
             wait_loads<0>();  // (once here, not for every use below)
         }
         const rsrc_t rp = rsrc(uniform(a.part), uniform((int)a.part_bytes));
@@ -724,15 +778,18 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
             const int j0 = t0 >> (3 - cur.lkw);
             const bool last_batch = t0 + MD_BATCH * per_tile >= cur.count;
             f32x4 acc[MD_BATCH];
-#pragma unroll
+#pragma unroll 1
             for (int j = 0; j < MD_BATCH; ++j) {
-                acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (j0 + j < tiles) {
 #pragma unroll
-                    for (int u = 0; u < U2; ++u)
-                        if (u < units)
-                            use(h + u * W::STEPS, low + u * W::STEPS, WT == MD_FP8 ? s[u] : 0.f,
-                                (uint32_t)(cur.k0 + wk + 8 * u) * 128 + 64 >= cur.row_bytes, acc[j]);
+                for (int i = 1; i < MD_BATCH; ++i)
+                    acc[i - 1] = acc[i];
+                acc[MD_BATCH - 1] = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (j0 + j < tiles) {
+                    upto<U2>(units, [&](auto c) {
+                        constexpr int u = decltype(c)::value;
+                        use(h + u * W::STEPS, low + u * W::STEPS, WT == MD_FP8 ? s[u] : 0.f,
+                            (uint32_t)(cur.k0 + wk + (u << cur.lkw)) * 128 + 64 >= cur.row_bytes, acc[MD_BATCH - 1]);
+                    });
                 }
             }
             lds_barrier();  // (the last sums have been read)
@@ -767,21 +824,25 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 asm volatile("" ::: "memory");
                 if (before + 1 == Cs + (entries - nshared) * C0) {  // every part of this tile of the output is there
                     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-                    const int t = min(l16, T - 1);
-                    for (int k = 0; k < slots; ++k) {
-                        const bool shared = k + 1 == slots;
-                        if (shared && !nshared)
-                            break;
-                        const bool have = shared ? on >> t & 1 : sh.ids[t][k] >= 0;
-                        const float gate = shared ? 1.0f : sh.gates[t][k];
-                        const int C = shared ? Cs : C0;
-                        f32x4 e = f32x4{0.f, 0.f, 0.f, 0.f};
-                        for (int c = 0; c < C; ++c)
-                            e += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                     rp, have ? (uint32_t)(((t * slots + k) * chunks + c) * H + n) * 4u : MD_OUT, 0, AUX_AGENT));
+                    const int t = min(l16, T - 1), routed = (slots - 1) * C0, n_parts = routed + Cs;
+                    constexpr int AT_ONCE = 8;
+#pragma unroll 1
+                    for (int i0 = 0; i0 < n_parts; i0 += AT_ONCE) {  // picks ascending, the shared expert last
+                        f32x4 v[AT_ONCE];
+                        float gate[AT_ONCE];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q)
-                            o[q] = have ? __builtin_fmaf(gate, e[q], o[q]) : o[q];
+                        for (int i = 0; i < AT_ONCE; ++i) {
+                            const int k = i0 + i < routed ? (i0 + i) / C0 : slots - 1, c = i0 + i < routed ? (i0 + i) % C0 : i0 + i - routed;
+                            const bool have = i0 + i < routed ? sh.ids[t][k] >= 0 : i0 + i < n_parts && (on >> t & 1);
+                            gate[i] = !have ? 0.0f : i0 + i < routed ? sh.gates[t][k] : 1.0f;
+                            v[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                       rp, have ? (uint32_t)(((t * slots + k) * chunks + c) * H + n) * 4u : MD_OUT, 0, AUX_AGENT));
+                        }
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                o[q] = __builtin_fmaf(gate[i], v[i][q], o[q]);  // (what is not there is 0 times 0)
                     }
                     if (l16 < T)
                         *reinterpret_cast<u32x2 *>(a.out + (size_t)t * H + n) =
@@ -845,7 +906,7 @@ hipError_t launch_moe_decode(const MoeDecodeArgs &a, void *ws, hipStream_t s)
     r.renorm = a.renorm;
     r.dtype = ROUTE_FP32;
     const int per = route_shares(r, 64);
-    d.route_per = per <= 4 ? 4 : 16;
+    d.route_per = per <= 1 ? 1 : per <= 4 ? 4 : 16;
     if (per > 16)
         return hipErrorInvalidValue;
     route_places(r, 64, d.route_per);
