@@ -457,7 +457,7 @@ CAMHIP_API camhipStatus camhipMoeDecodeLayer(void *workspace, uint64_t workspace
  * Products are exact, sums fp32, A x in between is held to 2^-16 of itself (fp16: 2^-21 of the row's largest), one rounding
  * at the end.
  * Limits: m <= 2^20, n <= 2^20, k a multiple of 16 and at most 131056, rank a multiple of 8 and at most 256, numAdapters
- * <= 65536; loraA and loraB 16-byte aligned (x may start anywhere; rows on 16 bytes are the fast ones). */
+ * <= 65536; loraA, loraB and the rows of x 16-byte aligned. */
 CAMHIP_API camhipStatus camhipLoraAddGetWorkspaceSize(const void *base, const void *x, const float *xScale,
                                                       const void *loraA, const void *loraB, const int32_t *adapterIds,
                                                       const float *scaling, int64_t m, int64_t n, int64_t k,

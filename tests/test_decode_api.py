@@ -52,7 +52,7 @@ def lora(base=P, x=P, xs=None, a=P, b=P, ids=P, scaling=None, m=4, n=64, k=64, r
     (dict(r=264), "rank"), (dict(L=0), "numAdapters"), (dict(L=65537), "numAdapters"), (dict(bt=2), "baseDtype"),
     (dict(lt=4), "loraDtype"), (dict(xt=1), "xDtype"), (dict(xt=4), "xDtype"), (dict(ot=4), "outDtype"),
     (dict(bstep=63), "baseRowStride"), (dict(xstep=63), "xRowStride"), (dict(bstep=1 << 40), "baseRowStride"),
-    (dict(a=P + 8), "aligned"), (dict(b=P + 2), "aligned"), (dict(x=P + 1), "aligned"), (dict(bt=4, base=P + 2), "aligned"),
+    (dict(a=P + 8), "aligned"), (dict(b=P + 2), "aligned"), (dict(x=P + 8), "aligned"), (dict(xstep=68), "aligned"), (dict(bt=4, base=P + 2), "aligned"),
     (dict(ids=P + 2), "aligned"), (dict(out=P + 1), "aligned"), (dict(scaling=P + 1), "aligned"),
 ])
 def test_lora_rejects(kw, frag):

@@ -216,7 +216,8 @@ camhipStatus camhipLoraAddGetWorkspaceSize(const void *base, const void *x, cons
             CHECK_PTR(op, xScale);
     }
     CHECK_ALIGN(op, base, dtype_bytes(baseDtype));
-    CHECK_ALIGN(op, x, dtype_bytes(xDtype));
+    CHECK_ALIGN(op, x, 16);
+    CHECK_PARAM(xRowStride * dtype_bytes(xDtype) % 16 == 0, "%s: xRowStride %lld: rows must be 16-byte aligned", op, (ll)xRowStride);
     CHECK_ALIGN(op, loraA, 16);
     CHECK_ALIGN(op, loraB, 16);
     CHECK_ALIGN(op, adapterIds, 4);

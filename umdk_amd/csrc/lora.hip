@@ -1,6 +1,18 @@
 // Low-rank adapters of many requests beside a projection that they share:
 //   out[t] = base[t] + scaling[a] * B_a (A_a x_t),  a = ids[t];  out[t] = base[t] where a is no adapter
-// Products exact, sums fp32, one rounding at the end.
+// Two launches: z = A x in fp32, then out = base + B z.
+//
+// Tokens come in any order, so every block sorts for itself: it looks at a window of 256 tokens, counts for each one the
+// earlier ones with the same adapter, and takes up to CHUNK tokens of one adapter, a chunk.  A decode batch is one window, in which an
+// adapter is read once for all of its tokens; in prompts a window holds a run or two.  No order is prepared in a launch of
+// its own or kept, and no sum hangs on what other tokens are there: a token's bits are the same in any order of a batch of its size.
+//
+// What bounds it: for few tokens the adapters' stream and the latency of two launches, for many the streams of x, base and out.
+// Matrix instructions take 16 tokens as their columns, rows of A or B as their rows.  z goes into the second product as two
+// 16-bit numbers, the second what the first leaves out, so that it loses 2^-16 (bf16) or, brought to the row's largest first, 2^-21 (fp16).
+#include <atomic>
+#include <type_traits>
+
 #include "cam_device.h"
 #include "launchers.h"
 
@@ -8,71 +20,569 @@ namespace cam {
 
 namespace {
 
-__device__ __forceinline__ float half_value(uint32_t h, int dtype)
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int LR_WINDOW = 256, LR_WAVES = 4, LR_THREADS = 64 * LR_WAVES;
+constexpr int LR_MAX_SPLITS = 16;
+static_assert(LR_THREADS == LR_WINDOW, "a thread per token of the window");
+
+// two fp32 -> two 16-bit numbers, the nearest
+template <bool BF16> __device__ __forceinline__ uint32_t pack2(float a, float b)
 {
-    return dtype == LORA_BF16 ? bf16_to_f32(h & 0xffffu) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+    if constexpr (BF16)
+        return f32x2_to_bf16x2(a, b);
+    else
+        return __builtin_bit_cast(uint32_t, f16x2{(_Float16)a, (_Float16)b});
 }
-__device__ __forceinline__ float element(const void *p, int64_t at, int dtype)
+template <bool BF16> __device__ __forceinline__ float unpack(uint32_t v, int i)
 {
-    if (dtype == LORA_FP32)
-        return reinterpret_cast<const float *>(p)[at];
-    if (dtype == LORA_INT8)
-        return (float)reinterpret_cast<const int8_t *>(p)[at];
-    return half_value(reinterpret_cast<const uint16_t *>(p)[at], dtype);
+    if constexpr (BF16)
+        return __uint_as_float(i ? v & 0xffff0000u : v << 16);
+    else
+        return (float)__builtin_bit_cast(f16x2, v)[i];
+}
+template <bool BF16> __device__ __forceinline__ f32x4 mfma(const u32x4 a, const u32x4 b, const f32x4 c)
+{
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// four int8 -> four 16-bit numbers
+template <bool BF16> __device__ __forceinline__ u32x2 bytes4(uint32_t d)
+{
+    return u32x2{pack2<BF16>((float)(int8_t)d, (float)(int8_t)(d >> 8)), pack2<BF16>((float)(int8_t)(d >> 16), (float)((int32_t)d >> 24))};
 }
 
-// z[t, r] = scaling * xs[t] * A_a[r] . x_t, a wave each
-__global__ __launch_bounds__(256) void lora_shrink_kernel(const LoraArgs p, float *z)
+// ---------------------------------------------------------------- chunks
+// The tokens of a window by chunks: chunk q holds up to SIZE tokens of one adapter (of none: id -1, last of all sorted as any other).
+struct Chunks {
+    int32_t id[LR_WINDOW];      // adapter, -1 for none
+    int32_t count[LR_WAVES];
+    int32_t at, members, adapter;  // of the chunk asked for
+    int32_t list[LR_WINDOW];
+};
+// This thread's token's place: (the chunk's number if it is the chunk's first, its rank among its adapter's); returns the number of chunks.
+__device__ __forceinline__ int find_chunks(Chunks &c, const int32_t *ids, int64_t m0, int n, int L, int size, int &rank, int &before)
 {
-    const int lane = threadIdx.x & 63, r = blockIdx.x * 4 + (threadIdx.x >> 6);
-    for (int64_t t = blockIdx.y; t < p.M; t += gridDim.y) {
-        const int a = p.ids[t];
-        if (a < 0 || a >= p.L || r >= p.R)
-            continue;
-        float sum = 0.0f;
-        for (int k = lane; k < p.K; k += 64)
-            sum = __builtin_fmaf(half_value(reinterpret_cast<const uint16_t *>(p.a)[((int64_t)a * p.R + r) * p.K + k], p.dtype),
-                                 element(p.x, t * p.x_stride + k, p.x_dtype), sum);
+    const int j = threadIdx.x;
+    int a = -2;
+    if (j < n) {
+        a = ids[m0 + j];
+        a = a < 0 || a >= L ? -1 : a;
+    }
+    c.id[j] = a;
+    __syncthreads();
+    rank = 0;
+    const int waves_end = (j & ~63) + 64;  // (as far as any token of the wave looks)
+    for (int i = 0; i < waves_end; i += 4) {
+        const i32x4 v = *reinterpret_cast<const i32x4 *>(&c.id[i]);
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1)
-            sum += __shfl_xor(sum, o, 64);
-        if (lane == 0)
-            z[t * p.R + r] = sum * (p.xs ? p.xs[t] : 1.0f) * (p.scaling ? p.scaling[a] : 1.0f);
+        for (int q = 0; q < 4; ++q)
+            rank += (v[q] == a) & (i + q < j);
+    }
+    const bool leads = j < n && (rank & (size - 1)) == 0;
+    const uint64_t mask = __ballot(leads);
+    if ((j & 63) == 0)
+        c.count[j >> 6] = __popcll(mask);
+    __syncthreads();
+    int total = 0;
+    before = __popcll(mask & lanemask_lt());
+#pragma unroll
+    for (int w = 0; w < LR_WAVES; ++w) {
+        before += w < (j >> 6) ? c.count[w] : 0;
+        total += c.count[w];
+    }
+    if (!leads)
+        before = -1;
+    return total;
+}
+// chunk q's tokens into c.list, their number and adapter
+__device__ __forceinline__ void take_chunk(Chunks &c, int n, int size, int q, int rank, int before)
+{
+    const int j = threadIdx.x;
+    __syncthreads();  // (the last chunk has been read)
+    if (before == q) {
+        c.adapter = c.id[j];
+        c.at = rank;
+        c.members = 0;
+    }
+    __syncthreads();
+    if (j < n && c.id[j] == c.adapter && rank >= c.at && rank < c.at + size) {
+        c.list[rank - c.at] = j;
+        atomicMax(&c.members, rank - c.at + 1);
+    }
+    __syncthreads();
+}
+
+// ---------------------------------------------------------------- A x
+struct ShrinkArgs {
+    const void *x, *a;
+    const int32_t *ids;
+    float *z;           // [splits, M, R]
+    int64_t M, x_stride;
+    int K, R, L, splits, slots, groups;  // slots: blocks that share a window's chunks; groups: of rows of A
+};
+// at most N of this wave's loads are in flight, and none of its LDS reads
+template <int N> __device__ __forceinline__ void wait_loads()
+{
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (7 << 4));
+    asm volatile("" ::: "memory");
+}
+template <int MOST, int LOADS> __device__ __forceinline__ void wait_steps(int left)
+{
+    if constexpr (MOST == 0) {
+        wait_loads<0>();
+    } else {
+        if (left >= MOST)
+            wait_loads<MOST * LOADS>();
+        else
+            wait_steps<MOST - 1, LOADS>(left);
+    }
+}
+__device__ __forceinline__ void dma(const uint8_t *g, uint8_t *lds)
+{
+    __builtin_amdgcn_global_load_lds(g, (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+}
+
+// 16 MF tokens by 16 NF rows of A over a block's share of K.  The waves take turns at units of 128 bytes of x (64 values, of
+// int8 128), each with a ring of SLOTS units of its own in LDS, so that no wave waits for another before the end.  A load
+// instruction brings 8 rows by 128 bytes, whole cache lines; 16-byte pieces are turned by (row / 2) mod 8, so that the rows of
+// a fragment fall on different banks.
+template <bool BF16, bool INT8, int MF, int NF, int SLOTS>
+__global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const ShrinkArgs p)
+{
+    constexpr int LINES = INT8 ? 2 : 1;                        // of A, to a line of x
+    constexpr int A_BANDS = 2 * NF * LINES, BANDS = A_BANDS + 2 * MF, SLOT = BANDS * 1024, UNIT = INT8 ? 128 : 64;
+    static_assert(MF * NF * 1024 <= SLOTS * SLOT && (SLOTS - 1) * BANDS < 64, "sums where the ring was; vmcnt range");
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+    __shared__ Chunks c;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    int id = blockIdx.x;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int group = id % p.groups;
+    id /= p.groups;
+    const int first = id % p.slots;
+    const int64_t m0 = (int64_t)(id / p.slots) * LR_WINDOW;
+    const int n = (int)min((int64_t)LR_WINDOW, p.M - m0);
+    int rank, before;
+    const int chunks = find_chunks(c, p.ids, m0, n, p.L, 16 * MF, rank, before);
+
+    const int K = p.K, x_bytes = INT8 ? K : 2 * K, a_bytes = 2 * K;
+    const int units = (K + UNIT - 1) / UNIT, from = units * split / p.splits, to = units * (split + 1) / p.splits;
+    const int mine = to - from > w ? (to - from - w + LR_WAVES - 1) / LR_WAVES : 0;
+    uint8_t *ring = smem + w * SLOTS * SLOT;
+    const int turned = (lane & 7) ^ (lane >> 4);  // in even bands of 8 rows; odd ones: ^ 4
+    for (int q = first; q < chunks; q += p.slots) {
+        take_chunk(c, n, 16 * MF, q, rank, before);
+        const int adapter = c.adapter, members = c.members;
+        if (adapter < 0)
+            continue;
+        const uint8_t *xr[2 * MF], *ar[2 * NF];
+#pragma unroll
+        for (int b = 0; b < 2 * MF; ++b)
+            xr[b] = reinterpret_cast<const uint8_t *>(p.x) +
+                    (m0 + c.list[min(b * 8 + (lane >> 3), members - 1)]) * p.x_stride * (INT8 ? 1 : 2);
+#pragma unroll
+        for (int b = 0; b < 2 * NF; ++b)
+            ar[b] = reinterpret_cast<const uint8_t *>(p.a) +
+                    ((int64_t)adapter * p.R + min((group * 2 * NF + b) * 8 + (lane >> 3), p.R - 1)) * a_bytes;
+        const auto load = [&](int t, int slot) {
+            const int u = from + w + t * LR_WAVES;
+            uint8_t *lds = ring + slot * SLOT;
+#pragma unroll
+            for (int b = 0; b < 2 * NF; ++b)
+#pragma unroll
+                for (int l = 0; l < LINES; ++l)
+                    dma(ar[b] + min((u * LINES + l) * 128 + ((turned ^ (4 * (b & 1))) << 4), a_bytes - 16), lds + (l * 2 * NF + b) * 1024);
+#pragma unroll
+            for (int b = 0; b < 2 * MF; ++b)
+                dma(xr[b] + min(u * 128 + ((turned ^ (4 * (b & 1))) << 4), x_bytes - 16), lds + (A_BANDS + b) * 1024);
+        };
+        f32x4 acc[MF][NF];
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+                acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < SLOTS; ++s)
+            if (s < mine)
+                load(s, s);
+        // 16-byte piece `piece` of row l16 of a fragment
+        const auto piece_at = [&](int piece) { return l16 * 128 + ((piece ^ (l16 >> 1)) << 4); };
+        int slot = 0;
+#pragma unroll 1
+        for (int t = 0; t < mine; ++t) {
+            wait_steps<SLOTS - 1, BANDS>(mine - 1 - t);
+            const uint8_t *at = ring + slot * SLOT;
+            constexpr int STEPS = INT8 ? 4 : 2;  // of 32 values
+            u32x4 xf[MF][STEPS], af[NF][STEPS];
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4 v = *reinterpret_cast<const u32x4 *>(at + (A_BANDS + 2 * i) * 1024 + piece_at(lq + 4 * h));
+                    if constexpr (INT8) {
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            const u32x2 lo = bytes4<BF16>(v[2 * s]), hi = bytes4<BF16>(v[2 * s + 1]);
+                            xf[i][2 * h + s] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+                        }
+                    } else {
+                        xf[i][h] = v;
+                    }
+                }
+            // the same columns of A: of int8 rows' piece lq + 4 h the 16 values from 64 h + 16 lq on
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+                    af[j][s] = *reinterpret_cast<const u32x4 *>(
+                        at + (INT8 ? (s >> 1) * 2 * NF + 2 * j : 2 * j) * 1024 + piece_at(INT8 ? 2 * lq + (s & 1) : lq + 4 * s));
+            wait_loads<63>();  // (the slot has been read)
+            if (t + SLOTS < mine)
+                load(t + SLOTS, slot);
+            const int k = (from + w + t * LR_WAVES) * UNIT;
+            if (k + UNIT > K) {
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s)
+                    if (k + (INT8 ? (s >> 1) * 64 + lq * 16 + (s & 1) * 8 : s * 32 + lq * 8) >= K) {
+#pragma unroll
+                        for (int j = 0; j < NF; ++j)
+                            af[j][s] = u32x4{0, 0, 0, 0};
+                    }
+            }
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+                for (int i = 0; i < MF; ++i)
+#pragma unroll
+                    for (int j = 0; j < NF; ++j)
+                        acc[i][j] = mfma<BF16>(af[j][s], xf[i][s], acc[i][j]);
+            slot = slot == SLOTS - 1 ? 0 : slot + 1;
+        }
+        // the waves' sums meet where their rings were
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+                *reinterpret_cast<f32x4 *>(ring + (i * NF + j) * 1024 + lane * 16) = acc[i][j];
+        __syncthreads();
+        for (int f = w; f < MF * NF; f += LR_WAVES) {
+            f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int v = 0; v < LR_WAVES; ++v)
+                sum += *reinterpret_cast<const f32x4 *>(smem + v * SLOTS * SLOT + f * 1024 + lane * 16);
+            const int i = f / NF * 16 + l16, r = (group * NF + f % NF) * 16 + lq * 4;
+            if (i < members && r < p.R)
+                *reinterpret_cast<f32x4 *>(p.z + ((int64_t)split * p.M + m0 + c.list[i]) * p.R + r) = sum;
+        }
     }
 }
 
-__global__ __launch_bounds__(256) void lora_expand_kernel(const LoraArgs p, const float *z)
+// ---------------------------------------------------------------- base + B z
+struct ExpandArgs {
+    const void *base, *b;
+    const float *z, *xs, *scaling;
+    const int32_t *ids;
+    void *out;
+    int64_t M, base_stride;
+    int N, R, L;
+    int16_t splits, slots, tiles;  // tiles: of 64 columns, that a wave does
+    int8_t base_dtype, out_bf16;
+};
+// 8 consecutive numbers of a row as fp32, the first `left` of them
+__device__ __forceinline__ void load8(const void *p, int64_t at, int dtype, int left, float *v)
 {
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= p.N)
+    if (dtype == LORA_FP32) {
+        const float *f = reinterpret_cast<const float *>(p) + at;
+        if (left >= 8) {
+            __builtin_memcpy(v, f, 32);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                v[i] = i < left ? f[i] : 0.0f;
+        }
         return;
-    for (int64_t t = blockIdx.y; t < p.M; t += gridDim.y) {
-        const int a = p.ids[t];
-        float sum = 0.0f;
-        if (a >= 0 && a < p.L)
-            for (int r = 0; r < p.R; ++r)
-                sum = __builtin_fmaf(half_value(reinterpret_cast<const uint16_t *>(p.b)[((int64_t)a * p.N + n) * p.R + r], p.dtype),
-                                     z[t * p.R + r], sum);
-        const float v = element(p.base, t * p.base_stride + n, p.base_dtype) + sum;
-        uint16_t *out = reinterpret_cast<uint16_t *>(p.out) + t * p.N + n;
-        *out = p.out_dtype == LORA_BF16 ? (uint16_t)(f32x2_to_bf16x2(v, 0.0f) & 0xffffu)
-                                        : __builtin_bit_cast(uint16_t, (_Float16)v);
     }
+    const uint16_t *h = reinterpret_cast<const uint16_t *>(p) + at;
+    u32x4 r = u32x4{0, 0, 0, 0};
+    if (left >= 8) {
+        __builtin_memcpy(&r, h, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left)
+                r[i >> 1] |= (uint32_t)h[i] << (16 * (i & 1));
+    }
+    if (dtype == LORA_BF16) {
+        unpack_bf16x8(r, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = unpack<false>(r[i >> 1], i & 1);
+    }
+}
+__device__ __forceinline__ void store8(void *p, int64_t at, bool bf16, int left, const float *v)
+{
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = bf16 ? pack2<true>(v[2 * i], v[2 * i + 1]) : pack2<false>(v[2 * i], v[2 * i + 1]);
+    uint16_t *h = reinterpret_cast<uint16_t *>(p) + at;
+    if (left >= 8) {
+        __builtin_memcpy(h, &r, 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left)
+                h[i] = (uint16_t)(r[i >> 1] >> (16 * (i & 1)));
+    }
+}
+
+// A chunk of up to 16 MF tokens by 64 columns a wave at a time.  z of the chunk lies in LDS as the instructions' second operand:
+// [token fragment][step of 32][first or second number][lane] 16 bytes.  Row i of the tile f of 64 columns is column
+// 32 (f / 2) + 8 (i / 4) + 4 (f mod 2) + i mod 4, so that a lane's results are twice 8 consecutive columns of one token.
+template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) void lora_expand_kernel(const ExpandArgs p)
+{
+    __shared__ Chunks c;
+    __shared__ u32x4 zs[MF][KS][2][64];
+    __shared__ float factor[16 * MF];
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int span = 64 * LR_WAVES * p.tiles, n_blocks = (p.N + span - 1) / span;
+    int id = blockIdx.x;
+    const int n_block = id % n_blocks;
+    id /= n_blocks;
+    const int first = id % p.slots;
+    const int64_t m0 = (int64_t)(id / p.slots) * LR_WINDOW;
+    const int n = (int)min((int64_t)LR_WINDOW, p.M - m0);
+    int rank, before;
+    const int chunks = find_chunks(c, p.ids, m0, n, p.L, 16 * MF, rank, before);
+    for (int q = first; q < chunks; q += p.slots) {
+        take_chunk(c, n, 16 * MF, q, rank, before);
+        const int adapter = c.adapter, members = c.members;
+        if (adapter >= 0) {
+            // 4 KS threads a token, 8 values each
+            for (int i = threadIdx.x; i < 16 * MF * 4 * KS; i += LR_THREADS) {
+                const int t = i / (4 * KS), part = i % (4 * KS), r = part * 8;
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    z[e] = 0.0f;
+                const int64_t m = m0 + c.list[min(t, members - 1)];
+                if (r < p.R)
+                    for (int s = 0; s < p.splits; ++s) {
+                        const f32x4 *v = reinterpret_cast<const f32x4 *>(p.z + ((int64_t)s * p.M + m) * p.R + r);
+                        const f32x4 a = v[0], b = v[1];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            z[e] += e < 4 ? a[e & 3] : b[e & 3];
+                    }
+                float f = p.scaling ? p.scaling[adapter] : 1.0f;
+                if (p.xs)
+                    f *= p.xs[m];
+                if constexpr (!BF16) {  // the row's largest to 2^10 or a little less: what is left out then keeps its bits
+                    float most = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        most = fmaxf(most, fabsf(z[e]));
+                    most = KS == 8 ? group_max<32>(most) : KS == 4 ? group_max<16>(most) : KS == 2 ? group_max<8>(most) : group_max<4>(most);
+                    const bool plain = most > 0.0f && most < INFINITY;
+                    const int e2 = plain ? 10 - ilogbf(most) : 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        z[e] = ldexpf(z[e], e2);
+                    f = ldexpf(f, -e2);
+                }
+                u32x4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    hi[e] = pack2<BF16>(z[2 * e], z[2 * e + 1]);
+                    lo[e] = pack2<BF16>(z[2 * e] - unpack<BF16>(hi[e], 0), z[2 * e + 1] - unpack<BF16>(hi[e], 1));
+                }
+                zs[t >> 4][part >> 2][0][(part & 3) * 16 + (t & 15)] = hi;
+                zs[t >> 4][part >> 2][1][(part & 3) * 16 + (t & 15)] = lo;
+                if (part == 0)
+                    factor[t] = f;
+            }
+        }
+        __syncthreads();
+        const int frags = (members + 15) >> 4;
+        for (int tile = 0; tile < p.tiles; ++tile) {
+            const int n0 = n_block * span + (tile * LR_WAVES + w) * 64;
+            if (n0 >= p.N)
+                break;
+            u32x4 bf[4][KS];
+            if (adapter >= 0) {
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                    const int col = min(n0 + 32 * (f >> 1) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3), p.N - 1);
+                    const uint16_t *row = reinterpret_cast<const uint16_t *>(p.b) + ((int64_t)adapter * p.N + col) * p.R;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)  // (past the rank: nothing, whatever lies there)
+                        bf[f][s] = s * 32 + lq * 8 < p.R ? *reinterpret_cast<const u32x4 *>(row + s * 32 + lq * 8) : u32x4{0, 0, 0, 0};
+                }
+            }
+            // (all of base first: out may be base, so that no load would pass a store)
+            float v[MF][2][8];
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+                if (i < frags) {
+                    const int64_t m = m0 + c.list[min(i * 16 + l16, members - 1)];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                        load8(p.base, m * p.base_stride + n0 + 32 * g + 8 * lq, p.base_dtype, p.N - (n0 + 32 * g + 8 * lq), v[i][g]);
+                }
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+                if (i < frags) {
+                    const int t = i * 16 + l16;
+                    if (adapter >= 0) {
+                        f32x4 acc[4];
+#pragma unroll
+                        for (int f = 0; f < 4; ++f)
+                            acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int s = 0; s < KS; ++s)
+#pragma unroll
+                            for (int part = 0; part < 2; ++part) {
+                                const u32x4 z = zs[i][s][part][lane];
+#pragma unroll
+                                for (int f = 0; f < 4; ++f)
+                                    acc[f] = mfma<BF16>(bf[f][s], z, acc[f]);
+                            }
+                        const float scale = factor[t];
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                v[i][g][e] = __builtin_fmaf(scale, acc[2 * g + (e >> 2)][e & 3], v[i][g][e]);
+                    }
+                    if (t < members) {
+                        const int64_t m = m0 + c.list[t];
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+                            store8(p.out, m * p.N + n0 + 32 * g + 8 * lq, p.out_bf16, p.N - (n0 + 32 * g + 8 * lq), v[i][g]);
+                    }
+                }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- which kernels
+// Tokens of a chunk: 16 in a decode batch, whose adapters have few each; 32 and 64 for prompts, where a chunk's share of A and B is read again for each.
+int chunk_frags(int64_t M) { return M <= LR_WINDOW ? 1 : M < 8192 ? 2 : 4; }
+struct Plan {
+    int mf, nf, groups, slots, splits;
+    int64_t windows;
+};
+Plan lora_plan(const LoraArgs &a)
+{
+    Plan p;
+    const bool int8 = a.x_dtype == LORA_INT8;
+    p.windows = (a.M + LR_WINDOW - 1) / LR_WINDOW;
+    p.mf = chunk_frags(a.M);
+    const int frags = (a.R + 15) / 16, most = int8 ? 2 : 4;
+    p.nf = frags >= most ? most : frags >= 2 ? 2 : 1;
+    p.groups = (frags + p.nf - 1) / p.nf;
+    // a window's chunks: all of a decode batch at once, of prompts a few more than if they had one adapter
+    p.slots = a.M <= LR_WINDOW ? (int)a.M : LR_WINDOW / (16 * p.mf) + 4;
+    // K is split until the chips' CUs have something to do, and no wave has less than a unit
+    const int64_t chunks = a.M <= LR_WINDOW ? (a.M < a.L + a.M / 16 ? a.M : a.L + a.M / 16) : a.M / (16 * p.mf);
+    const int64_t units = (a.K + (int8 ? 127 : 63)) / (int8 ? 128 : 64);
+    int64_t s = 256 / (chunks * p.groups > 0 ? chunks * p.groups : 1);
+    s = s < units / LR_WAVES ? s : units / LR_WAVES;
+    p.splits = (int)(s < 1 ? 1 : s > LR_MAX_SPLITS ? LR_MAX_SPLITS : s);
+    return p;
+}
+
+constexpr int LR_MAX_DEVICES = 64;
+template <bool BF16, bool INT8, int MF, int NF> hipError_t shrink(const ShrinkArgs &a, int64_t blocks, hipStream_t s)
+{
+    constexpr int SLOT = (2 * NF * (INT8 ? 2 : 1) + 2 * MF) * 1024, SLOTS = SLOT <= 4096 ? 4 : SLOT <= 8192 ? 3 : 2, LDS = LR_WAVES * SLOTS * SLOT;
+    static std::atomic<bool> done[LR_MAX_DEVICES];  // the kernel's dynamic LDS limit is raised once per device
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    if (e == hipSuccess && !(dev < LR_MAX_DEVICES && done[dev].load(std::memory_order_acquire))) {
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&lora_shrink_kernel<BF16, INT8, MF, NF, SLOTS>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e == hipSuccess && dev < LR_MAX_DEVICES)
+            done[dev].store(true, std::memory_order_release);
+    }
+    if (e != hipSuccess)
+        return e;
+    hipLaunchKernelGGL((lora_shrink_kernel<BF16, INT8, MF, NF, SLOTS>), dim3((uint32_t)blocks), dim3(LR_THREADS), LDS, s, a);
+    return hipGetLastError();
+}
+template <bool BF16, bool INT8, int MF> hipError_t shrink_nf(int nf, const ShrinkArgs &a, int64_t blocks, hipStream_t s)
+{
+    if (nf == 1)
+        return shrink<BF16, INT8, MF, 1>(a, blocks, s);
+    if (nf == 2)
+        return shrink<BF16, INT8, MF, 2>(a, blocks, s);
+    if constexpr (!INT8)
+        return shrink<BF16, INT8, MF, 4>(a, blocks, s);
+    return hipErrorInvalidValue;
+}
+template <bool BF16, bool INT8> hipError_t shrink_mf(int mf, int nf, const ShrinkArgs &a, int64_t blocks, hipStream_t s)
+{
+    return mf == 1 ? shrink_nf<BF16, INT8, 1>(nf, a, blocks, s) : mf == 2 ? shrink_nf<BF16, INT8, 2>(nf, a, blocks, s)
+                                                                          : shrink_nf<BF16, INT8, 4>(nf, a, blocks, s);
+}
+template <bool BF16, int MF> hipError_t expand_ks(const ExpandArgs &a, uint32_t blocks, hipStream_t s)
+{
+    const dim3 grid(blocks), block(LR_THREADS);
+    if (a.R <= 32)
+        hipLaunchKernelGGL((lora_expand_kernel<BF16, 1, MF>), grid, block, 0, s, a);
+    else if (a.R <= 64)
+        hipLaunchKernelGGL((lora_expand_kernel<BF16, 2, MF>), grid, block, 0, s, a);
+    else if (a.R <= 128)
+        hipLaunchKernelGGL((lora_expand_kernel<BF16, 4, MF>), grid, block, 0, s, a);
+    else
+        hipLaunchKernelGGL((lora_expand_kernel<BF16, 8, (MF < 4 ? MF : 2)>), grid, block, 0, s, a);
+    return hipGetLastError();
+}
+template <bool BF16> hipError_t expand(int mf, const ExpandArgs &a, uint32_t blocks, hipStream_t s)
+{
+    return mf == 1 ? expand_ks<BF16, 1>(a, blocks, s) : mf == 2 ? expand_ks<BF16, 2>(a, blocks, s) : expand_ks<BF16, 4>(a, blocks, s);
 }
 
 }  // namespace
 
-size_t lora_workspace_bytes(const LoraArgs &a) { return (size_t)a.M * a.R * 4; }
+size_t lora_workspace_bytes(const LoraArgs &a)
+{
+    return a.M == 0 ? 0 : (size_t)lora_plan(a).splits * (size_t)a.M * (size_t)a.R * 4;
+}
 
 hipError_t launch_lora_add(const LoraArgs &a, void *ws, hipStream_t s)
 {
     if (a.M == 0)
         return hipSuccess;
-    float *z = reinterpret_cast<float *>(ws);
-    const int rows = (int)(a.M < 32768 ? a.M : 32768);
-    hipLaunchKernelGGL(lora_shrink_kernel, dim3((a.R + 3) / 4, rows), dim3(256), 0, s, a, z);
-    hipLaunchKernelGGL(lora_expand_kernel, dim3((a.N + 255) / 256, rows), dim3(256), 0, s, a, (const float *)z);
-    return hipGetLastError();
+    const Plan p = lora_plan(a);
+    const bool bf16 = a.dtype == LORA_BF16, int8 = a.x_dtype == LORA_INT8;
+    const ShrinkArgs sa{a.x, a.a, a.ids, reinterpret_cast<float *>(ws), a.M, a.x_stride, a.K, a.R, a.L, p.splits, p.slots, p.groups};
+    const int64_t blocks = p.windows * p.slots * p.groups * p.splits;
+    if (blocks * LR_THREADS > 0xffffffffll)
+        return hipErrorInvalidValue;
+    hipError_t e = bf16 ? (int8 ? shrink_mf<true, true>(p.mf, p.nf, sa, blocks, s) : shrink_mf<true, false>(p.mf, p.nf, sa, blocks, s))
+                        : (int8 ? shrink_mf<false, true>(p.mf, p.nf, sa, blocks, s) : shrink_mf<false, false>(p.mf, p.nf, sa, blocks, s));
+    if (e != hipSuccess)
+        return e;
+    const int mf = a.R > 128 && p.mf > 2 ? 2 : p.mf, slots = a.M <= LR_WINDOW ? (int)a.M : LR_WINDOW / (16 * mf) + 4;
+    ExpandArgs ea{a.base, a.b, reinterpret_cast<const float *>(ws), a.xs, a.scaling, a.ids, a.out, a.M, a.base_stride, a.N, a.R, a.L,
+                  (int16_t)p.splits, (int16_t)slots, 1, a.base_dtype, (int8_t)(a.out_dtype == LORA_BF16)};
+    // a block's columns: the more, the seldomer z is laid out
+    while (ea.tiles < 4 && a.M > LR_WINDOW && p.windows * slots * ((a.N + 256 * 2 * ea.tiles - 1) / (256 * 2 * ea.tiles)) >= 1024)
+        ea.tiles *= 2;
+    const int64_t n_blocks = (a.N + 256 * ea.tiles - 1) / (256 * ea.tiles), eb = p.windows * slots * n_blocks;
+    if (eb * LR_THREADS > 0xffffffffll)
+        return hipErrorInvalidValue;
+    return bf16 ? expand<true>(mf, ea, (uint32_t)eb, s) : expand<false>(mf, ea, (uint32_t)eb, s);
 }
 
 }  // namespace cam

@@ -649,6 +649,9 @@ def lora_add(base, x, lora_a, lora_b, adapter_ids, scaling=None, x_scale=None, o
 
     bs, b_step = rows(base, n)
     xr, x_step = rows(x, k)
+    size = xr.element_size()
+    if xr.data_ptr() % 16 or x_step * size % 16:  # (the kernel reads rows by 16 bytes)
+        xr, x_step = xr.clone(memory_format=torch.contiguous_format), k
     with torch.cuda.device(index):
         # (ids past 32 bits stay outside [0, adapters))
         ids = (adapter_ids if adapter_ids.dtype == torch.int32 else adapter_ids.clamp(-1, L).to(torch.int32)).contiguous()
