@@ -76,7 +76,7 @@ __device__ __forceinline__ int find_chunks(Chunks &c, const int32_t *ids, int64_
     c.id[j] = a;
     __syncthreads();
     rank = 0;
-    const int waves_end = (j & ~63) + 64;  // (as far as any token of the wave looks)
+    const int waves_end = min((j & ~63) + 64, n);  // (as far as any token of the wave looks)
     for (int i = 0; i < waves_end; i += 4) {
         const i32x4 v = *reinterpret_cast<const i32x4 *>(&c.id[i]);
 #pragma unroll
@@ -296,47 +296,62 @@ struct ExpandArgs {
     int16_t splits, slots, tiles;  // tiles: of 64 columns, that a wave does
     int8_t base_dtype, out_bf16;
 };
-// 8 consecutive numbers of a row as fp32, the first `left` of them
-__device__ __forceinline__ void load8(const void *p, int64_t at, int dtype, int left, float *v)
+// 8 consecutive numbers of base, of 16 or (WIDE) of 32 bits.  FULL: all of them are there, otherwise the first `left`.
+template <bool WIDE> struct Raw8 {
+    u32x4 v[WIDE ? 2 : 1];
+};
+typedef u32x4 u32x4_u __attribute__((aligned(2)));
+template <bool WIDE, bool FULL> __device__ __forceinline__ Raw8<WIDE> load8(const void *p, int64_t at, int left)
 {
-    if (dtype == LORA_FP32) {
-        const float *f = reinterpret_cast<const float *>(p) + at;
-        if (left >= 8) {
-            __builtin_memcpy(v, f, 32);
+    Raw8<WIDE> r;
+    const uint8_t *b = reinterpret_cast<const uint8_t *>(p) + at * (WIDE ? 4 : 2);
+#pragma unroll
+    for (int h = 0; h < (WIDE ? 2 : 1); ++h) {
+        if constexpr (FULL) {
+            r.v[h] = *reinterpret_cast<const u32x4_u *>(b + 16 * h);
         } else {
+            r.v[h] = u32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                v[i] = i < left ? f[i] : 0.0f;
+            for (int i = 0; i < (WIDE ? 4 : 8); ++i)
+                if (i + 4 * h < left) {
+                    if constexpr (WIDE)
+                        r.v[h][i] = reinterpret_cast<const uint32_t *>(b)[i + 4 * h];
+                    else
+                        r.v[h][i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(b)[i] << (16 * (i & 1));
+                }
         }
-        return;
     }
-    const uint16_t *h = reinterpret_cast<const uint16_t *>(p) + at;
-    u32x4 r = u32x4{0, 0, 0, 0};
-    if (left >= 8) {
-        __builtin_memcpy(&r, h, 16);
+    return r;
+}
+template <bool WIDE> __device__ __forceinline__ void to_fp32(const Raw8<WIDE> &r, bool bf16, float *v)
+{
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = __uint_as_float(r.v[i >> 2][i & 3]);
+    } else if (bf16) {
+        unpack_bf16x8(r.v[0], v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < left)
-                r[i >> 1] |= (uint32_t)h[i] << (16 * (i & 1));
-    }
-    if (dtype == LORA_BF16) {
-        unpack_bf16x8(r, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v[i] = unpack<false>(r[i >> 1], i & 1);
+            v[i] = unpack<false>(r.v[0][i >> 1], i & 1);
     }
 }
-__device__ __forceinline__ void store8(void *p, int64_t at, bool bf16, int left, const float *v)
+template <bool FULL> __device__ __forceinline__ void store8(void *p, int64_t at, bool bf16, int left, const float *v)
 {
     u32x4 r;
+    if (bf16) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        r[i] = bf16 ? pack2<true>(v[2 * i], v[2 * i + 1]) : pack2<false>(v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < 4; ++i)
+            r[i] = pack2<true>(v[2 * i], v[2 * i + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            r[i] = pack2<false>(v[2 * i], v[2 * i + 1]);
+    }
     uint16_t *h = reinterpret_cast<uint16_t *>(p) + at;
-    if (left >= 8) {
-        __builtin_memcpy(h, &r, 16);
+    if constexpr (FULL) {
+        *reinterpret_cast<u32x4_u *>(h) = r;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -348,7 +363,7 @@ __device__ __forceinline__ void store8(void *p, int64_t at, bool bf16, int left,
 // A chunk of up to 16 MF tokens by 64 columns a wave at a time.  z of the chunk lies in LDS as the instructions' second operand:
 // [token fragment][step of 32][first or second number][lane] 16 bytes.  Row i of the tile f of 64 columns is column
 // 32 (f / 2) + 8 (i / 4) + 4 (f mod 2) + i mod 4, so that a lane's results are twice 8 consecutive columns of one token.
-template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) void lora_expand_kernel(const ExpandArgs p)
+template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) void lora_expand_kernel(const ExpandArgs p)
 {
     __shared__ Chunks c;
     __shared__ u32x4 zs[MF][KS][2][64];
@@ -375,14 +390,25 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
                 for (int e = 0; e < 8; ++e)
                     z[e] = 0.0f;
                 const int64_t m = m0 + c.list[min(t, members - 1)];
-                if (r < p.R)
-                    for (int s = 0; s < p.splits; ++s) {
-                        const f32x4 *v = reinterpret_cast<const f32x4 *>(p.z + ((int64_t)s * p.M + m) * p.R + r);
-                        const f32x4 a = v[0], b = v[1];
+                if (r < p.R) {
+                    constexpr int AT_ONCE = 4;
+                    for (int s0 = 0; s0 < p.splits; s0 += AT_ONCE) {
+                        f32x4 v[AT_ONCE][2];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            z[e] += e < 4 ? a[e & 3] : b[e & 3];
+                        for (int s = 0; s < AT_ONCE; ++s) {
+                            const f32x4 *from = reinterpret_cast<const f32x4 *>(p.z + ((int64_t)min(s0 + s, p.splits - 1) * p.M + m) * p.R + r);
+                            v[s][0] = from[0];
+                            v[s][1] = from[1];
+                        }
+#pragma unroll
+                        for (int s = 0; s < AT_ONCE; ++s)
+                            if (s0 + s < p.splits) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    z[e] += v[s][e >> 2][e & 3];
+                            }
                     }
+                }
                 float f = p.scaling ? p.scaling[adapter] : 1.0f;
                 if (p.xs)
                     f *= p.xs[m];
@@ -412,7 +438,6 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
             }
         }
         __syncthreads();
-        const int frags = (members + 15) >> 4;
         for (int tile = 0; tile < p.tiles; ++tile) {
             const int n0 = n_block * span + (tile * LR_WAVES + w) * 64;
             if (n0 >= p.N)
@@ -428,20 +453,24 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
                         bf[f][s] = s * 32 + lq * 8 < p.R ? *reinterpret_cast<const u32x4 *>(row + s * 32 + lq * 8) : u32x4{0, 0, 0, 0};
                 }
             }
-            // (all of base first: out may be base, so that no load would pass a store)
-            float v[MF][2][8];
+            const auto columns = [&](auto all_there) {
+                constexpr bool FULL = decltype(all_there)::value;
+                // (all of base first: out may be base, so that no load would pass a store)
+                Raw8<WIDE> raw[MF][2];
 #pragma unroll
-            for (int i = 0; i < MF; ++i)
-                if (i < frags) {
+                for (int i = 0; i < MF; ++i) {
                     const int64_t m = m0 + c.list[min(i * 16 + l16, members - 1)];
 #pragma unroll
                     for (int g = 0; g < 2; ++g)
-                        load8(p.base, m * p.base_stride + n0 + 32 * g + 8 * lq, p.base_dtype, p.N - (n0 + 32 * g + 8 * lq), v[i][g]);
+                        raw[i][g] = load8<WIDE, FULL>(p.base, m * p.base_stride + n0 + 32 * g + 8 * lq, p.N - (n0 + 32 * g + 8 * lq));
                 }
 #pragma unroll
-            for (int i = 0; i < MF; ++i)
-                if (i < frags) {
+                for (int i = 0; i < MF; ++i) {
                     const int t = i * 16 + l16;
+                    float v[2][8];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                        to_fp32<WIDE>(raw[i][g], p.base_dtype == LORA_BF16, v[g]);
                     if (adapter >= 0) {
                         f32x4 acc[4];
 #pragma unroll
@@ -461,15 +490,20 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
                         for (int g = 0; g < 2; ++g)
 #pragma unroll
                             for (int e = 0; e < 8; ++e)
-                                v[i][g][e] = __builtin_fmaf(scale, acc[2 * g + (e >> 2)][e & 3], v[i][g][e]);
+                                v[g][e] = __builtin_fmaf(scale, acc[2 * g + (e >> 2)][e & 3], v[g][e]);
                     }
                     if (t < members) {
                         const int64_t m = m0 + c.list[t];
 #pragma unroll
                         for (int g = 0; g < 2; ++g)
-                            store8(p.out, m * p.N + n0 + 32 * g + 8 * lq, p.out_bf16, p.N - (n0 + 32 * g + 8 * lq), v[i][g]);
+                            store8<FULL>(p.out, m * p.N + n0 + 32 * g + 8 * lq, p.out_bf16, p.N - (n0 + 32 * g + 8 * lq), v[g]);
                     }
                 }
+            };
+            if (n0 + 64 <= p.N)
+                columns(std::true_type{});
+            else
+                columns(std::false_type{});
         }
     }
 }
@@ -477,6 +511,14 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
 // ---------------------------------------------------------------- which kernels
 // Tokens of a chunk: 16 in a decode batch, whose adapters have few each; 32 and 64 for prompts, where a chunk's share of A and B is read again for each.
 int chunk_frags(int64_t M) { return M <= LR_WINDOW ? 1 : M < 8192 ? 2 : 4; }
+// Blocks that share a window's chunks: of a decode batch as many as there can be, of prompts as many as there are of one adapter,
+// or a few more.
+int chunk_slots(const LoraArgs &a, int mf)
+{
+    if (a.M <= LR_WINDOW)
+        return (int)(a.M < a.L + 1 + a.M / (16 * mf) ? a.M : a.L + 1 + a.M / (16 * mf));
+    return LR_WINDOW / (16 * mf) + (a.M < 8192 ? 2 : 0);
+}
 struct Plan {
     int mf, nf, groups, slots, splits;
     int64_t windows;
@@ -491,7 +533,7 @@ Plan lora_plan(const LoraArgs &a)
     p.nf = frags >= most ? most : frags >= 2 ? 2 : 1;
     p.groups = (frags + p.nf - 1) / p.nf;
     // a window's chunks: all of a decode batch at once, of prompts a few more than if they had one adapter
-    p.slots = a.M <= LR_WINDOW ? (int)a.M : LR_WINDOW / (16 * p.mf) + 4;
+    p.slots = chunk_slots(a, p.mf);
     // K is split until the chips' CUs have something to do, and no wave has less than a unit
     const int64_t chunks = a.M <= LR_WINDOW ? (a.M < a.L + a.M / 16 ? a.M : a.L + a.M / 16) : a.M / (16 * p.mf);
     const int64_t units = (a.K + (int8 ? 127 : 63)) / (int8 ? 128 : 64);
@@ -534,22 +576,23 @@ template <bool BF16, bool INT8> hipError_t shrink_mf(int mf, int nf, const Shrin
     return mf == 1 ? shrink_nf<BF16, INT8, 1>(nf, a, blocks, s) : mf == 2 ? shrink_nf<BF16, INT8, 2>(nf, a, blocks, s)
                                                                           : shrink_nf<BF16, INT8, 4>(nf, a, blocks, s);
 }
-template <bool BF16, int MF> hipError_t expand_ks(const ExpandArgs &a, uint32_t blocks, hipStream_t s)
+template <bool BF16, bool WIDE, int MF> hipError_t expand_ks(const ExpandArgs &a, uint32_t blocks, hipStream_t s)
 {
     const dim3 grid(blocks), block(LR_THREADS);
     if (a.R <= 32)
-        hipLaunchKernelGGL((lora_expand_kernel<BF16, 1, MF>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((lora_expand_kernel<BF16, WIDE, 1, MF>), grid, block, 0, s, a);
     else if (a.R <= 64)
-        hipLaunchKernelGGL((lora_expand_kernel<BF16, 2, MF>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((lora_expand_kernel<BF16, WIDE, 2, MF>), grid, block, 0, s, a);
     else if (a.R <= 128)
-        hipLaunchKernelGGL((lora_expand_kernel<BF16, 4, MF>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((lora_expand_kernel<BF16, WIDE, 4, MF>), grid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((lora_expand_kernel<BF16, 8, (MF < 4 ? MF : 2)>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((lora_expand_kernel<BF16, WIDE, 8, (MF < 4 ? MF : 2)>), grid, block, 0, s, a);
     return hipGetLastError();
 }
-template <bool BF16> hipError_t expand(int mf, const ExpandArgs &a, uint32_t blocks, hipStream_t s)
+template <bool BF16, bool WIDE> hipError_t expand(int mf, const ExpandArgs &a, uint32_t blocks, hipStream_t s)
 {
-    return mf == 1 ? expand_ks<BF16, 1>(a, blocks, s) : mf == 2 ? expand_ks<BF16, 2>(a, blocks, s) : expand_ks<BF16, 4>(a, blocks, s);
+    return mf == 1 ? expand_ks<BF16, WIDE, 1>(a, blocks, s) : mf == 2 ? expand_ks<BF16, WIDE, 2>(a, blocks, s)
+                                                                      : expand_ks<BF16, WIDE, 4>(a, blocks, s);
 }
 
 }  // namespace
@@ -573,7 +616,7 @@ hipError_t launch_lora_add(const LoraArgs &a, void *ws, hipStream_t s)
                         : (int8 ? shrink_mf<false, true>(p.mf, p.nf, sa, blocks, s) : shrink_mf<false, false>(p.mf, p.nf, sa, blocks, s));
     if (e != hipSuccess)
         return e;
-    const int mf = a.R > 128 && p.mf > 2 ? 2 : p.mf, slots = a.M <= LR_WINDOW ? (int)a.M : LR_WINDOW / (16 * mf) + 4;
+    const int mf = a.R > 128 && p.mf > 2 ? 2 : p.mf, slots = chunk_slots(a, mf);
     ExpandArgs ea{a.base, a.b, reinterpret_cast<const float *>(ws), a.xs, a.scaling, a.ids, a.out, a.M, a.base_stride, a.N, a.R, a.L,
                   (int16_t)p.splits, (int16_t)slots, 1, a.base_dtype, (int8_t)(a.out_dtype == LORA_BF16)};
     // a block's columns: the more, the seldomer z is laid out
@@ -582,7 +625,9 @@ hipError_t launch_lora_add(const LoraArgs &a, void *ws, hipStream_t s)
     const int64_t n_blocks = (a.N + 256 * ea.tiles - 1) / (256 * ea.tiles), eb = p.windows * slots * n_blocks;
     if (eb * LR_THREADS > 0xffffffffll)
         return hipErrorInvalidValue;
-    return bf16 ? expand<true>(mf, ea, (uint32_t)eb, s) : expand<false>(mf, ea, (uint32_t)eb, s);
+    if (a.base_dtype == LORA_FP32)
+        return bf16 ? expand<true, true>(mf, ea, (uint32_t)eb, s) : expand<false, true>(mf, ea, (uint32_t)eb, s);
+    return bf16 ? expand<true, false>(mf, ea, (uint32_t)eb, s) : expand<false, false>(mf, ea, (uint32_t)eb, s);
 }
 
 }  // namespace cam
