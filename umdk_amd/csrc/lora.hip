@@ -57,64 +57,104 @@ template <bool BF16> __device__ __forceinline__ u32x2 bytes4(uint32_t d)
 }
 
 // ---------------------------------------------------------------- chunks
-// The tokens of a window by chunks: chunk q holds up to SIZE tokens of one adapter (of none: id -1, last of all sorted as any other).
+// The tokens of a window by chunks: chunk q holds up to SIZE tokens of one adapter, or of none (id -1).  A token's rank is the
+// number of earlier ones with its adapter: those of its wave by ballots, an adapter of the wave at a time, those of earlier
+// waves from a table (open addressing; where an adapter lies in it hangs on the order of the waves, but nothing else
+// does: all blocks of a window, and both kernels, number its chunks alike).
+constexpr int LR_TABLE = 2 * LR_WINDOW, LR_EMPTY = -2;
 struct Chunks {
-    int32_t id[LR_WINDOW];      // adapter, -1 for none
+    int32_t key[LR_TABLE];
+    uint8_t tokens[LR_TABLE][LR_WAVES];  // of an adapter, in each wave
     int32_t count[LR_WAVES];
-    int32_t at, members, adapter;  // of the chunk asked for
+    int32_t at, place;  // of the chunk asked for: its first rank, its adapter's place in the table
     int32_t list[LR_WINDOW];
 };
-// This thread's token's place: (the chunk's number if it is the chunk's first, its rank among its adapter's); returns the number of chunks.
-__device__ __forceinline__ int find_chunks(Chunks &c, const int32_t *ids, int64_t m0, int n, int L, int size, int &rank, int &before)
+// This thread's token: its adapter's place, its rank, the number of the chunk that it leads (-1: none)
+struct Token {
+    int place, rank, leads;
+};
+// returns the number of chunks
+__device__ __forceinline__ int find_chunks(Chunks &c, const int32_t *ids, int64_t m0, int n, int L, int size, Token &tok)
 {
-    const int j = threadIdx.x;
-    int a = -2;
-    if (j < n) {
+    const int j = threadIdx.x, lane = j & 63, w = __builtin_amdgcn_readfirstlane(j >> 6);
+    int a = LR_EMPTY;
+    if (j < n)
         a = ids[m0 + j];
-        a = a < 0 || a >= L ? -1 : a;
-    }
-    c.id[j] = a;
-    __syncthreads();
-    rank = 0;
-    const int waves_end = min((j & ~63) + 64, n);  // (as far as any token of the wave looks)
-    for (int i = 0; i < waves_end; i += 4) {
-        const i32x4 v = *reinterpret_cast<const i32x4 *>(&c.id[i]);
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            rank += (v[q] == a) & (i + q < j);
+    for (int i = 0; i < LR_TABLE; i += LR_THREADS) {
+        c.key[i + j] = LR_EMPTY;
+        reinterpret_cast<uint32_t *>(c.tokens)[i + j] = 0;
     }
-    const bool leads = j < n && (rank & (size - 1)) == 0;
+    if (j < n)
+        a = a < 0 || a >= L ? -1 : a;
+    // among the wave
+    tok.rank = -1;
+    int leader = lane, same = 0;
+    for (uint64_t left = __ballot(j < n); left;) {
+        const int first = __builtin_ctzll(left);
+        const uint64_t m = __ballot(a == __builtin_amdgcn_readlane(a, first));
+        if (m >> lane & 1) {
+            leader = first;
+            tok.rank = __popcll(m & lanemask_lt());
+            same = __popcll(m);
+        }
+        left &= ~m;
+    }
+    __syncthreads();
+    int place = 0;
+    if (j < n && leader == lane) {
+        place = (int)((uint32_t)a * 0x9E3779B1u >> 23);
+        static_assert(LR_TABLE == 1 << 9, "the hash's bits");
+        for (;;) {  // (at most 256 of the 512 places are taken)
+            const int there = atomicCAS(&c.key[place], LR_EMPTY, a);
+            if (there == LR_EMPTY || there == a)
+                break;
+            place = (place + 1) & (LR_TABLE - 1);
+        }
+        c.tokens[place][w] = (uint8_t)same;
+    }
+    tok.place = j < n ? __shfl(place, leader, 64) : -1;
+    __syncthreads();
+    if (j < n) {
+#pragma unroll
+        for (int v = 0; v < LR_WAVES; ++v)
+            tok.rank += v < w ? c.tokens[tok.place][v] : 0;
+    }
+    const bool leads = j < n && (tok.rank & (size - 1)) == 0;
     const uint64_t mask = __ballot(leads);
-    if ((j & 63) == 0)
-        c.count[j >> 6] = __popcll(mask);
+    if (lane == 0)
+        c.count[w] = __popcll(mask);
     __syncthreads();
     int total = 0;
-    before = __popcll(mask & lanemask_lt());
+    tok.leads = __popcll(mask & lanemask_lt());
 #pragma unroll
-    for (int w = 0; w < LR_WAVES; ++w) {
-        before += w < (j >> 6) ? c.count[w] : 0;
-        total += c.count[w];
+    for (int v = 0; v < LR_WAVES; ++v) {
+        tok.leads += v < w ? c.count[v] : 0;
+        total += c.count[v];
     }
     if (!leads)
-        before = -1;
-    return total;
+        tok.leads = -1;
+    return __builtin_amdgcn_readfirstlane(total);
 }
-// chunk q's tokens into c.list, their number and adapter
-__device__ __forceinline__ void take_chunk(Chunks &c, int n, int size, int q, int rank, int before)
+// chunk q's tokens into c.list; its adapter (-1: none) and how many they are
+__device__ __forceinline__ int take_chunk(Chunks &c, int size, int q, const Token &tok, int &members)
 {
-    const int j = threadIdx.x;
-    __syncthreads();  // (the last chunk has been read)
-    if (before == q) {
-        c.adapter = c.id[j];
-        c.at = rank;
-        c.members = 0;
+    if (tok.leads == q) {
+        c.place = tok.place;
+        c.at = tok.rank;
     }
     __syncthreads();
-    if (j < n && c.id[j] == c.adapter && rank >= c.at && rank < c.at + size) {
-        c.list[rank - c.at] = j;
-        atomicMax(&c.members, rank - c.at + 1);
-    }
+    const int place = __builtin_amdgcn_readfirstlane(c.place), at = __builtin_amdgcn_readfirstlane(c.at);
+    if (tok.place == place && tok.rank >= at && tok.rank < at + size)
+        c.list[tok.rank - at] = threadIdx.x;
+    int all = 0;
+#pragma unroll
+    for (int v = 0; v < LR_WAVES; ++v)
+        all += c.tokens[place][v];
+    members = __builtin_amdgcn_readfirstlane(min(size, all - at));
+    const int adapter = __builtin_amdgcn_readfirstlane(c.key[place]);
     __syncthreads();
+    return adapter;
 }
 
 // ---------------------------------------------------------------- A x
@@ -169,8 +209,8 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const ShrinkArg
     const int first = id % p.slots;
     const int64_t m0 = (int64_t)(id / p.slots) * LR_WINDOW;
     const int n = (int)min((int64_t)LR_WINDOW, p.M - m0);
-    int rank, before;
-    const int chunks = find_chunks(c, p.ids, m0, n, p.L, 16 * MF, rank, before);
+    Token tok;
+    const int chunks = find_chunks(c, p.ids, m0, n, p.L, 16 * MF, tok);
 
     const int K = p.K, x_bytes = INT8 ? K : 2 * K, a_bytes = 2 * K;
     const int units = (K + UNIT - 1) / UNIT, from = units * split / p.splits, to = units * (split + 1) / p.splits;
@@ -178,8 +218,8 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const ShrinkArg
     uint8_t *ring = smem + w * SLOTS * SLOT;
     const int turned = (lane & 7) ^ (lane >> 4);  // in even bands of 8 rows; odd ones: ^ 4
     for (int q = first; q < chunks; q += p.slots) {
-        take_chunk(c, n, 16 * MF, q, rank, before);
-        const int adapter = c.adapter, members = c.members;
+        int members;
+        const int adapter = take_chunk(c, 16 * MF, q, tok, members);
         if (adapter < 0)
             continue;
         const uint8_t *xr[2 * MF], *ar[2 * NF];
@@ -376,11 +416,43 @@ template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_
     const int first = id % p.slots;
     const int64_t m0 = (int64_t)(id / p.slots) * LR_WINDOW;
     const int n = (int)min((int64_t)LR_WINDOW, p.M - m0);
-    int rank, before;
-    const int chunks = find_chunks(c, p.ids, m0, n, p.L, 16 * MF, rank, before);
+    Token tok;
+    const int chunks = find_chunks(c, p.ids, m0, n, p.L, 16 * MF, tok);
     for (int q = first; q < chunks; q += p.slots) {
-        take_chunk(c, n, 16 * MF, q, rank, before);
-        const int adapter = c.adapter, members = c.members;
+        int members;
+        const int adapter = take_chunk(c, 16 * MF, q, tok, members);
+        const auto column_of = [&](int tile) { return n_block * span + (tile * LR_WAVES + w) * 64; };
+        u32x4 bf[4][KS];
+        Raw8<WIDE> raw[MF][2];
+        const auto load_tile = [&](int n0) {
+            if (adapter >= 0) {
+#pragma unroll
+                for (int f = 0; f < 4; ++f) {
+                    const int col = min(n0 + 32 * (f >> 1) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3), p.N - 1);
+                    const uint16_t *row = reinterpret_cast<const uint16_t *>(p.b) + ((int64_t)adapter * p.N + col) * p.R;
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)  // (past the rank: the last of it, for now)
+                        bf[f][s] = *reinterpret_cast<const u32x4 *>(row + min(s * 32 + lq * 8, p.R - 8));
+                }
+            }
+            // (all of base before any output: out may be base, so that no load would pass a store)
+            const auto base = [&](auto all_there) {
+#pragma unroll
+                for (int i = 0; i < MF; ++i) {
+                    const int64_t m = m0 + c.list[min(i * 16 + l16, members - 1)];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+                        raw[i][g] = load8<WIDE, decltype(all_there)::value>(p.base, m * p.base_stride + n0 + 32 * g + 8 * lq,
+                                                                            p.N - (n0 + 32 * g + 8 * lq));
+                }
+            };
+            if (n0 + 64 <= p.N)
+                base(std::true_type{});
+            else
+                base(std::false_type{});
+        };
+        if (column_of(0) < p.N)  // (on its way while z is laid out)
+            load_tile(column_of(0));
         if (adapter >= 0) {
             // 4 KS threads a token, 8 values each
             for (int i = threadIdx.x; i < 16 * MF * 4 * KS; i += LR_THREADS) {
@@ -439,71 +511,62 @@ template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_
         }
         __syncthreads();
         for (int tile = 0; tile < p.tiles; ++tile) {
-            const int n0 = n_block * span + (tile * LR_WAVES + w) * 64;
+            const int n0 = column_of(tile);
             if (n0 >= p.N)
                 break;
-            u32x4 bf[4][KS];
-            if (adapter >= 0) {
+            if (tile > 0)
+                load_tile(n0);
+            if (32 * KS > p.R) {
 #pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    const int col = min(n0 + 32 * (f >> 1) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3), p.N - 1);
-                    const uint16_t *row = reinterpret_cast<const uint16_t *>(p.b) + ((int64_t)adapter * p.N + col) * p.R;
-#pragma unroll
-                    for (int s = 0; s < KS; ++s)  // (past the rank: nothing, whatever lies there)
-                        bf[f][s] = s * 32 + lq * 8 < p.R ? *reinterpret_cast<const u32x4 *>(row + s * 32 + lq * 8) : u32x4{0, 0, 0, 0};
-                }
-            }
-            const auto columns = [&](auto all_there) {
-                constexpr bool FULL = decltype(all_there)::value;
-                // (all of base first: out may be base, so that no load would pass a store)
-                Raw8<WIDE> raw[MF][2];
-#pragma unroll
-                for (int i = 0; i < MF; ++i) {
-                    const int64_t m = m0 + c.list[min(i * 16 + l16, members - 1)];
-#pragma unroll
-                    for (int g = 0; g < 2; ++g)
-                        raw[i][g] = load8<WIDE, FULL>(p.base, m * p.base_stride + n0 + 32 * g + 8 * lq, p.N - (n0 + 32 * g + 8 * lq));
-                }
-#pragma unroll
-                for (int i = 0; i < MF; ++i) {
-                    const int t = i * 16 + l16;
-                    float v[2][8];
-#pragma unroll
-                    for (int g = 0; g < 2; ++g)
-                        to_fp32<WIDE>(raw[i][g], p.base_dtype == LORA_BF16, v[g]);
-                    if (adapter >= 0) {
-                        f32x4 acc[4];
+                for (int s = 0; s < KS; ++s)
+                    if (s * 32 + lq * 8 >= p.R) {  // (whatever lies past the rank)
 #pragma unroll
                         for (int f = 0; f < 4; ++f)
-                            acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int s = 0; s < KS; ++s)
-#pragma unroll
-                            for (int part = 0; part < 2; ++part) {
-                                const u32x4 z = zs[i][s][part][lane];
-#pragma unroll
-                                for (int f = 0; f < 4; ++f)
-                                    acc[f] = mfma<BF16>(bf[f][s], z, acc[f]);
-                            }
-                        const float scale = factor[t];
-#pragma unroll
-                        for (int g = 0; g < 2; ++g)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                v[g][e] = __builtin_fmaf(scale, acc[2 * g + (e >> 2)][e & 3], v[g][e]);
+                            bf[f][s] = u32x4{0, 0, 0, 0};
                     }
-                    if (t < members) {
-                        const int64_t m = m0 + c.list[t];
+            }
 #pragma unroll
-                        for (int g = 0; g < 2; ++g)
-                            store8<FULL>(p.out, m * p.N + n0 + 32 * g + 8 * lq, p.out_bf16, p.N - (n0 + 32 * g + 8 * lq), v[g]);
+            for (int i = 0; i < MF; ++i) {
+                if (i * 16 >= members)
+                    break;
+                const int t = i * 16 + l16;
+                float v[2][8];
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+                    to_fp32<WIDE>(raw[i][g], p.base_dtype == LORA_BF16, v[g]);
+                if (adapter >= 0) {
+                    f32x4 acc[4];
+#pragma unroll
+                    for (int f = 0; f < 4; ++f)
+                        acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s)
+#pragma unroll
+                        for (int part = 0; part < 2; ++part) {
+                            const u32x4 z = zs[i][s][part][lane];
+#pragma unroll
+                            for (int f = 0; f < 4; ++f)
+                                acc[f] = mfma<BF16>(bf[f][s], z, acc[f]);
+                        }
+                    const float scale = factor[t];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            v[g][e] = __builtin_fmaf(scale, acc[2 * g + (e >> 2)][e & 3], v[g][e]);
+                }
+                if (t < members) {
+                    const int64_t m = m0 + c.list[t];
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        const int col = n0 + 32 * g + 8 * lq;
+                        if (n0 + 64 <= p.N)
+                            store8<true>(p.out, m * p.N + col, p.out_bf16, 8, v[g]);
+                        else
+                            store8<false>(p.out, m * p.N + col, p.out_bf16, p.N - col, v[g]);
                     }
                 }
-            };
-            if (n0 + 64 <= p.N)
-                columns(std::true_type{});
-            else
-                columns(std::false_type{});
+            }
         }
     }
 }
@@ -537,7 +600,7 @@ Plan lora_plan(const LoraArgs &a)
     // K is split until the chips' CUs have something to do, and no wave has less than a unit
     const int64_t chunks = a.M <= LR_WINDOW ? (a.M < a.L + a.M / 16 ? a.M : a.L + a.M / 16) : a.M / (16 * p.mf);
     const int64_t units = (a.K + (int8 ? 127 : 63)) / (int8 ? 128 : 64);
-    int64_t s = 256 / (chunks * p.groups > 0 ? chunks * p.groups : 1);
+    int64_t s = 512 / (chunks * p.groups > 0 ? chunks * p.groups : 1);
     s = s < units / LR_WAVES ? s : units / LR_WAVES;
     p.splits = (int)(s < 1 ? 1 : s > LR_MAX_SPLITS ? LR_MAX_SPLITS : s);
     return p;
@@ -546,7 +609,7 @@ Plan lora_plan(const LoraArgs &a)
 constexpr int LR_MAX_DEVICES = 64;
 template <bool BF16, bool INT8, int MF, int NF> hipError_t shrink(const ShrinkArgs &a, int64_t blocks, hipStream_t s)
 {
-    constexpr int SLOT = (2 * NF * (INT8 ? 2 : 1) + 2 * MF) * 1024, SLOTS = SLOT <= 4096 ? 4 : SLOT <= 8192 ? 3 : 2, LDS = LR_WAVES * SLOTS * SLOT;
+    constexpr int SLOT = (2 * NF * (INT8 ? 2 : 1) + 2 * MF) * 1024, SLOTS = SLOT <= 4096 ? 4 : SLOT <= 10240 ? 2 : 1, LDS = LR_WAVES * SLOTS * SLOT;
     static std::atomic<bool> done[LR_MAX_DEVICES];  // the kernel's dynamic LDS limit is raised once per device
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
