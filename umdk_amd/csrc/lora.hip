@@ -25,7 +25,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int LR_WINDOW = 256, LR_WAVES = 4, LR_THREADS = 64 * LR_WAVES;
-constexpr int LR_MAX_SPLITS = 16;
+constexpr int LR_MAX_SPLITS = 8;
 static_assert(LR_THREADS == LR_WINDOW, "a thread per token of the window");
 
 // two fp32 -> two 16-bit numbers, the nearest
@@ -463,7 +463,7 @@ template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_
                     z[e] = 0.0f;
                 const int64_t m = m0 + c.list[min(t, members - 1)];
                 if (r < p.R) {
-                    constexpr int AT_ONCE = 4;
+                    constexpr int AT_ONCE = MF == 4 ? 2 : LR_MAX_SPLITS;  // (many rows: few splits, and registers are waves)
                     for (int s0 = 0; s0 < p.splits; s0 += AT_ONCE) {
                         f32x4 v[AT_ONCE][2];
 #pragma unroll

@@ -579,6 +579,12 @@ def moe_decode_layer(x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weigh
     token's results are the same bits in any batch.  No backward: inputs that
     ask for a gradient are refused in grad mode, those with a forward-mode
     tangent too."""
+    out = (_lib._tensor_caller or _lib._tensors()).moe_decode_layer(
+        x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weight, gmm2_weight_scale, topk, n_group, topk_group,
+        score_func, group_score, renormalize, routed_scaling, share_gmm1_weight, share_gmm1_weight_scale,
+        share_gmm2_weight, share_gmm2_weight_scale, x_active_mask)
+    if out is not None:
+        return out
     T, H, E, I, Is = _moe_decode_check(x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weight, gmm2_weight_scale,
                                        topk, score_func, group_score, share_gmm1_weight, share_gmm1_weight_scale,
                                        share_gmm2_weight, share_gmm2_weight_scale, x_active_mask)
@@ -638,6 +644,9 @@ def lora_add(base, x, lora_a, lora_b, adapter_ids, scaling=None, x_scale=None, o
     out [m, n] in out_dtype (by default base's, lora_a's for a float32 base).
     No backward: inputs that ask for a gradient are refused in grad mode,
     those with a forward-mode tangent too."""
+    out = (_lib._tensor_caller or _lib._tensors()).lora_add(base, x, lora_a, lora_b, adapter_ids, scaling, x_scale, out_dtype)
+    if out is not None:
+        return out
     m, n, k, L, r, out_dtype = _lora_check(base, x, lora_a, lora_b, adapter_ids, scaling, x_scale, out_dtype)
     index = _device_index("lora_add", base, x, lora_a, lora_b, adapter_ids, scaling, x_scale)
 

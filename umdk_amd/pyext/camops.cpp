@@ -1,5 +1,6 @@
-// The ordinary call of the operators around the expert layer (grouped routing, residual norm, int8 product) from tensors
-// to launch in one native call: their smallest calls are bound by the host.  In Python the checks and the outputs of one
+// The ordinary call of the operators around the expert layer (grouped routing, residual norm, int8 product) and of those of a
+// decode step of a few requests (whole expert layer, low-rank adapters) from tensors to launch in one native call: their
+// smallest calls are bound by the host.  In Python the checks and the outputs of one
 // take 3 to 5 us beside a launch of 2.8 (small calls: routing 6.5, norm 8.0, product 6.4 us; through this 5.1, 5.8, 4.3).
 //
 // A function returns None, having done nothing, for a call that is not ordinary: other types, strides, devices, a gradient
@@ -29,8 +30,11 @@ decltype(&camhipGetLastErrorMsg) g_last_error = nullptr;
 decltype(&camhipMoeRouteGroupedGetWorkspaceSize) g_get_route = nullptr;
 decltype(&camhipAddRmsNormGetWorkspaceSize) g_get_norm = nullptr;
 decltype(&camhipQuantMatmulGetWorkspaceSize) g_get_qmm = nullptr;
+decltype(&camhipMoeDecodeLayerGetWorkspaceSize) g_get_layer = nullptr;
+decltype(&camhipLoraAddGetWorkspaceSize) g_get_lora = nullptr;
+decltype(&camhipReleaseExecutor) g_release = nullptr;
 using RunFn = camhipStatus (*)(void *, uint64_t, camhipExecutor *, void *);
-RunFn g_run_route = nullptr, g_run_norm = nullptr, g_run_qmm = nullptr;
+RunFn g_run_route = nullptr, g_run_norm = nullptr, g_run_qmm = nullptr, g_run_layer = nullptr, g_run_lora = nullptr;
 
 // A tensor of a call: plain, on the GPU, without a gradient to be recorded.  nullptr: not ordinary.
 const at::Tensor *plain(PyObject *o)
@@ -103,15 +107,27 @@ int current_stream(std::initializer_list<const at::Tensor *> tensors, void *&str
     return PyErr_Occurred() ? -1 : 1;
 }
 
-bool launch(const char *name, RunFn run, camhipExecutor *ex, void *stream)
+bool launch(const char *name, RunFn run, camhipExecutor *ex, void *stream, void *workspace = nullptr, uint64_t bytes = 0)
 {
     camhipStatus st;
     Py_BEGIN_ALLOW_THREADS
-    st = run(nullptr, 0, ex, stream);
+    st = run(workspace, bytes, ex, stream);
     Py_END_ALLOW_THREADS
     if (st != CAMHIP_SUCCESS)
         PyErr_Format(g_error, "%s failed (%d): %s", name, (int)st, g_last_error());
     return st == CAMHIP_SUCCESS;
+}
+// the same with a workspace, of torch's allocator
+bool launch_ws(const char *name, RunFn run, camhipExecutor *ex, void *stream, uint64_t bytes, const at::Tensor &like)
+{
+    at::Tensor ws;
+    try {
+        ws = at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
+    } catch (...) {
+        g_release(ex);
+        throw;
+    }
+    return launch(name, run, ex, stream, bytes ? ws.mutable_data_ptr() : nullptr, bytes);
 }
 PyObject *tuple_of(std::initializer_list<at::Tensor> tensors)
 {
@@ -221,6 +237,104 @@ PyObject *quant_matmul(PyObject *, PyObject *const *a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+// a weight [lead..., n, k] with its scales: none (bf16), [lead..., n] (int8), [lead..., n / 128, k / 128] (fp8)
+bool weight_of(const at::Tensor *w, const at::Tensor *s, at::ScalarType type, at::IntArrayRef shape)
+{
+    if (w->scalar_type() != type || w->sizes() != shape || !w->is_contiguous())
+        return false;
+    if (type == at::kBFloat16)
+        return !s;
+    if (!s || !is_fp32(*s) || !s->is_contiguous())
+        return false;
+    const size_t d = shape.size();
+    if (type == at::kChar)
+        return s->sizes() == shape.slice(0, d - 1);
+    if (s->dim() != (int64_t)d)
+        return false;
+    for (size_t i = 0; i < d; ++i)
+        if (s->size((int64_t)i) != (i + 2 < d ? shape[i] : shape[i] / 128))
+            return false;
+    return true;
+}
+template <typename T = void> T *ptr(const at::Tensor *t) { return t ? (T *)t->const_data_ptr() : nullptr; }
+
+// x, router, bias, w1, s1, w2, s2, topk, n_group, topk_group, score_func, group_score, renormalize, routed_scaling, share w1, s1,
+// w2, s2, active mask
+PyObject *moe_decode_layer(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    ORDINARY(n == 19 && g_error);
+    const at::Tensor *x = plain(a[0]), *router = plain(a[1]), *w1 = plain(a[3]), *w2 = plain(a[5]);
+    const at::Tensor *bias, *s1, *s2, *sw1, *ss1, *sw2, *ss2, *mask;
+    int64_t K, G, KG;
+    double scaling;
+    ORDINARY(x && router && w1 && w2 && optional(a[2], bias) && optional(a[4], s1) && optional(a[6], s2) && optional(a[14], sw1) &&
+             optional(a[15], ss1) && optional(a[16], sw2) && optional(a[17], ss2) && optional(a[18], mask));
+    ORDINARY(integer(a[7], K) && integer(a[8], G) && integer(a[9], KG) && PyBool_Check(a[12]) && number(a[13], scaling));
+    const bool softmax = is_string(a[10], "softmax"), top2 = is_string(a[11], "top2");
+    ORDINARY((softmax || is_string(a[10], "sigmoid")) && (top2 || is_string(a[11], "max")));
+    ORDINARY(x->dim() == 2 && x->scalar_type() == at::kBFloat16 && x->is_contiguous() && w1->dim() == 3 && K > 0 && K <= 16);
+    const int64_t T = x->size(0), H = x->size(1), E = w1->size(0), I = w1->size(1) / 2;
+    const at::ScalarType type = w1->scalar_type();
+    ORDINARY(T <= 16 && w1->size(1) % 2 == 0 && (type == at::kBFloat16 || type == at::kChar || type == at::kFloat8_e4m3fn));
+    ORDINARY(router->dim() == 2 && router->size(0) == E && router->size(1) == H && router->is_contiguous() &&
+             (is_fp32(*router) || router->scalar_type() == at::kBFloat16));
+    ORDINARY(!bias || (is_fp32(*bias) && vector_of(*bias, E)));
+    ORDINARY(!mask || (mask->scalar_type() == at::kBool && vector_of(*mask, T)));
+    ORDINARY(weight_of(w1, s1, type, {E, 2 * I, H}) && weight_of(w2, s2, type, {E, H, I}));
+    ORDINARY(!sw1 == !sw2 && (sw1 || (!ss1 && !ss2)));
+    int64_t Is = 0;
+    if (sw1) {
+        ORDINARY(sw1->dim() == 2 && sw1->size(0) > 0 && sw1->size(0) % 2 == 0);
+        Is = sw1->size(0) / 2;
+        ORDINARY(weight_of(sw1, ss1, type, {2 * Is, H}) && weight_of(sw2, ss2, type, {H, Is}));
+    }
+    STREAM(stream, x, router, bias, w1, s1, w2, s2, sw1, ss1, sw2, ss2, mask);
+    const auto opt = x->options();
+    at::Tensor out = at::empty({T, H}, opt), idx = at::empty({T, K}, opt.dtype(at::kInt)), w = at::empty({T, K}, opt.dtype(at::kFloat));
+    uint64_t need = 0;
+    camhipExecutor *ex = nullptr;
+    ORDINARY(g_get_layer(ptr<const uint16_t>(x), ptr(router), ptr<const float>(bias), ptr(w1), ptr<const float>(s1), ptr(w2),
+                         ptr<const float>(s2), ptr(sw1), ptr<const float>(ss1), ptr(sw2), ptr<const float>(ss2),
+                         ptr<const uint8_t>(mask), T, H, E, 2 * I, 2 * Is, K,
+                         type == at::kBFloat16 ? CAMHIP_DTYPE_BF16 : type == at::kChar ? CAMHIP_DTYPE_INT8 : CAMHIP_DTYPE_FP8,
+                         code(router->scalar_type()), G, KG, softmax ? CAMHIP_ROUTE_SOFTMAX : CAMHIP_ROUTE_SIGMOID,
+                         top2 ? CAMHIP_ROUTE_GROUP_TOP2 : CAMHIP_ROUTE_GROUP_MAX, a[12] == Py_True, scaling,
+                         (uint16_t *)out.mutable_data_ptr(), (int32_t *)idx.mutable_data_ptr(), (float *)w.mutable_data_ptr(), &need,
+                         &ex) == CAMHIP_SUCCESS);
+    return launch_ws("camhipMoeDecodeLayer", g_run_layer, ex, stream, need, *x) ? tuple_of({out, idx, w}) : nullptr;
+    END_HANDLE_TH_ERRORS
+}
+
+// base, x, lora_a, lora_b, adapter_ids, scaling, x_scale, out_dtype
+PyObject *lora_add(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    ORDINARY(n == 8 && g_error);
+    const at::Tensor *base = plain(a[0]), *x = plain(a[1]), *la = plain(a[2]), *lb = plain(a[3]), *ids = plain(a[4]), *scaling, *xs;
+    ORDINARY(base && x && la && lb && ids && optional(a[5], scaling) && optional(a[6], xs) && (a[7] == Py_None || THPDtype_Check(a[7])));
+    int64_t bstep, xstep;
+    ORDINARY(rows_of(*base, bstep) && rows_of(*x, xstep) && la->dim() == 3 && la->is_contiguous() && lb->is_contiguous());
+    const int64_t m = x->size(0), k = x->size(1), nn = base->size(1), L = la->size(0), r = la->size(1);
+    const at::ScalarType type = la->scalar_type(), bt = base->scalar_type();
+    const bool int8 = x->scalar_type() == at::kChar;
+    ORDINARY((type == at::kBFloat16 || type == at::kHalf) && (bt == at::kBFloat16 || bt == at::kHalf || bt == at::kFloat));
+    ORDINARY(base->size(0) == m && la->size(2) == k && lb->scalar_type() == type && lb->sizes() == at::IntArrayRef({L, nn, r}));
+    ORDINARY((int8 || x->scalar_type() == type) && int8 == (xs != nullptr) && (!xs || (is_fp32(*xs) && vector_of(*xs, m))));
+    ORDINARY(ids->scalar_type() == at::kInt && vector_of(*ids, m) && (!scaling || (is_fp32(*scaling) && vector_of(*scaling, L))));
+    const at::ScalarType ot = a[7] != Py_None ? reinterpret_cast<THPDtype *>(a[7])->scalar_type : bt == at::kFloat ? type : bt;
+    ORDINARY(ot == at::kBFloat16 || ot == at::kHalf);
+    STREAM(stream, base, x, la, lb, ids, scaling, xs);
+    at::Tensor out = at::empty({m, nn}, base->options().dtype(ot));
+    uint64_t need = 0;
+    camhipExecutor *ex = nullptr;
+    ORDINARY(g_get_lora(ptr(base), ptr(x), ptr<const float>(xs), ptr(la), ptr(lb), ptr<const int32_t>(ids), ptr<const float>(scaling), m, nn,
+                        k, r, L, bstep, xstep, code(bt), int8 ? CAMHIP_DTYPE_INT8 : code(type), code(type), code(ot),
+                        out.mutable_data_ptr(), &need, &ex) == CAMHIP_SUCCESS);
+    return launch_ws("camhipLoraAdd", g_run_lora, ex, stream, need, *base) ? THPVariable_Wrap(out) : nullptr;
+    END_HANDLE_TH_ERRORS
+}
+
 template <typename F> bool resolve(void *lib, const char *name, F &out)
 {
     out = (F)dlsym(lib, name);
@@ -241,7 +355,9 @@ PyObject *bind(PyObject *, PyObject *args)
         !resolve(lib, "camhipMoeRouteGrouped", g_run_route) ||
         !resolve(lib, "camhipAddRmsNormGetWorkspaceSize", g_get_norm) || !resolve(lib, "camhipAddRmsNorm", g_run_norm) ||
         !resolve(lib, "camhipQuantMatmulGetWorkspaceSize", g_get_qmm) || !resolve(lib, "camhipQuantMatmul", g_run_qmm) ||
-        !resolve(lib, "camhipGetLastErrorMsg", g_last_error))
+        !resolve(lib, "camhipMoeDecodeLayerGetWorkspaceSize", g_get_layer) || !resolve(lib, "camhipMoeDecodeLayer", g_run_layer) ||
+        !resolve(lib, "camhipLoraAddGetWorkspaceSize", g_get_lora) || !resolve(lib, "camhipLoraAdd", g_run_lora) ||
+        !resolve(lib, "camhipReleaseExecutor", g_release) || !resolve(lib, "camhipGetLastErrorMsg", g_last_error))
         return nullptr;
     Py_INCREF(device);
     Py_XSETREF(g_get_device, device);
@@ -253,7 +369,7 @@ PyObject *bind(PyObject *, PyObject *args)
 }
 
 #define METHOD(f) {#f, (PyCFunction)(void (*)(void))f, METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {METHOD(route_grouped), METHOD(add_rms_norm), METHOD(quant_matmul),
+PyMethodDef g_methods[] = {METHOD(route_grouped), METHOD(add_rms_norm), METHOD(quant_matmul), METHOD(moe_decode_layer), METHOD(lora_add),
                            {"bind", bind, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_camops", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
