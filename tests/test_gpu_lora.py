@@ -272,3 +272,36 @@ def test_gradients_are_refused_not_dropped():
             call(d, **{name: d[name].detach().clone().requires_grad_()})
     with torch.no_grad():
         call(d, x=d["x"].detach().clone().requires_grad_())
+
+
+@pytest.mark.parametrize("M,N,L,R,dtype,out", [
+    (9000, 2568, 5, 32, "bf16", None), (9000, 2568, 5, 8, "fp16", None), (8200, 4160, 7, 64, "bf16", torch.float16),
+    (8192, 4104, 3, 40, "fp16", torch.bfloat16), (3000, 4160, 4, 64, "fp16", None), (2900, 4232, 40, 32, "bf16", None),
+    (8300, 2600, 6, 128, "bf16", None), (8195, 2632, 3, 200, "fp16", None), (4100, 4168, 1, 256, "bf16", None),
+])
+def test_prompts_by_whole_lines(M, N, L, R, dtype, out):
+    """Aligned rows of 16 bits go by whole cache lines, others by a kernel that takes any: the same bits."""
+    d = make(M, 144, N, L, R, dtype, seed=M + R, runs=R != 32)
+    got = call(d, out)
+    check(d, got)
+    odd = torch.empty(M * N + 1, dtype=d["base"].dtype, device=DEV)[1:].view(M, N)
+    odd.copy_(d["base"])
+    assert torch.equal(call(d, out, base=odd), got)
+    wide = torch.full((M, N + 24), float("nan"), dtype=d["base"].dtype, device=DEV)
+    wide[:, 8:N + 8] = d["base"]
+    assert torch.equal(call(d, out, base=wide[:, 8:N + 8]), got)
+
+
+def test_prompts_in_place_of_the_base():
+    from umdk_amd import _lib
+    M, K, N, L, R = 8500, 64, 2696, 4, 16
+    d = make(M, K, N, L, R, seed=12, runs=True)
+    want = call(d)
+    guard = torch.full((M + 2, N), 7.0, dtype=torch.bfloat16, device=DEV)
+    guard[1:-1] = d["base"]
+    args = (guard[1:-1].data_ptr(), d["x"].data_ptr(), None, d["a"].data_ptr(), d["b"].data_ptr(), d["ids"].data_ptr(),
+            d["scaling"].data_ptr(), M, N, K, R, L, N, K, 0, 0, 0, 0, guard[1:-1].data_ptr())
+    ws = torch.empty(_lib.workspace_size("camhipLoraAdd", *args), dtype=torch.uint8, device=DEV)
+    _lib.launch("camhipLoraAdd", *args, workspace=ws)
+    torch.cuda.synchronize()
+    assert torch.equal(guard[1:-1], want) and (guard[0] == 7).all() and (guard[-1] == 7).all()

@@ -377,7 +377,7 @@ template <bool WIDE> __device__ __forceinline__ void to_fp32(const Raw8<WIDE> &r
             v[i] = unpack<false>(r.v[0][i >> 1], i & 1);
     }
 }
-template <bool FULL> __device__ __forceinline__ void store8(void *p, int64_t at, bool bf16, int left, const float *v)
+__device__ __forceinline__ u32x4 pack8(bool bf16, const float *v)
 {
     u32x4 r;
     if (bf16) {
@@ -389,6 +389,11 @@ template <bool FULL> __device__ __forceinline__ void store8(void *p, int64_t at,
         for (int i = 0; i < 4; ++i)
             r[i] = pack2<false>(v[2 * i], v[2 * i + 1]);
     }
+    return r;
+}
+template <bool FULL> __device__ __forceinline__ void store8(void *p, int64_t at, bool bf16, int left, const float *v)
+{
+    const u32x4 r = pack8(bf16, v);
     uint16_t *h = reinterpret_cast<uint16_t *>(p) + at;
     if constexpr (FULL) {
         *reinterpret_cast<u32x4_u *>(h) = r;
@@ -400,9 +405,122 @@ template <bool FULL> __device__ __forceinline__ void store8(void *p, int64_t at,
     }
 }
 
-// A chunk of up to 16 MF tokens by 64 columns a wave at a time.  z of the chunk lies in LDS as the instructions' second operand:
-// [token fragment][step of 32][first or second number][lane] 16 bytes.  Row i of the tile f of 64 columns is column
-// 32 (f / 2) + 8 (i / 4) + 4 (f mod 2) + i mod 4, so that a lane's results are twice 8 consecutive columns of one token.
+// z of a chunk into LDS as the instructions' second operand: [token fragment][step of 32][first or second number][lane] 16
+// bytes, and each token's factor
+template <bool BF16, int KS, int MF>
+__device__ __forceinline__ void lay_out(const ExpandArgs &p, const Chunks &c, int64_t m0, int members, int adapter,
+                                        u32x4 (&zs)[MF][KS][2][64], float (&factor)[16 * MF])
+{
+    // 4 KS threads a token, 8 values each
+    for (int i = threadIdx.x; i < 16 * MF * 4 * KS; i += LR_THREADS) {
+        const int t = i / (4 * KS), part = i % (4 * KS), r = part * 8;
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            z[e] = 0.0f;
+        const int64_t m = m0 + c.list[min(t, members - 1)];
+        if (r < p.R) {
+            constexpr int AT_ONCE = MF == 4 ? 2 : LR_MAX_SPLITS;  // (many rows: few splits, and registers are waves)
+            for (int s0 = 0; s0 < p.splits; s0 += AT_ONCE) {
+                f32x4 v[AT_ONCE][2];
+#pragma unroll
+                for (int s = 0; s < AT_ONCE; ++s) {
+                    const f32x4 *from = reinterpret_cast<const f32x4 *>(p.z + ((int64_t)min(s0 + s, p.splits - 1) * p.M + m) * p.R + r);
+                    v[s][0] = from[0];
+                    v[s][1] = from[1];
+                }
+#pragma unroll
+                for (int s = 0; s < AT_ONCE; ++s)
+                    if (s0 + s < p.splits) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            z[e] += v[s][e >> 2][e & 3];
+                    }
+            }
+        }
+        float f = p.scaling ? p.scaling[adapter] : 1.0f;
+        if (p.xs)
+            f *= p.xs[m];
+        if constexpr (!BF16) {  // the row's largest to 2^10 or a little less: what is left out then keeps its bits
+            float most = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                most = fmaxf(most, fabsf(z[e]));
+            most = KS == 8 ? group_max<32>(most) : KS == 4 ? group_max<16>(most) : KS == 2 ? group_max<8>(most) : group_max<4>(most);
+            const bool plain = most > 0.0f && most < INFINITY;
+            const int e2 = plain ? 10 - ilogbf(most) : 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                z[e] = ldexpf(z[e], e2);
+            f = ldexpf(f, -e2);
+        }
+        u32x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            hi[e] = pack2<BF16>(z[2 * e], z[2 * e + 1]);
+            lo[e] = pack2<BF16>(z[2 * e] - unpack<BF16>(hi[e], 0), z[2 * e + 1] - unpack<BF16>(hi[e], 1));
+        }
+        zs[t >> 4][part >> 2][0][(part & 3) * 16 + (t & 15)] = hi;
+        zs[t >> 4][part >> 2][1][(part & 3) * 16 + (t & 15)] = lo;
+        if (part == 0)
+            factor[t] = f;
+    }
+}
+// B's rows of a tile of 64 columns from n0 on.  Row i of fragment f is column 32 (f / 2) + 8 (i / 4) + 4 (f mod 2) + i mod 4,
+// so that a lane's results are twice 8 consecutive columns of one token.
+template <int KS> struct Tile {
+    u32x4 v[4][KS];
+};
+template <int KS> __device__ __forceinline__ Tile<KS> load_b(const ExpandArgs &p, int adapter, int n0, int l16, int lq)
+{
+    Tile<KS> t;
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+        const int col = min(n0 + 32 * (f >> 1) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3), p.N - 1);
+        const uint16_t *row = reinterpret_cast<const uint16_t *>(p.b) + ((int64_t)adapter * p.N + col) * p.R;
+#pragma unroll
+        for (int s = 0; s < KS; ++s)  // (past the rank: the last of it, for now)
+            t.v[f][s] = *reinterpret_cast<const u32x4 *>(row + min(s * 32 + lq * 8, p.R - 8));
+    }
+    return t;
+}
+template <int KS> __device__ __forceinline__ void clear_past_rank(Tile<KS> &t, int R, int lq)
+{
+    if (32 * KS > R) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+            if (s * 32 + lq * 8 >= R) {
+#pragma unroll
+                for (int f = 0; f < 4; ++f)
+                    t.v[f][s] = u32x4{0, 0, 0, 0};
+            }
+    }
+}
+// a fragment of 16 tokens' z times a tile of B, scaled, added to v
+template <bool BF16, int KS>
+__device__ __forceinline__ void add_product(const Tile<KS> &b, const u32x4 (&z)[KS][2][64], float scale, int lane, float (&v)[2][8])
+{
+    f32x4 acc[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+        acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            const u32x4 zv = z[s][part][lane];
+#pragma unroll
+            for (int f = 0; f < 4; ++f)
+                acc[f] = mfma<BF16>(b.v[f][s], zv, acc[f]);
+        }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[g][e] = __builtin_fmaf(scale, acc[2 * g + (e >> 2)][e & 3], v[g][e]);
+}
+
+// A chunk of up to 16 MF tokens by 64 columns a wave at a time, of base of any type and alignment.
 template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) void lora_expand_kernel(const ExpandArgs p)
 {
     __shared__ Chunks c;
@@ -422,19 +540,11 @@ template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_
         int members;
         const int adapter = take_chunk(c, 16 * MF, q, tok, members);
         const auto column_of = [&](int tile) { return n_block * span + (tile * LR_WAVES + w) * 64; };
-        u32x4 bf[4][KS];
+        Tile<KS> b;
         Raw8<WIDE> raw[MF][2];
         const auto load_tile = [&](int n0) {
-            if (adapter >= 0) {
-#pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    const int col = min(n0 + 32 * (f >> 1) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3), p.N - 1);
-                    const uint16_t *row = reinterpret_cast<const uint16_t *>(p.b) + ((int64_t)adapter * p.N + col) * p.R;
-#pragma unroll
-                    for (int s = 0; s < KS; ++s)  // (past the rank: the last of it, for now)
-                        bf[f][s] = *reinterpret_cast<const u32x4 *>(row + min(s * 32 + lq * 8, p.R - 8));
-                }
-            }
+            if (adapter >= 0)
+                b = load_b<KS>(p, adapter, n0, l16, lq);
             // (all of base before any output: out may be base, so that no load would pass a store)
             const auto base = [&](auto all_there) {
 #pragma unroll
@@ -453,62 +563,8 @@ template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_
         };
         if (column_of(0) < p.N)  // (on its way while z is laid out)
             load_tile(column_of(0));
-        if (adapter >= 0) {
-            // 4 KS threads a token, 8 values each
-            for (int i = threadIdx.x; i < 16 * MF * 4 * KS; i += LR_THREADS) {
-                const int t = i / (4 * KS), part = i % (4 * KS), r = part * 8;
-                float z[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    z[e] = 0.0f;
-                const int64_t m = m0 + c.list[min(t, members - 1)];
-                if (r < p.R) {
-                    constexpr int AT_ONCE = MF == 4 ? 2 : LR_MAX_SPLITS;  // (many rows: few splits, and registers are waves)
-                    for (int s0 = 0; s0 < p.splits; s0 += AT_ONCE) {
-                        f32x4 v[AT_ONCE][2];
-#pragma unroll
-                        for (int s = 0; s < AT_ONCE; ++s) {
-                            const f32x4 *from = reinterpret_cast<const f32x4 *>(p.z + ((int64_t)min(s0 + s, p.splits - 1) * p.M + m) * p.R + r);
-                            v[s][0] = from[0];
-                            v[s][1] = from[1];
-                        }
-#pragma unroll
-                        for (int s = 0; s < AT_ONCE; ++s)
-                            if (s0 + s < p.splits) {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    z[e] += v[s][e >> 2][e & 3];
-                            }
-                    }
-                }
-                float f = p.scaling ? p.scaling[adapter] : 1.0f;
-                if (p.xs)
-                    f *= p.xs[m];
-                if constexpr (!BF16) {  // the row's largest to 2^10 or a little less: what is left out then keeps its bits
-                    float most = 0.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        most = fmaxf(most, fabsf(z[e]));
-                    most = KS == 8 ? group_max<32>(most) : KS == 4 ? group_max<16>(most) : KS == 2 ? group_max<8>(most) : group_max<4>(most);
-                    const bool plain = most > 0.0f && most < INFINITY;
-                    const int e2 = plain ? 10 - ilogbf(most) : 0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        z[e] = ldexpf(z[e], e2);
-                    f = ldexpf(f, -e2);
-                }
-                u32x4 hi, lo;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    hi[e] = pack2<BF16>(z[2 * e], z[2 * e + 1]);
-                    lo[e] = pack2<BF16>(z[2 * e] - unpack<BF16>(hi[e], 0), z[2 * e + 1] - unpack<BF16>(hi[e], 1));
-                }
-                zs[t >> 4][part >> 2][0][(part & 3) * 16 + (t & 15)] = hi;
-                zs[t >> 4][part >> 2][1][(part & 3) * 16 + (t & 15)] = lo;
-                if (part == 0)
-                    factor[t] = f;
-            }
-        }
+        if (adapter >= 0)
+            lay_out<BF16, KS, MF>(p, c, m0, members, adapter, zs, factor);
         __syncthreads();
         for (int tile = 0; tile < p.tiles; ++tile) {
             const int n0 = column_of(tile);
@@ -516,15 +572,7 @@ template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_
                 break;
             if (tile > 0)
                 load_tile(n0);
-            if (32 * KS > p.R) {
-#pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    if (s * 32 + lq * 8 >= p.R) {  // (whatever lies past the rank)
-#pragma unroll
-                        for (int f = 0; f < 4; ++f)
-                            bf[f][s] = u32x4{0, 0, 0, 0};
-                    }
-            }
+            clear_past_rank(b, p.R, lq);
 #pragma unroll
             for (int i = 0; i < MF; ++i) {
                 if (i * 16 >= members)
@@ -534,27 +582,8 @@ template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_
 #pragma unroll
                 for (int g = 0; g < 2; ++g)
                     to_fp32<WIDE>(raw[i][g], p.base_dtype == LORA_BF16, v[g]);
-                if (adapter >= 0) {
-                    f32x4 acc[4];
-#pragma unroll
-                    for (int f = 0; f < 4; ++f)
-                        acc[f] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int s = 0; s < KS; ++s)
-#pragma unroll
-                        for (int part = 0; part < 2; ++part) {
-                            const u32x4 z = zs[i][s][part][lane];
-#pragma unroll
-                            for (int f = 0; f < 4; ++f)
-                                acc[f] = mfma<BF16>(bf[f][s], z, acc[f]);
-                        }
-                    const float scale = factor[t];
-#pragma unroll
-                    for (int g = 0; g < 2; ++g)
-#pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            v[g][e] = __builtin_fmaf(scale, acc[2 * g + (e >> 2)][e & 3], v[g][e]);
-                }
+                if (adapter >= 0)
+                    add_product<BF16, KS>(b, zs[i], factor[t], lane, v);
                 if (t < members) {
                     const int64_t m = m0 + c.list[t];
 #pragma unroll
@@ -571,6 +600,140 @@ template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_
     }
 }
 
+// The same of many tokens, where base and out are of 16 bits, their rows begin at 16-byte boundaries and a window's lie within
+// 2 GiB: both go through LDS, so that they are read and written by whole cache lines.  A wave has a ring of units of its own,
+// 32 tokens by 64 columns of base each; what comes out lies in the unit's place before it is stored.  What is not there is asked
+// for past the buffers' ends, which costs no memory access: every unit has the same number of memory operations, so that
+// a wait can name the ones that it does not need.
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr int LE_UNIT = 4096, LE_SLOTS = 3, LE_MAX_WIDTH = 1 << 20;  // (256 rows of 2^20 16-bit numbers are 2^29 bytes)
+constexpr int LE_NT = 2;  // base and out pass once: the caches are B's and z's (16384 rows: 256 -> 239 us)
+constexpr uint32_t LE_BYTES = 0x80000000u, LE_OUT = 0x80000000u;
+__device__ __forceinline__ rsrc_t lines_of(const void *p)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, LE_BYTES, 0x00020000);
+}
+__device__ __forceinline__ void dma_line(rsrc_t r, uint32_t lane_off, uint32_t off, uint8_t *lds)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, lane_off, off, 0, LE_NT);
+}
+template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) void lora_expand_lines_kernel(const ExpandArgs p)
+{
+    static_assert(MF == 2 || MF == 4, "units of two fragments");
+    constexpr int HALVES = MF / 2;  // units of a tile of 64 columns
+    __shared__ Chunks c;
+    __shared__ u32x4 zs[MF][KS][2][64];
+    __shared__ float factor[16 * MF];
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // rings [wave][slot]
+    uint8_t *const my_ring = smem + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * LE_SLOTS * LE_UNIT;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int span = 64 * LR_WAVES * p.tiles, n_blocks = (p.N + span - 1) / span;
+    int id = blockIdx.x;
+    const int n_block = id % n_blocks;
+    id /= n_blocks;
+    const int first = id % p.slots;
+    const int64_t m0 = (int64_t)(id / p.slots) * LR_WINDOW;
+    const int n = (int)min((int64_t)LR_WINDOW, p.M - m0);
+    const int n_first = n_block * span + w * 64, n_end = min(n_block * span + span, p.N);
+    const int turned = (lane & 7) ^ (lane >> 4);  // this lane's 16-byte piece of a row, in even bands of 8 rows; odd ones: ^ 4
+    const rsrc_t base = lines_of(reinterpret_cast<const uint16_t *>(p.base) + m0 * p.base_stride);
+    const rsrc_t out = lines_of(reinterpret_cast<const uint16_t *>(p.out) + m0 * p.N);
+    Token tok;
+    const int chunks = find_chunks(c, p.ids, m0, n, p.L, 16 * MF, tok);
+    for (int q = first; q < chunks; q += p.slots) {
+        int members;
+        const int adapter = take_chunk(c, 16 * MF, q, tok, members);
+        const rsrc_t rb = lines_of(reinterpret_cast<const uint16_t *>(p.b) + (int64_t)max(adapter, 0) * p.N * p.R);
+        uint32_t from[2 * MF], to[2 * MF];  // this lane's row of each band of 8 rows
+#pragma unroll
+        for (int b = 0; b < 2 * MF; ++b) {
+            const int t = b * 8 + (lane >> 3), row = c.list[min(t, members - 1)];
+            from[b] = t < members ? (uint32_t)row * (uint32_t)p.base_stride * 2 : LE_OUT;
+            to[b] = t < members ? (uint32_t)row * (uint32_t)p.N * 2 : LE_OUT;
+        }
+        const auto at = [&](uint32_t row, int b, int n0) {  // 8 columns of it, or nowhere
+            const int piece = (turned ^ (4 * (b & 1))) * 8;
+            return n0 + piece < n_end ? row + piece * 2 : LE_OUT;
+        };
+        const auto load = [&](int half, int n0, int slot) {
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+                dma_line(base, at(from[half * 4 + b], b, n0), (uint32_t)n0 * 2, my_ring + slot * LE_UNIT + b * 1024);
+        };
+        const auto load_next = [&](int n0) {
+            Tile<KS> t;
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const int col = n0 + 32 * (f >> 1) + 8 * (l16 >> 2) + 4 * (f & 1) + (l16 & 3);
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const int r = s * 32 + lq * 8;
+                    t.v[f][s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                    rb, col < n_end && r < p.R && adapter >= 0 ? ((uint32_t)col * p.R + r) * 2 : LE_OUT, 0, 0));
+                }
+            }
+            return t;
+        };
+        constexpr int STEP = 64 * LR_WAVES;
+        // (unit u: half u mod HALVES of tile u / HALVES)
+#pragma unroll
+        for (int u = 0; u < LE_SLOTS; ++u)
+            load(u % HALVES, n_first + u / HALVES * STEP, u);
+        Tile<KS> next = load_next(n_first);
+        if (adapter >= 0)
+            lay_out<BF16, KS, MF>(p, c, m0, members, adapter, zs, factor);
+        wait_loads<0>();
+        __syncthreads();
+        int slot = 0;
+#pragma unroll 1
+        for (int n0 = n_first; n0 < n_end; n0 += STEP) {
+            const Tile<KS> b = next;
+            next = load_next(n0 + STEP);  // (a tile ahead: loads are done in order)
+#pragma unroll
+            for (int half = 0; half < HALVES; ++half) {
+                // since the loads of this unit: the stores of the unit before them, loads and stores of two units, and
+                // of B those at the beginnings of tiles
+                constexpr int B_LOADS = 4 * KS;
+                const int later = 20 + B_LOADS * (HALVES == 1 ? 3 : half ? 1 : 2);
+                if (later == 20 + 3 * B_LOADS)
+                    wait_loads<(20 + 3 * B_LOADS < 63 ? 20 + 3 * B_LOADS : 63)>();
+                else if (later == 20 + 2 * B_LOADS)
+                    wait_loads<(20 + 2 * B_LOADS < 63 ? 20 + 2 * B_LOADS : 63)>();
+                else
+                    wait_loads<(20 + B_LOADS < 63 ? 20 + B_LOADS : 63)>();
+                uint8_t *ring = my_ring + slot * LE_UNIT;
+                if (half * 32 < members) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float v[2][8];
+#pragma unroll
+                        for (int g = 0; g < 2; ++g) {
+                            Raw8<false> raw;
+                            raw.v[0] = *reinterpret_cast<const u32x4 *>(ring + i * 2048 + l16 * 128 + (((4 * g + lq) ^ (l16 >> 1)) << 4));
+                            to_fp32<false>(raw, p.base_dtype == LORA_BF16, v[g]);
+                        }
+                        if (adapter >= 0)
+                            add_product<BF16, KS>(b, zs[half * 2 + i], factor[half * 32 + i * 16 + l16], lane, v);
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+                            *reinterpret_cast<u32x4 *>(ring + i * 2048 + l16 * 128 + (((4 * g + lq) ^ (l16 >> 1)) << 4)) = pack8(p.out_bf16, v[g]);
+                    }
+                }
+                u32x4 o[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    o[k] = *reinterpret_cast<const u32x4 *>(ring + k * 1024 + lane * 16);
+                wait_loads<63>();  // (the unit's place has been read)
+                load((half + LE_SLOTS) % HALVES, n0 + (half + LE_SLOTS) / HALVES * STEP, slot);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    __builtin_amdgcn_raw_buffer_store_b128(o[k], out, at(to[half * 4 + k], k, n0), (uint32_t)n0 * 2, LE_NT);
+                slot = slot == LE_SLOTS - 1 ? 0 : slot + 1;
+            }
+        }
+    }
+}
+
 // ---------------------------------------------------------------- which kernels
 // Tokens of a chunk: 16 in a decode batch, whose adapters have few each; 32 and 64 for prompts, where a chunk's share of A and B is read again for each.
 int chunk_frags(int64_t M) { return M <= LR_WINDOW ? 1 : M < 8192 ? 2 : 4; }
@@ -580,7 +743,7 @@ int chunk_slots(const LoraArgs &a, int mf)
 {
     if (a.M <= LR_WINDOW)
         return (int)(a.M < a.L + 1 + a.M / (16 * mf) ? a.M : a.L + 1 + a.M / (16 * mf));
-    return LR_WINDOW / (16 * mf) + (a.M < 8192 ? 2 : 0);
+    return LR_WINDOW / (16 * mf) + 2;
 }
 struct Plan {
     int mf, nf, groups, slots, splits;
@@ -607,22 +770,26 @@ Plan lora_plan(const LoraArgs &a)
 }
 
 constexpr int LR_MAX_DEVICES = 64;
-template <bool BF16, bool INT8, int MF, int NF> hipError_t shrink(const ShrinkArgs &a, int64_t blocks, hipStream_t s)
+// a launch with LDS bytes of dynamic LDS, for which the kernel's limit is raised once per device
+template <auto KERNEL, int LDS, typename Args> hipError_t launch_with_lds(const Args &a, uint32_t blocks, hipStream_t s)
 {
-    constexpr int SLOT = (2 * NF * (INT8 ? 2 : 1) + 2 * MF) * 1024, SLOTS = SLOT <= 4096 ? 4 : SLOT <= 10240 ? 2 : 1, LDS = LR_WAVES * SLOTS * SLOT;
-    static std::atomic<bool> done[LR_MAX_DEVICES];  // the kernel's dynamic LDS limit is raised once per device
+    static std::atomic<bool> done[LR_MAX_DEVICES];
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
     if (e == hipSuccess && !(dev < LR_MAX_DEVICES && done[dev].load(std::memory_order_acquire))) {
-        e = hipFuncSetAttribute(reinterpret_cast<const void *>(&lora_shrink_kernel<BF16, INT8, MF, NF, SLOTS>),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        e = hipFuncSetAttribute(reinterpret_cast<const void *>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e == hipSuccess && dev < LR_MAX_DEVICES)
             done[dev].store(true, std::memory_order_release);
     }
     if (e != hipSuccess)
         return e;
-    hipLaunchKernelGGL((lora_shrink_kernel<BF16, INT8, MF, NF, SLOTS>), dim3((uint32_t)blocks), dim3(LR_THREADS), LDS, s, a);
+    hipLaunchKernelGGL(KERNEL, dim3(blocks), dim3(LR_THREADS), LDS, s, a);
     return hipGetLastError();
+}
+template <bool BF16, bool INT8, int MF, int NF> hipError_t shrink(const ShrinkArgs &a, int64_t blocks, hipStream_t s)
+{
+    constexpr int SLOT = (2 * NF * (INT8 ? 2 : 1) + 2 * MF) * 1024, SLOTS = SLOT <= 4096 ? 4 : SLOT <= 10240 ? 2 : 1, LDS = LR_WAVES * SLOTS * SLOT;
+    return launch_with_lds<&lora_shrink_kernel<BF16, INT8, MF, NF, SLOTS>, LDS>(a, (uint32_t)blocks, s);
 }
 template <bool BF16, bool INT8, int MF> hipError_t shrink_nf(int nf, const ShrinkArgs &a, int64_t blocks, hipStream_t s)
 {
@@ -638,6 +805,17 @@ template <bool BF16, bool INT8> hipError_t shrink_mf(int mf, int nf, const Shrin
 {
     return mf == 1 ? shrink_nf<BF16, INT8, 1>(nf, a, blocks, s) : mf == 2 ? shrink_nf<BF16, INT8, 2>(nf, a, blocks, s)
                                                                           : shrink_nf<BF16, INT8, 4>(nf, a, blocks, s);
+}
+template <bool BF16, int MF> hipError_t expand_lines(const ExpandArgs &a, uint32_t blocks, hipStream_t s)
+{
+    constexpr int LDS = LR_WAVES * LE_SLOTS * LE_UNIT;
+    if (a.R <= 32)
+        return launch_with_lds<&lora_expand_lines_kernel<BF16, 1, MF>, LDS>(a, blocks, s);
+    if (a.R <= 64)
+        return launch_with_lds<&lora_expand_lines_kernel<BF16, 2, MF>, LDS>(a, blocks, s);
+    if (a.R <= 128)
+        return launch_with_lds<&lora_expand_lines_kernel<BF16, 4, 2>, LDS>(a, blocks, s);
+    return launch_with_lds<&lora_expand_lines_kernel<BF16, 8, 2>, LDS>(a, blocks, s);
 }
 template <bool BF16, bool WIDE, int MF> hipError_t expand_ks(const ExpandArgs &a, uint32_t blocks, hipStream_t s)
 {
@@ -679,7 +857,11 @@ hipError_t launch_lora_add(const LoraArgs &a, void *ws, hipStream_t s)
                         : (int8 ? shrink_mf<false, true>(p.mf, p.nf, sa, blocks, s) : shrink_mf<false, false>(p.mf, p.nf, sa, blocks, s));
     if (e != hipSuccess)
         return e;
-    const int mf = a.R > 128 && p.mf > 2 ? 2 : p.mf, slots = chunk_slots(a, mf);
+    // base and out by whole lines, where they are of 16 bits and their rows aligned
+    const bool lines = p.mf > 1 && a.base_dtype != LORA_FP32 && a.N % 8 == 0 && a.base_stride % 8 == 0 && a.N <= LE_MAX_WIDTH &&
+                       a.base_stride <= LE_MAX_WIDTH &&
+                       (reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
+    const int mf = a.R > (lines ? 64 : 128) && p.mf > 2 ? 2 : p.mf, slots = chunk_slots(a, mf);
     ExpandArgs ea{a.base, a.b, reinterpret_cast<const float *>(ws), a.xs, a.scaling, a.ids, a.out, a.M, a.base_stride, a.N, a.R, a.L,
                   (int16_t)p.splits, (int16_t)slots, 1, a.base_dtype, (int8_t)(a.out_dtype == LORA_BF16)};
     // a block's columns: the more, the seldomer z is laid out
@@ -688,6 +870,10 @@ hipError_t launch_lora_add(const LoraArgs &a, void *ws, hipStream_t s)
     const int64_t n_blocks = (a.N + 256 * ea.tiles - 1) / (256 * ea.tiles), eb = p.windows * slots * n_blocks;
     if (eb * LR_THREADS > 0xffffffffll)
         return hipErrorInvalidValue;
+    if (lines && ea.tiles > 1 && mf == 4)
+        return bf16 ? expand_lines<true, 4>(ea, (uint32_t)eb, s) : expand_lines<false, 4>(ea, (uint32_t)eb, s);
+    if (lines && ea.tiles > 1)
+        return bf16 ? expand_lines<true, 2>(ea, (uint32_t)eb, s) : expand_lines<false, 2>(ea, (uint32_t)eb, s);
     if (a.base_dtype == LORA_FP32)
         return bf16 ? expand<true, true>(mf, ea, (uint32_t)eb, s) : expand<false, true>(mf, ea, (uint32_t)eb, s);
     return bf16 ? expand<true, false>(mf, ea, (uint32_t)eb, s) : expand<false, false>(mf, ea, (uint32_t)eb, s);
