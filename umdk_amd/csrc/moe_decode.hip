@@ -236,6 +236,14 @@ struct Item {
     const float *s;             // the matrix's scales
 };
 
+// How the tiles of the second product make up items: first the shared expert's parts (chunks of it), `run` tiles an item, then
+// the other entries' parts, the last of them by fewer tiles.
+struct Split {
+    int run_s, runs_s, items_s;   // the shared expert's tiles an item, items a part, items
+    int run, runs, big, items_b;  // the first `big` other parts' tiles an item, items a part, items
+    int run_e, runs_e;            // the rest's tiles an item, items a part
+};
+
 // What the streams need of the arguments, in LDS: in scalar registers it would crowd out what they work with.
 struct Late {
     const void *w1, *w2, *sw1, *sw2;
@@ -260,6 +268,7 @@ struct Shared {
     uint8_t entry_pick[MD_MAX_ENTRIES][MD_MAX_TOKENS];
     int wave_count[MD_WAVES], known;
     Item item[2];
+    Split split;
     Late a;
 };
 static_assert(sizeof(Shared) <= 160 * 1024, "a CU's LDS");
@@ -310,12 +319,14 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
     const bool nshared = args.p.Is > 0;
 
     // The last wave is the block's clerk: it takes the tickets and says what their items are.  (The first two are on their way
-    // while the tokens are routed, by other waves where there are few.)
+    // while the tokens are routed, by other waves where there are few; otherwise the second is not asked for before the clerk's
+    // tokens' logits, which would come after it: 2 us of 44.)
     const bool clerk = w == MD_WAVES - 1;
     int ticket = 0, ticket2 = 0;
     if (clerk && lane == 0) {
         ticket = ctr_add(args.ws.ctr, 1);
-        ticket2 = ctr_add(args.ws.ctr, 1);
+        if (T < MD_WAVES)
+            ticket2 = ctr_add(args.ws.ctr, 1);
     }
     int entries;
     uint32_t on;  // the tokens that are active
@@ -345,6 +356,8 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 }
             }
         }
+        if (clerk && lane == 0 && T >= MD_WAVES)
+            ticket2 = ctr_add(args.ws.ctr, 1);
         if (threadIdx.x == MD_WAVES * 64 - 1)
             sh.a = Late{p.w1,  p.w2, p.sw1, p.sw2, p.s1, p.s2,       p.ss1,       p.ss2,          p.out,          args.ws.h, args.ws.h_low,
                         args.ws.part, args.ws.ctr, p.I, p.Is, p.K, args.width, args.chunks, args.ws.h_bytes, args.ws.part_bytes};
@@ -397,6 +410,50 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
     // ---- the items
     const uint32_t row1 = (uint32_t)(H * W::SIZE);  // bytes of a row of the first matrix
     const auto chunks_of = [](int I) { return (I + MD_CHUNK - 1) / MD_CHUNK; };
+    const auto log_waves = [](int units) {  // that share a tile of so many units: the fewer, the more tiles are done at once
+        return units > 4 * U2 ? 3 : units > 2 * U2 ? 2 : units > U2 ? 1 : 0;
+    };
+    const auto first_items = [&] {  // how many items the first product has
+        return (nshared ? uniform(a.Is) / 16 : 0) + (entries - nshared) * (uniform(a.I) / 16);
+    };
+    if (w == MD_WAVES - 2 || (clerk && uniform(ticket) >= first_items())) {  // (the clerk where it needs it at once: the same numbers)
+        // An item costs about what 100 KB more of weights would (4 us: h, a meeting of the waves, the parts' way to memory).  Of
+        // 1 to 32 tiles an item and 1 to 8 of the shared expert's the cheapest, a lane each: what the blocks' share of all items
+        // costs, and half of the largest for their not ending together.  (A wave's four tiles between two meetings at most, but 8 in
+        // any case; fp8: a block of 128 rows.)
+        constexpr int ITEM_COST = 100;  // KB
+        const int I0 = uniform(a.I), Is = uniform(a.Is), tiles = H / 16;
+        const int C0 = chunks_of(I0), Cs = nshared ? chunks_of(Is) : 0, parts = (entries - nshared) * C0;
+        const auto most = [&](int I, int C) {
+            const int units = (I * W::SIZE + 127) / 128;
+            return WT == MD_FP8 ? 8 : max(8, 32 >> log_waves((units + C - 1) / C));
+        };
+        const int kb = parts ? 16 * I0 * W::SIZE / C0 >> 10 : 0, kb_s = Cs ? 16 * Is * W::SIZE / Cs >> 10 : 0;  // a tile's
+        const int log = min(lane & 7, 5), log_s = Cs ? lane >> 3 & 3 : 0, run = 1 << log, run_s = 1 << log_s;
+        const int runs_s = (tiles + run_s - 1) >> log_s, runs = (tiles + run - 1) >> log;
+        const int items_s = Cs * runs_s, items_0 = parts * runs, items = items_s + items_0;
+        const int one_s = ITEM_COST + run_s * kb_s, one = ITEM_COST + run * kb;
+        int cost = items <= MD_BLOCKS ? max(one, one_s) : (items_s * one_s + items_0 * one) / MD_BLOCKS + max(one, one_s) / 2;
+        if (run > (parts ? most(I0, C0) : 1))
+            cost = 0x3ffffff;
+        int least = cost << 5 | (lane & 31);
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2)
+            least = min(least, __shfl_xor(least, d, 64));
+        if (lane == (least & 31)) {
+            Split v;
+            v.run_s = run_s;
+            v.runs_s = runs_s;
+            v.items_s = items_s;
+            v.run = run;
+            v.runs = runs;
+            v.big = items > MD_BLOCKS && run > 1 ? parts - parts / 4 : parts;  // (so that the blocks end together)
+            v.items_b = v.big * v.runs;
+            v.run_e = max(run / 2, 1);
+            v.runs_e = (tiles + v.run_e - 1) >> max(log - 1, 0);
+            sh.split = v;
+        }
+    }
     // the item of the clerk's ticket, for all to read
     const auto describe = [&](int slot) {
         const int q = uniform(ticket), I0 = uniform(a.I), Is = uniform(a.Is);
@@ -421,21 +478,24 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 it.s = (shared ? a.ss1 : a.s1) + (size_t)e * 2 * I;
         } else {
             const int C0 = chunks_of(I0), Cs = nshared ? chunks_of(Is) : 0, parts = Cs + (entries - nshared) * C0;
-            // tiles of an item: about two items for every block, and small ones for the last quarter of the parts, which the
-            // blocks share out to end together
-            int run = H / 16 * parts / (MD_BLOCKS + MD_BLOCKS / 2);
-            run = run >= 8 ? 8 : run >= 4 ? 4 : run >= 2 ? 2 : 1;
-            const int big = parts - parts / 4, runs0 = (H / 16 + run - 1) / run;
-            int at = q - N1, c = at / runs0;
-            if (c < big) {
-                at %= runs0;
+            const Split &v = sh.split;
+            const int items_s = uniform(v.items_s), items_b = uniform(v.items_b);
+            int at = q - N1, c = 0, run, runs;
+            if (at < items_s) {
+                run = uniform(v.run_s);
+                runs = uniform(v.runs_s);
+            } else if (at -= items_s; at < items_b) {
+                run = uniform(v.run);
+                runs = uniform(v.runs);
+                c = Cs;
             } else {
-                at -= big * runs0;
-                run = max(run / 2, 1);
-                const int runs = (H / 16 + run - 1) / run;
-                c = big + at / runs;
-                at %= runs;
+                at -= items_b;
+                run = uniform(v.run_e);
+                runs = uniform(v.runs_e);
+                c = Cs + uniform(v.big);
             }
+            c += at / runs;
+            at %= runs;
             if (c < parts) {
                 const bool shared = c < Cs;
                 const int I = shared ? Is : I0, C = shared ? Cs : C0, d = shared ? 0 : nshared + (c - Cs) / C0;
@@ -446,7 +506,7 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 it.chunk = shared ? c : (c - Cs) % C0;
                 it.tile = at * run;
                 it.count = min(run, H / 16 - it.tile);
-                it.lkw = cu > 4 * U2 ? 3 : cu > 2 * U2 ? 2 : cu > U2 ? 1 : 0;  // (the fewer, the more tiles are done at once)
+                it.lkw = log_waves(cu);
                 it.k0 = it.chunk * cu;
                 it.units = min(cu, units - it.k0);
                 it.row_bytes = (uint32_t)(I * W::SIZE);
@@ -800,13 +860,15 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 describe(turn);
             lds_barrier();
             // tile v of the batch is the (v / per_tile)-th of the 2^lkw waves from (v mod per_tile) 2^lkw on; another wave each
-            // time adds them up
-            for (int v = (w + cur.tile) & 7; v < min(MD_BATCH * per_tile, cur.count - t0); v += MD_WAVES) {
+            // time adds them up, and up to four at once
+            const int v0 = (w + cur.tile) & 7, here = min(MD_BATCH * per_tile, cur.count - t0);
+#pragma unroll 1
+            for (int v = v0; v < here; v += MD_WAVES) {
                 const int from = (v & (per_tile - 1)) << cur.lkw, j = v >> (3 - cur.lkw);
                 f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
                 for (int k = 0; k < min(1 << cur.lkw, cur.units); ++k)
                     y += sh.red[from + k][j][lane];
-                const int tile = cur.tile + t0 + v, n = tile * 16 + lq * 4;
+                const int n = (cur.tile + t0 + v) * 16 + lq * 4;
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     if constexpr (WT == MD_INT8)
@@ -816,13 +878,17 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 }
                 const uint32_t at = (uint32_t)(((l16 * slots + pick) * chunks + cur.chunk) * H + n) * 4u;
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, y), rp, mine ? at : MD_OUT, 0, AUX_AGENT);
+            }
+            if (v0 < here) {
                 wait_loads<0>();
-                int before = 0;
-                if (lane == 0)
-                    before = ctr_add(a.ctr + (MD_CTR_DONE + tile) * MD_CTR, 1);
-                before = uniform(before);
+                const int v = v0 + MD_WAVES * lane;
+                int before = -1;
+                if (v < here)
+                    before = ctr_add(a.ctr + (MD_CTR_DONE + cur.tile + t0 + v) * MD_CTR, 1);
+                uint64_t last = __ballot(before + 1 == Cs + (entries - nshared) * C0);  // every part of this tile of the output is there
                 asm volatile("" ::: "memory");
-                if (before + 1 == Cs + (entries - nshared) * C0) {  // every part of this tile of the output is there
+                for (; last; last &= last - 1) {
+                    const int n = (cur.tile + t0 + v0 + MD_WAVES * __builtin_ctzll(last)) * 16 + lq * 4;
                     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
                     const int t = min(l16, T - 1), routed = (slots - 1) * C0, n_parts = routed + Cs;
                     constexpr int AT_ONCE = 8;
