@@ -781,22 +781,21 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
             for (int u = 0; u < U2; ++u)
                 s[u] = scale(cur.s, (cur.tile >> 3) * (int)(cur.row_bytes / 128) + min(cur.k0 + wk + (u << cur.lkw), (int)(cur.row_bytes / 128) - 1));
         }
-        // h of the entry, once all of it has been written.  One wave looks, at 64 entries at once.
+        // h of the entry, once all of it has been written.  One wave looks, at this entry and the 63 after it, and then, while it
+        // waits, at this one alone: all blocks' looks at many counters slow down the streams that they wait for.
         if (cur.entry >= known) {
             if (w == 0) {
                 const uint64_t t0 = wall_clock64();
-                const int d = min(known + lane, entries - 1), want = (nshared && d == 0 ? a.Is : a.I) / 16;
-                int to;
-                for (;;) {
-                    const uint64_t not_yet = __ballot(ctr_load(a.ctr + (MD_CTR_READY + d) * MD_CTR) < want);
-                    to = known + (not_yet ? __builtin_ctzll(not_yet) : 64);
-                    if (to > cur.entry)
-                        break;
-                    if (wall_clock64() - t0 > 200000000ull) {  // 2 s: no launch that has the workspace to itself waits so long
+                const int d = min(cur.entry + lane, entries - 1), want = (nshared && d == 0 ? a.Is : a.I) / 16;
+                int *const counter = a.ctr + (MD_CTR_READY + d) * MD_CTR;
+                const uint64_t not_yet = __ballot(ctr_load(counter) < want);
+                int to = cur.entry + (not_yet ? __builtin_ctzll(not_yet) : 64);
+                while (to == cur.entry) {
+                    __builtin_amdgcn_s_sleep(8);
+                    if (wall_clock64() - t0 > 200000000ull)  // 2 s: no launch that has the workspace to itself waits so long
                         to = -1;
-                        break;
-                    }
-                    __builtin_amdgcn_s_sleep(4);
+                    else if (__ballot(lane == 0 && ctr_load(counter) >= want))
+                        to = cur.entry + 1;
                 }
                 if (lane == 0)
                     sh.known = to;
