@@ -737,13 +737,16 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
 // ---------------------------------------------------------------- which kernels
 // Tokens of a chunk: 16 in a decode batch, whose adapters have few each; 32 and 64 for prompts, where a chunk's share of A and B is read again for each.
 int chunk_frags(int64_t M) { return M <= LR_WINDOW ? 1 : M < 8192 ? 2 : 4; }
-// Blocks that share a window's chunks: of a decode batch as many as there can be, of prompts as many as there are of one adapter,
-// or a few more.
+// Blocks that share a window's chunks: of a decode batch as many as there can be; of prompts as many as there are of one adapter
+// and two more, or, while they do not fill the chip twice, as many as there can be (441 rows, 41 adapters 41 -> 22 us; 2048 rows
+// of 4096 columns and 16 adapters with 8 more 33 -> 39).
 int chunk_slots(const LoraArgs &a, int mf)
 {
+    const int64_t alone = (a.M <= LR_WINDOW ? a.M : LR_WINDOW) / (16 * mf), most = alone + 1 + a.L;
     if (a.M <= LR_WINDOW)
-        return (int)(a.M < a.L + 1 + a.M / (16 * mf) ? a.M : a.L + 1 + a.M / (16 * mf));
-    return LR_WINDOW / (16 * mf) + 2;
+        return (int)(a.M < most ? a.M : most);
+    const int64_t fill = 2 * 256 / ((a.M + LR_WINDOW - 1) / LR_WINDOW * ((a.N + 255) / 256));
+    return (int)(fill < alone + 2 ? alone + 2 : fill < most ? fill : most);
 }
 struct Plan {
     int mf, nf, groups, slots, splits;
