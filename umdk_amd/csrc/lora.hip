@@ -8,6 +8,10 @@
 // its own or kept, and no sum hangs on what other tokens are there: a token's bits are the same in any order of a batch of its size.
 //
 // What bounds it: for few tokens the adapters' stream and the latency of two launches, for many the streams of x, base and out.
+// Measured (K x N): one row of 4096 x 4096 at rank 16 3.6 + 4.3 us; 64 int8 rows of 7168 x 4096 with 32 adapters 6.7 + 6.9; 1021
+// rows of 4096 x 4096 6.3 + 9.2; 16384 rows of 4096 x 14336 at rank 64 33.5 (4.1 TB/s) + 196 (4.8 TB/s; B and z, 100 MB of
+// them past L2, included 5.4).  Both in one launch, each block with a z of its own, took longer where it should have helped
+// (one row 8.3 -> 10.8 us, 64 rows 13 -> 20).
 // Matrix instructions take 16 tokens as their columns, rows of A or B as their rows.  z goes into the second product as two
 // 16-bit numbers, the second what the first leaves out, so that it loses 2^-16 (bf16) or, brought to the row's largest first, 2^-21 (fp16).
 #include <atomic>
@@ -735,10 +739,11 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
 }
 
 // ---------------------------------------------------------------- which kernels
-// Tokens of a chunk: 16 in a decode batch, whose adapters have few each; 32 and 64 for prompts, where a chunk's share of A and B is read again for each.
+// Tokens of a chunk: 16 in a decode batch, whose adapters have few each; 32 and 64 for prompts, where a chunk's share of A and B
+// is read again for each.
 int chunk_frags(int64_t M) { return M <= LR_WINDOW ? 1 : M < 8192 ? 2 : 4; }
 // Blocks that share a window's chunks: of a decode batch as many as there can be; of prompts as many as there are of one adapter
-// and two more, or, while they do not fill the chip twice, as many as there can be (441 rows, 41 adapters 41 -> 22 us; 2048 rows
+// and two more, or, while they do not fill the chip twice, as many as there can be (441 rows, 41 adapters 41 -> 16 us; 2048 rows
 // of 4096 columns and 16 adapters with 8 more 33 -> 39).
 int chunk_slots(const LoraArgs &a, int mf)
 {
@@ -860,7 +865,8 @@ hipError_t launch_lora_add(const LoraArgs &a, void *ws, hipStream_t s)
                         : (int8 ? shrink_mf<false, true>(p.mf, p.nf, sa, blocks, s) : shrink_mf<false, false>(p.mf, p.nf, sa, blocks, s));
     if (e != hipSuccess)
         return e;
-    // base and out by whole lines, where they are of 16 bits and their rows aligned
+    // base and out by whole lines, where they are of 16 bits and their rows aligned, and a wave has two tiles at least (16384 rows
+    // of 14336 columns 299 -> 256 us; 1021 rows of 4096, with one tile a wave, 15.7 -> 18.2)
     const bool lines = p.mf > 1 && a.base_dtype != LORA_FP32 && a.N % 8 == 0 && a.base_stride % 8 == 0 && a.N <= LE_MAX_WIDTH &&
                        a.base_stride <= LE_MAX_WIDTH &&
                        (reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
