@@ -302,3 +302,29 @@ def test_gradients_are_refused_not_dropped():
         with torch.no_grad():
             call(d, 2)
         d[name] = t
+
+
+@pytest.mark.parametrize("dtype,T,H,E,I,Is,K", [
+    ("int8", 16, 768, 32, 192, 0, 5), ("int8", 2, 5824, 16, 320, 0, 4), ("int8", 3, 3904, 16, 256, 1344, 8),
+    ("bf16", 5, 8192, 32, 64, 0, 6), ("bf16", 16, 8128, 16, 64, 64, 4), ("bf16", 1, 8192, 2, 64, 4160, 1),
+    ("int8", 9, 8192, 24, 64, 8256, 3), ("bf16", 8, 4160, 12, 448, 64, 2), ("fp8", 12, 8064, 20, 128, 1920, 3),
+    ("bf16", 4, 1088, 8, 8256, 0, 2), ("fp8", 7, 1152, 6, 8320, 128, 2),
+])
+def test_narrow_and_wide_experts_share_out_tiles(dtype, T, H, E, I, Is, K):
+    """Items of 1 to 32 tiles, shared experts by other numbers, parts whose tiles do not come out even."""
+    d = make(T, H, E, I, Is, dtype, seed=T + I)
+    check(d, K, call(d, K))
+
+
+@pytest.mark.parametrize("dtype,Is", [("bf16", 64), ("int8", 4160), ("fp8", 4224)])
+@pytest.mark.parametrize("T", [1, 9])
+def test_the_shared_expert_alone(dtype, Is, T):
+    """No token has an expert: every score is NaN."""
+    d = make(T, 1024, 4, 128, Is, dtype, seed=T)
+    d["router"].fill_(float("nan"))
+    out, ids, gates = call(d, 2)
+    assert (ids == -1).all() and not gates.any()
+    x = d["x"].cpu().double()
+    for t in range(T):
+        want, bound = expert(x[t], d["SW1"], d["SW2"])
+        assert ((out[t].cpu().double() - want).abs() <= want.abs() * 2.0 ** -8 + bound * (1 + 2.0 ** -8) + 20 * E32 * want.abs()).all()

@@ -695,16 +695,16 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
             next = load_next(n0 + STEP);  // (a tile ahead: loads are done in order)
 #pragma unroll
             for (int half = 0; half < HALVES; ++half) {
-                // since the loads of this unit: the stores of the unit before them, loads and stores of two units, and
-                // of B those at the beginnings of tiles
+                // since the loads of this unit: the stores of the unit before them, loads and stores of two units, and of B those
+                // at the beginnings of tiles (the counter ends at 63, where a wait would wait for nothing)
                 constexpr int B_LOADS = 4 * KS;
-                const int later = 20 + B_LOADS * (HALVES == 1 ? 3 : half ? 1 : 2);
-                if (later == 20 + 3 * B_LOADS)
-                    wait_loads<(20 + 3 * B_LOADS < 63 ? 20 + 3 * B_LOADS : 63)>();
-                else if (later == 20 + 2 * B_LOADS)
-                    wait_loads<(20 + 2 * B_LOADS < 63 ? 20 + 2 * B_LOADS : 63)>();
+                constexpr auto most = [](int tiles) { return 20 + tiles * B_LOADS < 63 ? 20 + tiles * B_LOADS : 62; };
+                if (HALVES == 1)
+                    wait_loads<most(3)>();
+                else if (half == 0)
+                    wait_loads<most(2)>();
                 else
-                    wait_loads<(20 + B_LOADS < 63 ? 20 + B_LOADS : 63)>();
+                    wait_loads<most(1)>();
                 uint8_t *ring = my_ring + slot * LE_UNIT;
                 if (half * 32 < members) {
 #pragma unroll
@@ -821,9 +821,7 @@ template <bool BF16, int MF> hipError_t expand_lines(const ExpandArgs &a, uint32
         return launch_with_lds<&lora_expand_lines_kernel<BF16, 1, MF>, LDS>(a, blocks, s);
     if (a.R <= 64)
         return launch_with_lds<&lora_expand_lines_kernel<BF16, 2, MF>, LDS>(a, blocks, s);
-    if (a.R <= 128)
-        return launch_with_lds<&lora_expand_lines_kernel<BF16, 4, 2>, LDS>(a, blocks, s);
-    return launch_with_lds<&lora_expand_lines_kernel<BF16, 8, 2>, LDS>(a, blocks, s);
+    return launch_with_lds<&lora_expand_lines_kernel<BF16, 4, 2>, LDS>(a, blocks, s);
 }
 template <bool BF16, bool WIDE, int MF> hipError_t expand_ks(const ExpandArgs &a, uint32_t blocks, hipStream_t s)
 {
@@ -866,8 +864,9 @@ hipError_t launch_lora_add(const LoraArgs &a, void *ws, hipStream_t s)
     if (e != hipSuccess)
         return e;
     // base and out by whole lines, where they are of 16 bits and their rows aligned, and a wave has two tiles at least (16384 rows
-    // of 14336 columns 299 -> 256 us; 1021 rows of 4096, with one tile a wave, 15.7 -> 18.2)
-    const bool lines = p.mf > 1 && a.base_dtype != LORA_FP32 && a.N % 8 == 0 && a.base_stride % 8 == 0 && a.N <= LE_MAX_WIDTH &&
+    // of 14336 columns 299 -> 256 us; 1021 rows of 4096, with one tile a wave, 15.7 -> 18.2; ranks past 128 leave too few registers
+    // for a tile of B ahead: 305 -> 309)
+    const bool lines = p.mf > 1 && a.R <= 128 && a.base_dtype != LORA_FP32 && a.N % 8 == 0 && a.base_stride % 8 == 0 && a.N <= LE_MAX_WIDTH &&
                        a.base_stride <= LE_MAX_WIDTH &&
                        (reinterpret_cast<uintptr_t>(a.base) | reinterpret_cast<uintptr_t>(a.out)) % 16 == 0;
     const int mf = a.R > (lines ? 64 : 128) && p.mf > 2 ? 2 : p.mf, slots = chunk_slots(a, mf);
