@@ -26,9 +26,9 @@
 // them up, picks ascending.  h is held as two bf16 numbers, of which the second is what the first leaves out (2^-16 in
 // all): one would add 2^-8 roundings of I values to the result's own, and the matrix instructions for the second are free.
 //
-// Measured: one token on 8 of 64 fp8 experts and a shared one of 7168 x 2048 (398 MB of weights) 91-96 us, of which 4.5 are the
+// Measured: one token on 8 of 64 fp8 experts and a shared one of 7168 x 2048 (398 MB of weights) 92 us, of which 4.5 are the
 // logits, 6 the routing, 4 until the first weights are there and some 10 the blocks' not ending together; 16 such tokens (44 to
-// 56 experts, 2.0 to 2.5 GB) 384-398 us, 7.0 TB/s in the first product and 5.4 in the second, whose items' h comes behind
+// 56 experts, 2.0 to 2.5 GB) 357-390 us, 7.0 TB/s in the first product and 5.4 in the second, whose items' h comes behind
 // their own first weights; 7 tokens on 6 of 160 bf16 experts of 5120 x 1408 (1.67 GB) 277 us; one token on 2 of 8 bf16 experts of
 // 1024 x 512 27 us, all of it latency: two launches, the routing, an expert's h on its way from block to block.
 #include <atomic>
