@@ -426,13 +426,13 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
         // An item costs about what 100 KB more of weights would (4 us: h, a meeting of the waves, the parts' way to memory).  Of
         // 1 to 32 tiles an item and 1 to 8 of the shared expert's the cheapest, a lane each: what the blocks' share of all items
         // costs, and half of the largest for their not ending together.  (A wave's four tiles between two meetings at most, but 8 in
-        // any case; fp8: a block of 128 rows.)
+        // any case.)
         constexpr int ITEM_COST = 100;  // KB
         const int I0 = uniform(a.I), Is = uniform(a.Is), tiles = H / 16;
         const int C0 = chunks_of(I0), Cs = nshared ? chunks_of(Is) : 0, parts = (entries - nshared) * C0;
         const auto most = [&](int I, int C) {
             const int units = (I * W::SIZE + 127) / 128;
-            return WT == MD_FP8 ? 8 : max(8, 32 >> log_waves((units + C - 1) / C));
+            return max(8, 32 >> log_waves((units + C - 1) / C));
         };
         const int kb = parts ? 16 * I0 * W::SIZE / C0 >> 10 : 0, kb_s = Cs ? 16 * Is * W::SIZE / Cs >> 10 : 0;  // a tile's
         const int log = min(lane & 7, 5), log_s = Cs ? lane >> 3 & 3 : 0, run = 1 << log, run_s = 1 << log_s;
@@ -782,11 +782,14 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
         const int pick = sh.entry_pick[cur.entry][l16];
         const bool mine = mask >> l16 & 1;  // this lane's token has the expert
         float s[U2];
-        if constexpr (WT == MD_FP8) {  // (an item's tiles are of one block of rows)
+        const auto scales_of = [&](int tile) {
+            if constexpr (WT == MD_FP8) {
 #pragma unroll
-            for (int u = 0; u < U2; ++u)
-                s[u] = scale(cur.s, (cur.tile >> 3) * (int)(cur.row_bytes / 128) + min(cur.k0 + wk + (u << cur.lkw), (int)(cur.row_bytes / 128) - 1));
-        }
+                for (int u = 0; u < U2; ++u)
+                    s[u] = scale(cur.s, (tile >> 3) * (int)(cur.row_bytes / 128) + min(cur.k0 + wk + (u << cur.lkw), (int)(cur.row_bytes / 128) - 1));
+            }
+        };
+        scales_of(cur.tile);
         // h of the entry, once all of it has been written.  One wave looks, at this entry and the 63 after it, and then, while it
         // waits, at this one alone: all blocks' looks at many counters slow down the streams that they wait for.
         if (cur.entry >= known) {
@@ -850,6 +853,8 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                     acc[i - 1] = acc[i];
                 acc[MD_BATCH - 1] = f32x4{0.f, 0.f, 0.f, 0.f};
                 if (j0 + j < tiles) {
+                    if (WT == MD_FP8 && cur.count > 8)  // (otherwise all of one block of rows)
+                        scales_of(cur.tile + (w >> cur.lkw) + (j0 + j) * per_tile);
                     upto<U2>(units, [&](auto c) {
                         constexpr int u = decltype(c)::value;
                         use(h + u * W::STEPS, low + u * W::STEPS, WT == MD_FP8 ? s[u] : 0.f,
