@@ -425,8 +425,8 @@ CAMHIP_API camhipStatus camhipQuantMatmul(void *workspace, uint64_t workspaceSiz
  *   E_e(x) = W2_e (silu(g) * u),  (g, u) = the halves of W1_e x
  *   out[t] = sum_k topkWeights[t, k] E_topkIdx[t, k](x_t) + E_shared(x_t), k ascending, rounded once to bf16
  * in fp32, of the weights' exact values (code * scale): int8 and fp8 quantise the weights alone, the rows stay in 16 bits
- * (camhipFusedDeepMoe quantises them too, and its results differ by that), and what is between the two products is held
- * to 2^-16 of itself.  Weights with the reduction dimension contiguous, as camhipMoeExperts takes them: gmm1Weight [numExperts,
+ * (camhipFusedDeepMoe quantises them too, and its results differ by that), and what is between the two products keeps
+ * its 32 bits.  Weights with the reduction dimension contiguous, as camhipMoeExperts takes them: gmm1Weight [numExperts,
  * gmm1HiddenSize, hidden] (rows [0,I) gate, [I,2I) up), gmm2Weight [numExperts, hidden, I]; weightDtype
  * CAMHIP_DTYPE_BF16 (no scales), _INT8 (scales [numExperts, gmm1HiddenSize], [numExperts, hidden]) or _FP8 (128x128
  * block scales [numExperts, n/128, k/128]).  Shared expert (optional): the same for one expert of shareGmm1HiddenSize / 2

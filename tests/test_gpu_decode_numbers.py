@@ -1,0 +1,46 @@
+"""The numbers inside the operators of a decode step: sums whose terms cancel, so that what the operators hold in between
+comes out at the end, unhidden by the output's rounding."""
+import pytest
+import torch
+
+import umdk_amd
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+TYPES = {"bf16": torch.bfloat16, "int8": torch.int8, "fp8": torch.float8_e4m3fn}
+
+
+def one_expert(x, w1, w2, dtype):
+    """moe_decode_layer with one expert, whose gate is 1, of small whole weights, the same in every type."""
+    H, I = x.shape[1], w2.shape[1]
+    cast = lambda w: w.to(torch.float32).to(TYPES[dtype])[None].contiguous().to(DEV)  # noqa: E731
+    ones = lambda n, k: None if dtype == "bf16" else torch.ones(  # noqa: E731
+        (1, n) if dtype == "int8" else (1, n // 128, k // 128), device=DEV)
+    router = torch.zeros(1, H, device=DEV)
+    out, ids, gates = umdk_amd.moe_decode_layer(x.to(DEV), router, None, cast(w1), ones(2 * I, H), cast(w2), ones(H, I), 1)
+    assert (ids == 0).all() and (gates == 1).all()
+    return out.cpu().double()
+
+
+def cancelling_pairs(I, H, pairs):
+    """W1 and W2 by which out[n] = 3 silu(x[2 + n]) x[0] - silu(x[2 + n]) x[1] for n < pairs, 0 for the others."""
+    w1, w2 = torch.zeros(2 * I, H), torch.zeros(H, I)
+    for n in range(pairs):
+        w1[2 * n, 2 + n] = w1[2 * n + 1, 2 + n] = 1
+        w1[I + 2 * n, 0] = w1[I + 2 * n + 1, 1] = 1
+        w2[n, 2 * n], w2[n, 2 * n + 1] = 3, -1
+    return w1, w2
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int8", "fp8"])
+def test_h_reaches_the_second_product_with_all_its_bits(dtype):
+    """With x[0] = 1 and x[1] = 3 every output is 3 s - 3 s = 0.  g and u are exact, s is the same number in both terms, 3 s is
+    rounded once (2^-24 of it); the products' six parts are exact and each addition of theirs loses 2^-23 of 3 s at most, however a
+    matrix instruction rounds: together less than 2^-20 of 3 s.  (With 16 bits of h the terms are up to 2^-18 of 3 s apart.)"""
+    T, H, I, pairs = 5, 256, 128, 64
+    x = torch.randn(T, H, generator=torch.Generator().manual_seed(1)).bfloat16()
+    x[:, 0], x[:, 1] = 1, 3
+    g = x[:, 2:2 + pairs].double()
+    out = one_expert(x, *cancelling_pairs(I, H, pairs), dtype)
+    assert (out[:, :pairs].abs() <= 3 * (torch.sigmoid(g) * g).abs() * 2.0 ** -20).all()
+    assert (out[:, pairs:] == 0).all()

@@ -23,8 +23,9 @@
 //
 // Sums are fp32 in an order that hangs on the shapes alone: a token's results are the same bits in any batch, on any
 // schedule.  Each (token, pick) gets its own row of partial results; whoever adds the last one to a tile of the output sums
-// them up, picks ascending.  h is held as two bf16 numbers, of which the second is what the first leaves out (2^-16 in
-// all): one would add 2^-8 roundings of I values to the result's own, and the matrix instructions for the second are free.
+// them up, picks ascending.  h is held as three bf16 numbers, each the leading bits of what those before it leave out, so that
+// all 24 bits of it go into the second product: one number would add 2^-8 roundings of I values to the result's own, two leave
+// an error ten times that of the fp32 sums, and the matrix instructions for the others are free.
 //
 // Measured: one token on 8 of 64 fp8 experts and a shared one of 7168 x 2048 (398 MB of weights) 92 us, of which 4.5 are the
 // logits, 6 the routing, 4 until the first weights are there and some 10 the blocks' not ending together; 16 such tokens (44 to
@@ -48,8 +49,9 @@ constexpr int MD_WAVES = 8, MD_RING = 7, MD_BLOCKS = 256;
 constexpr int MD_SLOT = 2048;  // bytes of a slot of the ring: 16 rows by 128 bytes
 constexpr int MD_BATCH = 4;    // tiles of a wave between two meetings of the waves
 constexpr int MD_MAX_PICKS = 16, MD_MAX_EXPERTS = 512, MD_MAX_ENTRIES = MD_MAX_TOKENS * MD_MAX_PICKS + 1;
-// The longest run of h that a work item of the second product multiplies by: what 128 registers hold of it (both numbers).
-constexpr int MD_CHUNK = 4096;
+// The longest run of h that a work item of the second product multiplies by: what the waves hold of it in MD_NUMBERS numbers of
+// MD_STEPS matrix instructions each, 144 registers.
+constexpr int MD_NUMBERS = 3, MD_STEPS = 12, MD_CHUNK = MD_WAVES * MD_STEPS * 32;
 // Counters in the workspace, 64 bytes apart: the queue, the experts' h (finished pairs of tiles), the output's tiles.
 constexpr int MD_CTR = 16, MD_CTR_READY = 1, MD_CTR_DONE = MD_CTR_READY + MD_MAX_ENTRIES;
 constexpr int MD_COUNTERS = MD_CTR_DONE + MD_MAX_HIDDEN / 16;
@@ -59,12 +61,12 @@ constexpr int AUX_NT = 2, AUX_AGENT = 16;
 struct Ws {
     int *ctr;
     float *logits;           // [T, E]
-    uint16_t *h, *h_low;     // [T, K + 1, width]
+    uint16_t *h;             // [MD_NUMBERS][T, K + 1, width]
     float *part;             // [T, K + 1, chunks, H]
     uint32_t h_bytes, part_bytes;
 };
 struct Layout {
-    size_t logits, h, h_low, part, total;
+    size_t logits, h, part, total;
     uint32_t h_bytes, part_bytes;
     int width, chunks;
 };
@@ -75,12 +77,11 @@ Layout md_layout(const MoeDecodeArgs &a)
     Layout l;
     l.width = a.I > a.Is ? a.I : a.Is;
     l.chunks = md_chunks(l.width);
-    l.h_bytes = (uint32_t)((size_t)a.T * (a.K + 1) * l.width * 2);
+    l.h_bytes = (uint32_t)((size_t)MD_NUMBERS * a.T * (a.K + 1) * l.width * 2);
     l.part_bytes = (uint32_t)((size_t)a.T * (a.K + 1) * l.chunks * a.H * 4);
     l.logits = up((size_t)MD_COUNTERS * MD_CTR * 4);
     l.h = l.logits + up((size_t)a.T * a.E * 4);
-    l.h_low = l.h + up(l.h_bytes);
-    l.part = l.h_low + up(l.h_bytes);
+    l.part = l.h + up(l.h_bytes);
     l.total = l.part + up(l.part_bytes);
     return l;
 }
@@ -254,7 +255,7 @@ struct Split {
 struct Late {
     const void *w1, *w2, *sw1, *sw2;
     const float *s1, *s2, *ss1, *ss2;
-    uint16_t *out, *h, *h_low;
+    uint16_t *out, *h;
     float *part;
     int *ctr;
     int I, Is, K, width, chunks;
@@ -315,7 +316,7 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
     using W = Weight<WT>;
     constexpr int PIECES = 16 / W::SIZE / 8;               // steps of 16 bytes
     constexpr int U1 = MD_MAX_HIDDEN / W::UNIT / MD_WAVES;  // a wave's units of a row of the first matrix at most
-    constexpr int U2 = MD_CHUNK / W::UNIT / MD_WAVES;       // and of a chunk of the second
+    constexpr int U2 = MD_STEPS / W::STEPS;                 // and of a chunk of the second
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
     Shared &sh = *reinterpret_cast<Shared *>(smem);
     const Late &a = sh.a;
@@ -365,8 +366,8 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
         if (clerk && lane == 0 && T >= MD_WAVES)
             ticket2 = ctr_add(args.ws.ctr, 1);
         if (threadIdx.x == MD_WAVES * 64 - 1)
-            sh.a = Late{p.w1,  p.w2, p.sw1, p.sw2, p.s1, p.s2,       p.ss1,       p.ss2,          p.out,          args.ws.h, args.ws.h_low,
-                        args.ws.part, args.ws.ctr, p.I, p.Is, p.K, args.width, args.chunks, args.ws.h_bytes, args.ws.part_bytes};
+            sh.a = Late{p.w1,         p.w2,        p.sw1, p.sw2, p.s1, p.s2,       p.ss1,       p.ss2,           p.out,             args.ws.h,
+                        args.ws.part, args.ws.ctr, p.I,   p.Is,  p.K,  args.width, args.chunks, args.ws.h_bytes, args.ws.part_bytes};
         __syncthreads();
         if ((int)threadIdx.x < T * K) {
             const int t = threadIdx.x / K, e = sh.ids[t][threadIdx.x % K];
@@ -607,8 +608,9 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
         while (ahead < MD_RING && in.tiles > 0)
             fill();
     };
-    // the next slot's products with x, or with both numbers of h, added to acc; the slot is filled again
-    const auto use = [&](const u32x4 *x, const u32x4 *x_low, float s, bool half, f32x4 &acc) {
+    // the next slot's products with x, or with the numbers of h (step by step), added to acc; the slot is filled again
+    const auto use = [&](const u32x4 *x, auto numbers, float s, bool half, f32x4 &acc) {
+        constexpr int NUMBERS = decltype(numbers)::value;
         wait_slot<MD_RING>(ahead);
         const uint8_t *at = my_ring + out_slot * MD_SLOT;
         u32x4 v[2];
@@ -625,9 +627,9 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
 #pragma unroll
         for (int i = 0; i < W::STEPS; ++i) {
             const bf16x8 b = values<WT>(v[i / PIECES], i % PIECES);
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, __builtin_bit_cast(bf16x8, x[i]), sum, 0, 0, 0);
-            if (x_low)
-                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, __builtin_bit_cast(bf16x8, x_low[i]), sum, 0, 0, 0);
+#pragma unroll
+            for (int k = 0; k < NUMBERS; ++k)
+                sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, __builtin_bit_cast(bf16x8, x[i * NUMBERS + k]), sum, 0, 0, 0);
         }
         if constexpr (WT == MD_FP8) {
 #pragma unroll
@@ -716,7 +718,7 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
                 upto<U1>(units, [&](auto c) {
                     constexpr int u = decltype(c)::value;
-                    use(x + u * W::STEPS, nullptr, WT == MD_FP8 ? s[0][u] : 0.f, (uint32_t)(w + 8 * u) * 128 + 64 >= row1, acc[1]);
+                    use(x + u * W::STEPS, std::integral_constant<int, 1>{}, WT == MD_FP8 ? s[0][u] : 0.f, (uint32_t)(w + 8 * u) * 128 + 64 >= row1, acc[1]);
                 });
                 if constexpr (WT == MD_FP8) {
 #pragma unroll
@@ -746,21 +748,26 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                         u[q] *= cur.s[cur.step + i0 + q];
                     }
                 }
-                f32x4 h, low;
+                f32x4 h;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     h[q] = g[q] / (1.0f + __expf(-g[q])) * u[q];
-                const u32x2 hi = u32x2{f32x2_to_bf16x2(h[0], h[1]), f32x2_to_bf16x2(h[2], h[3])};
+                const bool mine = l16 < T && (sh.entry_mask[cur.entry] >> l16 & 1);
+                const size_t plane = (size_t)T * (a.K + 1) * a.width;
+                uint16_t *to = a.h + (size_t)(mine ? l16 * (a.K + 1) + sh.entry_pick[cur.entry][l16] : 0) * a.width + i0;
+                // (cut off, not rounded: what is left out then has 8 bits less, and nothing is left of 24 bits after three)
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    low[q] = h[q] - bf16_to_f32((hi[q >> 1] >> (16 * (q & 1))) & 0xffffu);
-                const u32x2 lo = u32x2{f32x2_to_bf16x2(low[0], low[1]), f32x2_to_bf16x2(low[2], low[3])};
-                if (l16 < T && (sh.entry_mask[cur.entry] >> l16 & 1)) {
-                    const size_t at = (size_t)(l16 * (a.K + 1) + sh.entry_pick[cur.entry][l16]) * a.width + i0;
-                    __hip_atomic_store(gp(reinterpret_cast<uint64_t *>(a.h + at)), __builtin_bit_cast(uint64_t, hi), __ATOMIC_RELAXED,
-                                       __HIP_MEMORY_SCOPE_AGENT);
-                    __hip_atomic_store(gp(reinterpret_cast<uint64_t *>(a.h_low + at)), __builtin_bit_cast(uint64_t, lo),
-                                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                for (int k = 0; k < MD_NUMBERS; ++k) {
+                    uint32_t v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        v[q] = __float_as_uint(h[q]) & 0xffff0000u;
+                        h[q] -= __uint_as_float(v[q]);
+                    }
+                    if (mine)
+                        __hip_atomic_store(gp(reinterpret_cast<uint64_t *>(to + k * plane)),
+                                           (uint64_t)(v[2] >> 16 | v[3]) << 32 | (v[0] >> 16 | v[1]), __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_AGENT);
                 }
                 wait_loads<0>();
                 if (lane == 0)
@@ -817,14 +824,14 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
             }
         }
         asm volatile("" ::: "memory");
-        u32x4 h[U2 * W::STEPS], low[U2 * W::STEPS];
+        u32x4 h[U2 * W::STEPS * MD_NUMBERS];
         {
-            const rsrc_t rh = rsrc(uniform(a.h), uniform((int)a.h_bytes)), rl = rsrc(uniform(a.h_low), uniform((int)a.h_bytes));
-            const uint32_t row = (uint32_t)((l16 * slots + pick) * a.width);
+            const rsrc_t rh = rsrc(uniform(a.h), uniform((int)a.h_bytes));
+            const uint32_t row = (uint32_t)((l16 * slots + pick) * a.width), plane = uniform((int)a.h_bytes) / MD_NUMBERS;
             const int limit = (int)(cur.row_bytes / W::SIZE);
 #pragma unroll
-            for (int u = 0; u < U2 * W::STEPS; ++u)
-                h[u] = low[u] = u32x4{0, 0, 0, 0};
+            for (int i = 0; i < U2 * W::STEPS * MD_NUMBERS; ++i)
+                h[i] = u32x4{0, 0, 0, 0};
             upto<U2>(units, [&](auto c) {
                 constexpr int u = decltype(c)::value;
                 if (mine) {
@@ -832,8 +839,9 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                     for (int st = 0; st < W::STEPS; ++st) {
                         const int col = (cur.k0 + wk + (u << cur.lkw)) * W::UNIT + (16 / W::SIZE) * (4 * (st / PIECES) + lq) + 8 * (st % PIECES);
                         const uint32_t off = col < limit ? (row + col) * 2 : MD_OUT;
-                        h[u * W::STEPS + st] = __builtin_amdgcn_raw_buffer_load_b128(rh, off, 0, AUX_AGENT);
-                        low[u * W::STEPS + st] = __builtin_amdgcn_raw_buffer_load_b128(rl, off, 0, AUX_AGENT);
+#pragma unroll
+                        for (int k = 0; k < MD_NUMBERS; ++k)
+                            h[(u * W::STEPS + st) * MD_NUMBERS + k] = __builtin_amdgcn_raw_buffer_load_b128(rh, off, k * plane, AUX_AGENT);
                     }
                 }
             });
@@ -857,7 +865,7 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                         scales_of(cur.tile + (w >> cur.lkw) + (j0 + j) * per_tile);
                     upto<U2>(units, [&](auto c) {
                         constexpr int u = decltype(c)::value;
-                        use(h + u * W::STEPS, low + u * W::STEPS, WT == MD_FP8 ? s[u] : 0.f,
+                        use(h + u * W::STEPS * MD_NUMBERS, std::integral_constant<int, MD_NUMBERS>{}, WT == MD_FP8 ? s[u] : 0.f,
                             (uint32_t)(cur.k0 + wk + (u << cur.lkw)) * 128 + 64 >= cur.row_bytes, acc[MD_BATCH - 1]);
                     });
                 }
@@ -965,7 +973,6 @@ hipError_t launch_moe_decode(const MoeDecodeArgs &a, void *ws, hipStream_t s)
     d.ws.ctr = reinterpret_cast<int *>(ws);
     d.ws.logits = reinterpret_cast<float *>((char *)ws + l.logits);
     d.ws.h = reinterpret_cast<uint16_t *>((char *)ws + l.h);
-    d.ws.h_low = reinterpret_cast<uint16_t *>((char *)ws + l.h_low);
     d.ws.part = reinterpret_cast<float *>((char *)ws + l.part);
     d.ws.h_bytes = l.h_bytes;
     d.ws.part_bytes = l.part_bytes;
