@@ -44,3 +44,19 @@ def test_h_reaches_the_second_product_with_all_its_bits(dtype):
     out = one_expert(x, *cancelling_pairs(I, H, pairs), dtype)
     assert (out[:, :pairs].abs() <= 3 * (torch.sigmoid(g) * g).abs() * 2.0 ** -20).all()
     assert (out[:, pairs:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "int8", "fp8"])
+def test_an_infinite_h_stays_infinite(dtype):
+    """h past the range of 32 bits is an infinity, and so are sums of it with weights of one sign."""
+    H, I = 256, 128
+    x = torch.zeros(3, H, dtype=torch.bfloat16)
+    x[:, 0], x[:, 1] = 1e30, torch.tensor([1e30, -1e30, 1e-30])
+    w1, w2 = torch.zeros(2 * I, H), torch.ones(H, I)
+    w1[:I, 0] = w1[I:, 1] = 1
+    w2[1::2] = -1
+    out = one_expert(x, w1, w2, dtype)
+    sign = torch.tensor([1.0, -1.0]).repeat(H // 2)
+    assert torch.equal(out[0], sign * float("inf")) and torch.equal(out[1], -sign * float("inf"))
+    # (1e30 and 1e-30 to 2^-9 each, the sum of 128 products of 1, the output to 2^-8)
+    assert ((out[2] - 128 * sign).abs() <= 128 * (2.0 ** -7 + 2.0 ** -8)).all()

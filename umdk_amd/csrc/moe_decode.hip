@@ -755,14 +755,15 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 const bool mine = l16 < T && (sh.entry_mask[cur.entry] >> l16 & 1);
                 const size_t plane = (size_t)T * (a.K + 1) * a.width;
                 uint16_t *to = a.h + (size_t)(mine ? l16 * (a.K + 1) + sh.entry_pick[cur.entry][l16] : 0) * a.width + i0;
-                // (cut off, not rounded: what is left out then has 8 bits less, and nothing is left of 24 bits after three)
+                // (cut off, not rounded: what is left out then has 8 bits less, and nothing is left of 24 bits after three; nothing is
+                // left of an infinity or a NaN either, where the difference would make a NaN of both)
 #pragma unroll
                 for (int k = 0; k < MD_NUMBERS; ++k) {
                     uint32_t v[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         v[q] = __float_as_uint(h[q]) & 0xffff0000u;
-                        h[q] -= __uint_as_float(v[q]);
+                        h[q] = __builtin_fabsf(h[q]) < INFINITY ? h[q] - __uint_as_float(v[q]) : 0.0f;
                     }
                     if (mine)
                         __hip_atomic_store(gp(reinterpret_cast<uint64_t *>(to + k * plane)),
