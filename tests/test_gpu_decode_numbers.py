@@ -60,3 +60,28 @@ def test_an_infinite_h_stays_infinite(dtype):
     assert torch.equal(out[0], sign * float("inf")) and torch.equal(out[1], -sign * float("inf"))
     # (1e30 and 1e-30 to 2^-9 each, the sum of 128 products of 1, the output to 2^-8)
     assert ((out[2] - 128 * sign).abs() <= 128 * (2.0 ** -7 + 2.0 ** -8)).all()
+
+
+@pytest.mark.parametrize("lo,hi", [(-4, 4), (-30, -4), (-80, -30)])
+def test_silu_far_from_zero(lo, hi):
+    """out[n] = h - 64 v - 64 w with v and w the leading 16 bits of h / 64, exact as products with a gate of 64, whose sigmoid
+    is 1.  The exponential is within 2^-22 of itself, 1 + e and the quotient are rounded once each, u is a power of two, and five
+    additions lose 2^-23 of h each at most: 2^-20 of h, and the output's rounding."""
+    T, H, I, n = 4, 256, 256, 60
+    g = torch.Generator().manual_seed(2)
+    x = torch.zeros(T, H, dtype=torch.bfloat16)
+    x[:, 0], x[:, 1] = 64, 2.0 ** 40
+    x[:, 2:2 + n] = (torch.rand(T, n, generator=g) * (hi - lo) + lo).bfloat16()
+    gate = x[:, 2:2 + n].double()
+    h = torch.sigmoid(gate) * gate * 2.0 ** 40
+    x[:, 2 + n:2 + 2 * n] = (h / 64).bfloat16()
+    x[:, 2 + 2 * n:2 + 3 * n] = (h / 64 - x[:, 2 + n:2 + 2 * n].double()).bfloat16()
+    w1, w2 = torch.zeros(2 * I, H), torch.zeros(H, I)
+    for i in range(n):
+        w1[i, 2 + i] = w1[I + i, 1] = 1
+        for k in (1, 2):
+            w1[k * n + i, 0] = w1[I + k * n + i, 2 + k * n + i] = 1
+        w2[i, i], w2[i, n + i], w2[i, 2 * n + i] = 1, -1, -1
+    want = h - 64 * (x[:, 2 + n:2 + 2 * n].double() + x[:, 2 + 2 * n:2 + 3 * n].double())
+    out = one_expert(x, w1, w2, "bf16")[:, :n]
+    assert ((out - want).abs() <= h.abs() * 2.0 ** -20 + want.abs() * 2.0 ** -8).all()

@@ -751,7 +751,7 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 f32x4 h;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    h[q] = g[q] / (1.0f + __expf(-g[q])) * u[q];
+                    h[q] = g[q] / (1.0f + expf(-g[q])) * u[q];  // (the quick exponential is off by |g| 2^-24)
                 const bool mine = l16 < T && (sh.entry_mask[cur.entry] >> l16 & 1);
                 const size_t plane = (size_t)T * (a.K + 1) * a.width;
                 uint16_t *to = a.h + (size_t)(mine ? l16 * (a.K + 1) + sh.entry_pick[cur.entry][l16] : 0) * a.width + i0;
