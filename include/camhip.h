@@ -431,7 +431,8 @@ CAMHIP_API camhipStatus camhipQuantMatmul(void *workspace, uint64_t workspaceSiz
  * CAMHIP_DTYPE_BF16 (no scales), _INT8 (scales [numExperts, gmm1HiddenSize], [numExperts, hidden]) or _FP8 (128x128
  * block scales [numExperts, n/128, k/128]).  Shared expert (optional): the same for one expert of shareGmm1HiddenSize / 2
  * columns, of the same type.  xActiveMask [numTokens] bool (1 byte) or NULL: a token that is not active gets ids -1,
- * weights 0 and a row of zeros.  Slots without an expert (id -1, see camhipMoeRouteGrouped) add nothing.
+ * weights 0 and a row of zeros.  Slots without an expert (id -1, see camhipMoeRouteGrouped) add nothing; but an active token
+ * that has none because its row holds a NaN, or infinities that cancel in its logits, gets a row of NaN.
  * A token's results are the same bits in any batch.  Limits: numTokens <= 16, hidden <= 8192 and I, the shared one too,
  * <= 32768, multiples of 64 (fp8: 128); numExperts <= 512, topK <= 16; x and the weights 16-byte aligned, one expert's
  * weights below 4 GiB. */

@@ -85,3 +85,34 @@ def test_silu_far_from_zero(lo, hi):
     want = h - 64 * (x[:, 2 + n:2 + 2 * n].double() + x[:, 2 + 2 * n:2 + 3 * n].double())
     out = one_expert(x, w1, w2, "bf16")[:, :n]
     assert ((out - want).abs() <= h.abs() * 2.0 ** -20 + want.abs() * 2.0 ** -8).all()
+
+
+@pytest.mark.parametrize("shared", [False, True])
+@pytest.mark.parametrize("T", [1, 6, 13])
+def test_rows_that_are_not_finite_do_not_come_out_clean(T, shared):
+    """A NaN, or infinities that cancel, leave a token without a logit and so without an expert: its results are NaN, with a shared
+    expert beside the others or without, unless the token is not active; the tokens beside it keep their bits."""
+    g = torch.Generator().manual_seed(3)
+    H, E, I = 512, 16, 128
+    x = torch.randn(T, H, generator=g).bfloat16().to(DEV)
+    router = (torch.randn(E, H, generator=g) * H ** -0.5).to(DEV)
+    router[:, 9] = router[:, 5]
+    w1, w2 = (torch.randn(E, n, k, generator=g).mul_(k ** -0.5).bfloat16().to(DEV) for n, k in ((2 * I, H), (H, I)))
+    kw = dict(share_gmm1_weight=w1[0], share_gmm2_weight=w2[0]) if shared else {}
+    call = lambda x, m: umdk_amd.moe_decode_layer(x, router, None, w1, None, w2, None, 4, x_active_mask=m, **kw)  # noqa: E731
+    want = call(x, None)
+    bad = x.clone()
+    bad[0, 7] = float("nan")
+    bad[T - 1, 500] = float("-nan")
+    if T > 4:
+        bad[2, 5], bad[2, 9] = float("inf"), -float("inf")
+    rows = sorted({0, T - 1} | ({2} if T > 4 else set()))
+    keep = [t for t in range(T) if t not in rows]
+    out, ids, gates = call(bad, None)
+    assert (ids[rows] == -1).all() and (gates[rows] == 0).all() and out[rows].isnan().all()
+    for a, b in zip((out, ids, gates), want):
+        assert torch.equal(a[keep], b[keep])
+    mask = torch.ones(T, dtype=torch.bool, device=DEV)
+    mask[T - 1] = False
+    out, ids, _ = call(bad, mask)
+    assert (out[T - 1] == 0).all() and (T == 1 or out[0].isnan().all()) and torch.equal(out[keep], want[0][keep])

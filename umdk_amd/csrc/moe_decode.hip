@@ -270,6 +270,7 @@ struct Shared {
     int16_t expert_entry[MD_MAX_EXPERTS];
     int16_t ids[MD_MAX_TOKENS][MD_MAX_PICKS];
     float gates[MD_MAX_TOKENS][MD_MAX_PICKS];
+    uint8_t lost[MD_MAX_TOKENS];  // an active token without an expert whose row is not finite: its results are NaN, not empty sums
     int16_t entry_expert[MD_MAX_ENTRIES];
     uint16_t entry_mask[MD_MAX_ENTRIES];
     uint8_t entry_pick[MD_MAX_ENTRIES][MD_MAX_TOKENS];
@@ -362,6 +363,18 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                     p.topk_w[t * K + lane] = g;
                 }
             }
+            bool lost = false;
+            if (uniform(idx) < 0 && (!p.active || p.active[t])) {
+                for (int k = lane * 8; k < H; k += 512) {
+                    const u32x4 v = *reinterpret_cast<const u32x4 *>(p.x + (size_t)t * H + k);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        lost |= (v[q] & 0x7f80u) == 0x7f80u || (v[q] & 0x7f800000u) == 0x7f800000u;
+                }
+                lost = __ballot(lost) != 0;
+            }
+            if (lane == 0)
+                sh.lost[t] = lost;
         }
         if (clerk && lane == 0 && T >= MD_WAVES)
             ticket2 = ctr_add(args.ws.ctr, 1);
@@ -409,7 +422,7 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
         entries = uniform(all);
         if (entries == 0) {  // nobody has an expert
             for (int i = blockIdx.x * MD_WAVES * 64 + threadIdx.x; i < T * H / 4; i += gridDim.x * MD_WAVES * 64)
-                reinterpret_cast<u32x2 *>(p.out)[i] = u32x2{0, 0};
+                reinterpret_cast<u32x2 *>(p.out)[i] = sh.lost[i / (H / 4)] ? u32x2{0x7fc07fc0u, 0x7fc07fc0u} : u32x2{0, 0};
             return;
         }
     }
@@ -908,8 +921,9 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
                 asm volatile("" ::: "memory");
                 for (; last; last &= last - 1) {
                     const int n = (cur.tile + t0 + v0 + MD_WAVES * __builtin_ctzll(last)) * 16 + lq * 4;
-                    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
                     const int t = min(l16, T - 1), routed = (slots - 1) * C0, n_parts = routed + Cs;
+                    const float none = sh.lost[t] ? __builtin_nanf("") : 0.0f;
+                    f32x4 o = f32x4{none, none, none, none};
                     constexpr int AT_ONCE = 8;
 #pragma unroll 1
                     for (int i0 = 0; i0 < n_parts; i0 += AT_ONCE) {  // picks ascending, the shared expert last
