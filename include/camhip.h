@@ -328,13 +328,14 @@ CAMHIP_API camhipStatus camhipMoeExpertsGetWorkspaceSize(const void *x, const fl
 CAMHIP_API camhipStatus camhipMoeExperts(void *workspace, uint64_t workspaceSize, camhipExecutor *executor,
                                          void *stream);
 
-/* Sync status of the current device's chained GEMM launches (camhipMoeExperts, camhipFusedDeepMoe), an
- * extension with no reference counterpart: *status = 0, or nonzero once a readiness wait gave up (sticky;
- * clear != 0 resets it).  A wait only gives up when blocks of its launch cannot run (a GPU shared with other
- * work that holds the compute units); the launch's outputs are then unspecified.  Synchronous: call it after
+/* Sync status of the current device's chained GEMM launches (camhipMoeExperts, camhipFusedDeepMoe; bit 0) and of
+ * camhipMoeDecodeLayer's (bit 1), an extension with no reference counterpart: *status = 0, or nonzero once a
+ * readiness wait gave up (sticky; clear != 0 resets it).  A wait only gives up when blocks of its launch cannot run (a GPU shared with other
+ * work that holds the compute units); the launch's outputs are then unspecified (camhipMoeDecodeLayer's: NaN where
+ * an expert's h was not there).  Synchronous: call it after
  * the launches have completed. */
 CAMHIP_API camhipStatus camhipGetSyncStatus(int32_t *status, int32_t clear);
-/* Test hook (extension): waitTicks > 0 sets the chained launches' wait bound in 100 MHz constant-clock
+/* Test hook (extension): waitTicks > 0 sets these launches' wait bound in 100 MHz constant-clock
  * ticks (<= 0 restores 2 s); unreachable != 0 makes every wait unreachable, so that each one gives up at
  * the bound.  Applies to launches issued after the call, from any thread. */
 CAMHIP_API void camhipDebugSetSyncWait(int64_t waitTicks, int32_t unreachable);
@@ -433,7 +434,9 @@ CAMHIP_API camhipStatus camhipQuantMatmul(void *workspace, uint64_t workspaceSiz
  * columns, of the same type.  xActiveMask [numTokens] bool (1 byte) or NULL: a token that is not active gets ids -1,
  * weights 0 and a row of zeros.  Slots without an expert (id -1, see camhipMoeRouteGrouped) add nothing; but an active token
  * that has none because its row holds a NaN, or infinities that cancel in its logits, gets a row of NaN.
- * A token's results are the same bits in any batch.  Limits: numTokens <= 16, hidden <= 8192 and I, the shared one too,
+ * A token's results are the same bits in any batch.  The second product of an expert waits, bounded, for its first within the
+ * launch; a wait that outlasts its bound (2 s, which only other work that holds the compute units could cause) sets the device's
+ * sync status (camhipGetSyncStatus) and leaves NaN in the rows of the expert's tokens.  Limits: numTokens <= 16, hidden <= 8192 and I, the shared one too,
  * <= 32768, multiples of 64 (fp8: 128); numExperts <= 512, topK <= 16; x and the weights 16-byte aligned, one expert's
  * weights below 4 GiB. */
 CAMHIP_API camhipStatus camhipMoeDecodeLayerGetWorkspaceSize(

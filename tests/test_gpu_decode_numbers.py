@@ -116,3 +116,33 @@ def test_rows_that_are_not_finite_do_not_come_out_clean(T, shared):
     mask[T - 1] = False
     out, ids, _ = call(bad, mask)
     assert (out[T - 1] == 0).all() and (T == 1 or out[0].isnan().all()) and torch.equal(out[keep], want[0][keep])
+
+
+@pytest.mark.parametrize("T,shared", [(1, True), (9, False)])
+def test_a_wait_that_gives_up_says_so(T, shared):
+    """Forced by the host: with every target unreachable and a bound of 20 us each wait gives up, the launch ends normally, its rows
+    are NaN, those of tokens that are not active 0, and the status is set; the next call is itself again."""
+    from umdk_amd import _lib
+    g = torch.Generator().manual_seed(4)
+    H, E, I = 512, 16, 256
+    x = torch.randn(T, H, generator=g).bfloat16().to(DEV)
+    router = torch.randn(E, H, generator=g).to(DEV)
+    w1, w2 = (torch.randn(E, n, k, generator=g).mul_(k ** -0.5).bfloat16().to(DEV) for n, k in ((2 * I, H), (H, I)))
+    kw = dict(share_gmm1_weight=w1[0], share_gmm2_weight=w2[0]) if shared else {}
+    mask = torch.arange(T, device=DEV) != 3
+    call = lambda: umdk_amd.moe_decode_layer(x, router, None, w1, None, w2, None, 4, x_active_mask=mask, **kw)  # noqa: E731
+    _lib.sync_status(clear=True)
+    want = call()
+    assert _lib.sync_status() == 0
+    L = _lib.lib()
+    print("layer, forced give-up", flush=True)
+    L.camhipDebugSetSyncWait(2000, 1)
+    try:
+        out, ids, gates = call()
+        torch.cuda.synchronize()
+    finally:
+        L.camhipDebugSetSyncWait(0, 0)
+    assert _lib.sync_status() == 2 and _lib.sync_status(clear=True) == 2 and _lib.sync_status() == 0
+    assert out[mask].isnan().all() and (out[~mask] == 0).all()
+    assert torch.equal(ids, want[1]) and torch.equal(gates, want[2])
+    assert all(torch.equal(a, b) for a, b in zip(call(), want)) and _lib.sync_status() == 0

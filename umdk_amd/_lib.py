@@ -145,8 +145,8 @@ def launch(name, *args, workspace=None, stream=None, device=None):
 
 
 def sync_status(clear=False):
-    """The current device's sync status of the chained GEMM launches (0: no readiness wait gave up);
-    synchronous, call after the launches have completed."""
+    """The current device's sync status of the chained GEMM launches (bit 0) and of moe_decode_layer (bit 1) (0: no
+    readiness wait gave up); synchronous, call after the launches have completed."""
     L = lib()
     v = ctypes.c_int32(0)
     st = L.camhipGetSyncStatus(ctypes.byref(v), 1 if clear else 0)

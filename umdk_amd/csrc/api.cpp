@@ -701,11 +701,13 @@ camhipStatus camhipMoeExperts(void *workspace, uint64_t workspaceSize, camhipExe
 camhipStatus camhipGetSyncStatus(int32_t *status, int32_t clear)
 {
     CHECK_PTR(status);
-    int v = 0;
-    hipError_t e = cam::sync_status_read(&v, clear != 0);
+    int chained = 0, layer = 0;
+    hipError_t e = cam::sync_status_read(&chained, clear != 0);
+    if (e == hipSuccess)
+        e = cam::moe_decode_sync_status(&layer, clear != 0);
     if (e != hipSuccess)
         return fail(CAMHIP_ERROR_RUNTIME, "get_sync_status: %s", hipGetErrorString(e));
-    *status = v;
+    *status = (chained ? 1 : 0) | (layer ? 2 : 0);
     g_last_error.clear();
     return CAMHIP_SUCCESS;
 }

@@ -56,6 +56,14 @@ hipError_t sync_status_read(int *status, bool clear);
 // Test hooks: the wait bound in constant-clock ticks (<= 0: the default, 2 s) and an unreachable target
 // (every wait gives up at the bound).
 void sync_debug_set(long long wait_ticks, int unreachable);
+// What a launch takes of them: its bound, and what makes its targets unreachable when it is added to them (0 or 1).
+struct SyncWait {
+    long long ticks;
+    int unreachable;
+};
+SyncWait sync_wait();
+// a status word: read, and cleared if it is set and `clear` asks for it
+hipError_t sync_word_read(const void *symbol, int *status, bool clear);
 // fp8 activation scales [M, nb] row-major -> [nb, M] k-major (the layout the GEMMs read: one k-step's
 // scales of consecutive rows are contiguous), rows [0, sum(group_list)) only.
 hipError_t launch_scales_to_kmajor(const float *src, const int64_t *group_list, int L, int M, int nb, float *dst,

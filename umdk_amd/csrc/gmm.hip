@@ -1972,21 +1972,29 @@ void sync_debug_set(long long wait_ticks, int unreachable)
     g_sync_unreach.store(unreachable ? 1 : 0, std::memory_order_relaxed);
 }
 
-hipError_t sync_status_read(int *status, bool clear)
+SyncWait sync_wait()
+{
+    const long long t = g_sync_ticks.load(std::memory_order_relaxed);
+    return {t > 0 ? t : 200000000LL, g_sync_unreach.load(std::memory_order_relaxed)};  // 2 s of the 100 MHz constant clock
+}
+
+hipError_t sync_word_read(const void *symbol, int *status, bool clear)
 {
     int v = 0;
-    hipError_t e = hipMemcpyFromSymbol(&v, HIP_SYMBOL(g_cam_sync_status), sizeof(int), 0, hipMemcpyDeviceToHost);
+    hipError_t e = hipMemcpyFromSymbol(&v, symbol, sizeof(int), 0, hipMemcpyDeviceToHost);
     if (e != hipSuccess)
         return e;
     if (clear && v != 0) {
         const int zero = 0;
-        e = hipMemcpyToSymbol(HIP_SYMBOL(g_cam_sync_status), &zero, sizeof(int), 0, hipMemcpyHostToDevice);
+        e = hipMemcpyToSymbol(symbol, &zero, sizeof(int), 0, hipMemcpyHostToDevice);
         if (e != hipSuccess)
             return e;
     }
     *status = v;
     return hipSuccess;
 }
+
+hipError_t sync_status_read(int *status, bool clear) { return sync_word_read(&g_cam_sync_status, status, clear); }
 
 template <int DT, int EPI1> static hipError_t launch_chain_t(GmmArgs g1, GmmArgs g2, GmmSync sy, hipStream_t s)
 {
@@ -2021,9 +2029,8 @@ hipError_t launch_gmm_chain(const GmmArgs &g1, const GmmArgs &g2, int dt, int *r
         return hipErrorInvalidValue;
     if (!gmm_chain_supported(g1, g2, dt))
         return hipErrorNotSupported;
-    const long long t = g_sync_ticks.load(std::memory_order_relaxed);
-    const GmmSync sy{ready, g1.N / 2 / 128 + g_sync_unreach.load(std::memory_order_relaxed),
-                     t > 0 ? t : 200000000LL};  // 2 s of the 100 MHz constant clock
+    const SyncWait wait = sync_wait();
+    const GmmSync sy{ready, g1.N / 2 / 128 + wait.unreachable, wait.ticks};
     if (dt == DT_FP8)
         return launch_chain_t<DT_FP8, EPI_SWIGLU_FP8>(g1, g2, sy, s);
     return launch_chain_t<DT_BF16, EPI_SWIGLU_BF16>(g1, g2, sy, s);

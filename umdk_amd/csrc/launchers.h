@@ -96,6 +96,8 @@ struct MoeDecodeArgs {
     int G, KG, score, group_top2, renorm, router_fp32, wtype;
     float scaling;
 };
+// The layer's sync status (as gmm.h's): nonzero once a wait for an expert's h has given up.
+hipError_t moe_decode_sync_status(int *status, bool clear);
 size_t moe_decode_workspace_bytes(const MoeDecodeArgs &a);
 hipError_t launch_moe_decode(const MoeDecodeArgs &a, void *ws, hipStream_t s);
 

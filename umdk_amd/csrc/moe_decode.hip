@@ -32,9 +32,11 @@
 // 56 experts, 2.0 to 2.5 GB) 357-390 us, 7.0 TB/s in the first product and 5.4 in the second, whose items' h comes behind
 // their own first weights; 7 tokens on 6 of 160 bf16 experts of 5120 x 1408 (1.67 GB) 277 us; one token on 2 of 8 bf16 experts of
 // 1024 x 512 27 us, all of it latency: two launches, the routing, an expert's h on its way from block to block.
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
+#include "gmm.h"
 #include "route_dev.h"
 
 namespace cam {
@@ -57,6 +59,9 @@ constexpr int MD_CTR = 16, MD_CTR_READY = 1, MD_CTR_DONE = MD_CTR_READY + MD_MAX
 constexpr int MD_COUNTERS = MD_CTR_DONE + MD_MAX_HIDDEN / 16;
 constexpr uint32_t MD_OUT = 0x80000000u;  // an offset past every buffer here: loads give 0, stores nothing
 constexpr int AUX_NT = 2, AUX_AGENT = 16;
+
+// nonzero once a wait for an expert's h has given up (sticky; read and cleared by the host, moe_decode_sync_status)
+__device__ int g_decode_sync_status;
 
 struct Ws {
     int *ctr;
@@ -231,6 +236,8 @@ struct DecodeArgs {
     RouteGroupedArgs r;  // one token's routing by a wave
     int route_per, width, chunks;
     Ws ws;
+    uint32_t wait_ticks;  // the bound of a wait for h
+    int unreachable;      // 1: a test makes every wait give up
 };
 
 // A work item.  phase 1: a pair of 16-row tiles (gate, up) of an entry's first matrix; 2: `count` tiles of a chunk of its
@@ -259,7 +266,8 @@ struct Late {
     float *part;
     int *ctr;
     int I, Is, K, width, chunks;
-    uint32_t h_bytes, part_bytes;
+    uint32_t h_bytes, part_bytes, wait_ticks;
+    int unreachable;
 };
 
 // LDS.  red: what the waves have summed up of their tiles.
@@ -380,7 +388,8 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
             ticket2 = ctr_add(args.ws.ctr, 1);
         if (threadIdx.x == MD_WAVES * 64 - 1)
             sh.a = Late{p.w1,         p.w2,        p.sw1, p.sw2, p.s1, p.s2,       p.ss1,       p.ss2,           p.out,             args.ws.h,
-                        args.ws.part, args.ws.ctr, p.I,   p.Is,  p.K,  args.width, args.chunks, args.ws.h_bytes, args.ws.part_bytes};
+                        args.ws.part, args.ws.ctr, p.I,   p.Is,  p.K,  args.width, args.chunks, args.ws.h_bytes, args.ws.part_bytes,
+                        args.wait_ticks, args.unreachable};
         __syncthreads();
         if ((int)threadIdx.x < T * K) {
             const int t = threadIdx.x / K, e = sh.ids[t][threadIdx.x % K];
@@ -815,17 +824,25 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
         // waits, at this one alone: all blocks' looks at many counters slow down the streams that they wait for.
         if (cur.entry >= known) {
             if (w == 0) {
-                const uint64_t t0 = wall_clock64();
-                const int d = min(cur.entry + lane, entries - 1), want = (nshared && d == 0 ? a.Is : a.I) / 16;
+                uint32_t last = (uint32_t)wall_clock64(), waited = 0;
+                const int d = min(cur.entry + lane, entries - 1), want = (nshared && d == 0 ? a.Is : a.I) / 16 + a.unreachable;
                 int *const counter = a.ctr + (MD_CTR_READY + d) * MD_CTR;
                 const uint64_t not_yet = __ballot(ctr_load(counter) < want);
                 int to = cur.entry + (not_yet ? __builtin_ctzll(not_yet) : 64);
                 while (to == cur.entry) {
                     __builtin_amdgcn_s_sleep(8);
-                    if (wall_clock64() - t0 > 200000000ull)  // 2 s: no launch that has the workspace to itself waits so long
-                        to = -1;
-                    else if (__ballot(lane == 0 && ctr_load(counter) >= want))
+                    if (__ballot(lane == 0 && ctr_load(counter) >= want)) {
                         to = cur.entry + 1;
+                        break;
+                    }
+                    const uint32_t now = (uint32_t)wall_clock64();
+                    waited += min(now - last, 100000u);  // (1 ms: what else passes between two looks, this wave did not run in)
+                    last = now;
+                    if (waited > a.wait_ticks) {
+                        to = -1;
+                        if (lane == 0)
+                            __hip_atomic_fetch_or(gp(&g_decode_sync_status), 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    }
                 }
                 if (lane == 0)
                     sh.known = to;
@@ -974,6 +991,8 @@ template <int WT> hipError_t run(const DecodeArgs &a, hipStream_t s)
 
 }  // namespace
 
+hipError_t moe_decode_sync_status(int *status, bool clear) { return sync_word_read(&g_decode_sync_status, status, clear); }
+
 size_t moe_decode_workspace_bytes(const MoeDecodeArgs &a) { return md_layout(a).total; }
 
 hipError_t launch_moe_decode(const MoeDecodeArgs &a, void *ws, hipStream_t s)
@@ -991,6 +1010,9 @@ hipError_t launch_moe_decode(const MoeDecodeArgs &a, void *ws, hipStream_t s)
     d.ws.part = reinterpret_cast<float *>((char *)ws + l.part);
     d.ws.h_bytes = l.h_bytes;
     d.ws.part_bytes = l.part_bytes;
+    const SyncWait wait = sync_wait();
+    d.wait_ticks = (uint32_t)std::min(wait.ticks, 0x7fffffffll);
+    d.unreachable = wait.unreachable;
     RouteGroupedArgs &r = d.r;
     r.row_bytes = (int64_t)a.E * 4;
     r.bias = a.bias;

@@ -577,7 +577,9 @@ def moe_decode_layer(x, router, bias, gmm1_weight, gmm1_weight_scale, gmm2_weigh
     rows stay in 16 bits whatever the weights' type.  x_active_mask [T] bool:
     tokens that are not active get ids -1, weights 0 and rows of zeros; one
     that is active and has no expert because its row is not finite gets a row
-    of NaN.  A token's results are the same bits in any batch.  No backward: inputs that
+    of NaN (as are rows whose wait for another block's results was given up
+    after 2 s, which sets the device's sync status).  A token's results are
+    the same bits in any batch.  No backward: inputs that
     ask for a gradient are refused in grad mode, those with a forward-mode
     tangent too."""
     out = (_lib._tensor_caller or _lib._tensors()).moe_decode_layer(
