@@ -458,8 +458,8 @@ CAMHIP_API camhipStatus camhipMoeDecodeLayer(void *workspace, uint64_t workspace
  * camhipQuantMatmul; values code * scale).  loraA [numAdapters, rank, k], loraB [numAdapters, n, rank] of loraDtype (bf16
  * or fp16); adapters of a lower rank are padded with zeros.  adapterIds [m] in any order; scaling [numAdapters] fp32 or NULL
  * (ones).  out [m, n] of outDtype (bf16 or fp16), rows contiguous; it may be base itself, where type and stride agree.
- * Products are exact, sums fp32, A x in between is held to 2^-16 of itself (fp16: 2^-21 of the row's largest), one rounding
- * at the end.
+ * Products are exact, sums fp32, A x in between keeps its 32 bits (fp16: 2^-24 of itself, and 2^-35 of the row's largest), one
+ * rounding at the end.
  * Limits: m <= 2^20, n <= 2^20, k a multiple of 16 and at most 131056, rank a multiple of 8 and at most 256, numAdapters
  * <= 65536; loraA, loraB and the rows of x 16-byte aligned. */
 CAMHIP_API camhipStatus camhipLoraAddGetWorkspaceSize(const void *base, const void *x, const float *xScale,

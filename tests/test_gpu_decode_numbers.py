@@ -146,3 +146,23 @@ def test_a_wait_that_gives_up_says_so(T, shared):
     assert out[mask].isnan().all() and (out[~mask] == 0).all()
     assert torch.equal(ids, want[1]) and torch.equal(gates, want[2])
     assert all(torch.equal(a, b) for a, b in zip(call(), want)) and _lib.sync_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,base", [(1, 64, torch.float32), (70, 33, torch.float32), (300, 100, torch.float16),
+                                      (2900, 4232, torch.bfloat16), (8300, 2600, torch.bfloat16)])
+def test_z_reaches_the_second_product_with_all_its_bits(M, N, base, dtype):
+    """Whole numbers: with A's row 9 three times its row 3 out[n] = 3 z - 1 (3 z) = 0, exactly: the magnitudes of no sum on the way
+    come to 2^24 (32 products of up to 255 * 2^7 by up to 3 are below 2^22, the second product's two terms together below 2^23)."""
+    g = torch.Generator().manual_seed(5)
+    K, R, L = 32, 16, 2
+    x = torch.randint(128, 256, (M, K), generator=g) * 2 ** torch.randint(0, 8, (M, K), generator=g)
+    x = (x * (torch.randint(0, 2, (M, K), generator=g) * 2 - 1)).to(dtype).to(DEV)
+    a = torch.zeros(L, R, K, dtype=dtype)
+    a[:, 3] = torch.randint(-1, 2, (L, K), generator=g).to(dtype)
+    a[:, 9] = 3 * a[:, 3]
+    b = torch.zeros(L, N, R, dtype=dtype)
+    b[:, :, 3], b[:, :, 9] = 3, -1
+    ids = (torch.arange(M) % 2).int().to(DEV)
+    out = umdk_amd.lora_add(torch.zeros(M, N, dtype=base, device=DEV), x, a.to(DEV), b.to(DEV), ids)
+    assert not out.any()

@@ -12,8 +12,10 @@
 // rows of 4096 x 4096 6.3 + 9.2; 16384 rows of 4096 x 14336 at rank 64 33.5 (4.1 TB/s) + 196 (4.8 TB/s; B and z, 100 MB of
 // them past L2, included 5.4).  Both in one launch, each block with a z of its own, took longer where it should have helped
 // (one row 8.3 -> 10.8 us, 64 rows 13 -> 20).
-// Matrix instructions take 16 tokens as their columns, rows of A or B as their rows.  z goes into the second product as two
-// 16-bit numbers, the second what the first leaves out, so that it loses 2^-16 (bf16) or, brought to the row's largest first, 2^-21 (fp16).
+// Matrix instructions take 16 tokens as their columns, rows of A or B as their rows.  z goes into the second product as 16-bit
+// numbers, each what those before it leave out, with all the bits of the fp32 sums: three bf16 numbers, or two of fp16, which are
+// within 2^-24 of it (2^-35 of the row's largest, brought to 2^10 first).  (Two bf16 numbers lost 2^-18: 16384 rows of rank 64 230 us,
+// with three 236.)
 #include <atomic>
 #include <type_traits>
 
@@ -409,11 +411,12 @@ template <bool FULL> __device__ __forceinline__ void store8(void *p, int64_t at,
     }
 }
 
-// z of a chunk into LDS as the instructions' second operand: [token fragment][step of 32][first or second number][lane] 16
-// bytes, and each token's factor
+// z of a chunk into LDS as the instructions' second operand: [token fragment][step of 32][number][lane] 16 bytes, and each
+// token's factor
+template <bool BF16> constexpr int NUMBERS = BF16 ? 3 : 2;
 template <bool BF16, int KS, int MF>
 __device__ __forceinline__ void lay_out(const ExpandArgs &p, const Chunks &c, int64_t m0, int members, int adapter,
-                                        u32x4 (&zs)[MF][KS][2][64], float (&factor)[16 * MF])
+                                        u32x4 (&zs)[MF][KS][NUMBERS<BF16>][64], float (&factor)[16 * MF])
 {
     // 4 KS threads a token, 8 values each
     for (int i = threadIdx.x; i < 16 * MF * 4 * KS; i += LR_THREADS) {
@@ -458,14 +461,17 @@ __device__ __forceinline__ void lay_out(const ExpandArgs &p, const Chunks &c, in
                 z[e] = ldexpf(z[e], e2);
             f = ldexpf(f, -e2);
         }
-        u32x4 hi, lo;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            hi[e] = pack2<BF16>(z[2 * e], z[2 * e + 1]);
-            lo[e] = pack2<BF16>(z[2 * e] - unpack<BF16>(hi[e], 0), z[2 * e + 1] - unpack<BF16>(hi[e], 1));
+        for (int k = 0; k < NUMBERS<BF16>; ++k) {
+            u32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = pack2<BF16>(z[2 * e], z[2 * e + 1]);
+                z[2 * e] -= unpack<BF16>(v[e], 0);
+                z[2 * e + 1] -= unpack<BF16>(v[e], 1);
+            }
+            zs[t >> 4][part >> 2][k][(part & 3) * 16 + (t & 15)] = v;
         }
-        zs[t >> 4][part >> 2][0][(part & 3) * 16 + (t & 15)] = hi;
-        zs[t >> 4][part >> 2][1][(part & 3) * 16 + (t & 15)] = lo;
         if (part == 0)
             factor[t] = f;
     }
@@ -502,7 +508,7 @@ template <int KS> __device__ __forceinline__ void clear_past_rank(Tile<KS> &t, i
 }
 // a fragment of 16 tokens' z times a tile of B, scaled, added to v
 template <bool BF16, int KS>
-__device__ __forceinline__ void add_product(const Tile<KS> &b, const u32x4 (&z)[KS][2][64], float scale, int lane, float (&v)[2][8])
+__device__ __forceinline__ void add_product(const Tile<KS> &b, const u32x4 (&z)[KS][NUMBERS<BF16>][64], float scale, int lane, float (&v)[2][8])
 {
     f32x4 acc[4];
 #pragma unroll
@@ -511,7 +517,7 @@ __device__ __forceinline__ void add_product(const Tile<KS> &b, const u32x4 (&z)[
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
+        for (int part = 0; part < NUMBERS<BF16>; ++part) {
             const u32x4 zv = z[s][part][lane];
 #pragma unroll
             for (int f = 0; f < 4; ++f)
@@ -528,7 +534,7 @@ __device__ __forceinline__ void add_product(const Tile<KS> &b, const u32x4 (&z)[
 template <bool BF16, bool WIDE, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) void lora_expand_kernel(const ExpandArgs p)
 {
     __shared__ Chunks c;
-    __shared__ u32x4 zs[MF][KS][2][64];
+    __shared__ u32x4 zs[MF][KS][NUMBERS<BF16>][64];
     __shared__ float factor[16 * MF];
     const int lane = threadIdx.x & 63, l16 = lane & 15, lq = lane >> 4, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int span = 64 * LR_WAVES * p.tiles, n_blocks = (p.N + span - 1) / span;
@@ -626,7 +632,7 @@ template <bool BF16, int KS, int MF> __global__ __launch_bounds__(LR_THREADS) vo
     static_assert(MF == 2 || MF == 4, "units of two fragments");
     constexpr int HALVES = MF / 2;  // units of a tile of 64 columns
     __shared__ Chunks c;
-    __shared__ u32x4 zs[MF][KS][2][64];
+    __shared__ u32x4 zs[MF][KS][NUMBERS<BF16>][64];
     __shared__ float factor[16 * MF];
     extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];  // rings [wave][slot]
     uint8_t *const my_ring = smem + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) * LE_SLOTS * LE_UNIT;
