@@ -166,3 +166,33 @@ def test_z_reaches_the_second_product_with_all_its_bits(M, N, base, dtype):
     ids = (torch.arange(M) % 2).int().to(DEV)
     out = umdk_amd.lora_add(torch.zeros(M, N, dtype=base, device=DEV), x, a.to(DEV), b.to(DEV), ids)
     assert not out.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,N,K", [(5, 64, 48), (40, 72, 208), (300, 100, 64), (2900, 4232, 80), (8300, 2600, 48)])
+def test_an_infinite_z_stays_infinite(M, N, K, dtype):
+    """Products of an infinity with ones are infinite, and so are their sums with finite terms, wherever in the row it stands."""
+    R = 16
+    x = torch.ones(M, K, dtype=dtype)
+    x[0::3, K - 1] = float("inf")
+    x[1::3, 0] = -float("inf")
+    a, b = torch.ones(2, R, K, dtype=dtype), torch.ones(2, N, R, dtype=dtype)
+    a[1] = -1
+    b[:, 1::2] = -1
+    ids = (torch.arange(M) // 7 % 2).int()
+    base = torch.zeros(M, N, dtype=dtype)
+    out = umdk_amd.lora_add(base.to(DEV), x.to(DEV), a.to(DEV), b.to(DEV), ids.to(DEV)).cpu()
+    z = (x.float().sum(1) * (1 - 2 * ids.float()))[:, None] * R
+    assert torch.equal(out.float(), (z * torch.tensor([1.0, -1.0]).repeat(N // 2)).to(dtype).float())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_finite_numbers_beside_an_infinite_z_stay_finite(dtype):
+    """One row of A is infinite: its z is, and the others', far past what fp16 holds, are not."""
+    K, R, N = 32, 16, 40
+    x = torch.full((3, K), 60000.0, dtype=dtype)
+    a, b = torch.full((1, R, K), -30000.0, dtype=dtype), torch.ones(1, N, R, dtype=dtype)
+    a[0, 4, 7] = float("inf")
+    out = umdk_amd.lora_add(torch.zeros(3, N, dtype=dtype, device=DEV), x.to(DEV), a.to(DEV), b.to(DEV),
+                            torch.zeros(3, dtype=torch.int32, device=DEV))
+    assert (out == float("inf")).all()

@@ -301,6 +301,9 @@ __global__ __launch_bounds__(LR_THREADS) void lora_shrink_kernel(const ShrinkArg
 #pragma unroll
                         for (int j = 0; j < NF; ++j)
                             af[j][s] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                        for (int i = 0; i < MF; ++i)
+                            xf[i][s] = u32x4{0, 0, 0, 0};
                     }
             }
 #pragma unroll
@@ -448,27 +451,32 @@ __device__ __forceinline__ void lay_out(const ExpandArgs &p, const Chunks &c, in
         float f = p.scaling ? p.scaling[adapter] : 1.0f;
         if (p.xs)
             f *= p.xs[m];
-        if constexpr (!BF16) {  // the row's largest to 2^10 or a little less: what is left out then keeps its bits
+        if constexpr (!BF16) {  // the row's largest finite one to 2^10 or a little less: what is left out then keeps its bits
             float most = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                most = fmaxf(most, fabsf(z[e]));
+                most = fmaxf(most, fabsf(z[e]) < INFINITY ? fabsf(z[e]) : 0.0f);
             most = KS == 8 ? group_max<32>(most) : KS == 4 ? group_max<16>(most) : KS == 2 ? group_max<8>(most) : group_max<4>(most);
-            const bool plain = most > 0.0f && most < INFINITY;
-            const int e2 = plain ? 10 - ilogbf(most) : 0;
+            const int e2 = most > 0.0f ? 10 - ilogbf(most) : 0;
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 z[e] = ldexpf(z[e], e2);
             f = ldexpf(f, -e2);
         }
+        // (Nothing is left of an infinity or a NaN, where the difference would make a NaN of both.  bf16 numbers are cut off, not
+        // rounded: what is left out then has 8 bits less, and no finite number becomes an infinity.)
 #pragma unroll
         for (int k = 0; k < NUMBERS<BF16>; ++k) {
             u32x4 v;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[e] = pack2<BF16>(z[2 * e], z[2 * e + 1]);
-                z[2 * e] -= unpack<BF16>(v[e], 0);
-                z[2 * e + 1] -= unpack<BF16>(v[e], 1);
+                if constexpr (BF16)
+                    v[e] = __float_as_uint(z[2 * e]) >> 16 | (__float_as_uint(z[2 * e + 1]) & 0xffff0000u);
+                else
+                    v[e] = pack2<BF16>(z[2 * e], z[2 * e + 1]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    z[2 * e + i] = fabsf(z[2 * e + i]) < INFINITY ? z[2 * e + i] - unpack<BF16>(v[e], i) : 0.0f;
             }
             zs[t >> 4][part >> 2][k][(part & 3) * 16 + (t & 15)] = v;
         }
