@@ -8,9 +8,9 @@
 // its own or kept, and no sum hangs on what other tokens are there: a token's bits are the same in any order of a batch of its size.
 //
 // What bounds it: for few tokens the adapters' stream and the latency of two launches, for many the streams of x, base and out.
-// Measured (K x N): one row of 4096 x 4096 at rank 16 3.6 + 4.3 us; 64 int8 rows of 7168 x 4096 with 32 adapters 6.7 + 6.9; 1021
-// rows of 4096 x 4096 6.3 + 9.2; 16384 rows of 4096 x 14336 at rank 64 33.5 (4.1 TB/s) + 196 (4.8 TB/s; B and z, 100 MB of
-// them past L2, included 5.4).  Both in one launch, each block with a z of its own, took longer where it should have helped
+// Measured (K x N): one row of 4096 x 4096 at rank 16 3.5 + 4.4 us; 64 int8 rows of 7168 x 4096 with 32 adapters 6.7 + 7.5; 1021
+// rows of 4096 x 4096 6.3 + 9.4; 16384 rows of 4096 x 14336 at rank 64 33.6 (4.1 TB/s) + 202 (4.6 TB/s; B and z, 100 MB of
+// them past L2, included 5.2).  Both in one launch, each block with a z of its own, took longer where it should have helped
 // (one row 8.3 -> 10.8 us, 64 rows 13 -> 20).
 // Matrix instructions take 16 tokens as their columns, rows of A or B as their rows.  z goes into the second product as 16-bit
 // numbers, each what those before it leave out, with all the bits of the fp32 sums: three bf16 numbers, or two of fp16, which are

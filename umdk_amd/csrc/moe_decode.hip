@@ -27,11 +27,12 @@
 // all 24 bits of it go into the second product: one number would add 2^-8 roundings of I values to the result's own, two leave
 // an error ten times that of the fp32 sums, and the matrix instructions for the others are free.
 //
-// Measured: one token on 8 of 64 fp8 experts and a shared one of 7168 x 2048 (398 MB of weights) 92 us, of which 4.5 are the
+// Measured: one token on 8 of 64 fp8 experts and a shared one of 7168 x 2048 (398 MB of weights) 95 us, of which 4.5 are the
 // logits, 6 the routing, 4 until the first weights are there and some 10 the blocks' not ending together; 16 such tokens (44 to
-// 56 experts, 2.0 to 2.5 GB) 357-390 us, 7.0 TB/s in the first product and 5.4 in the second, whose items' h comes behind
-// their own first weights; 7 tokens on 6 of 160 bf16 experts of 5120 x 1408 (1.67 GB) 277 us; one token on 2 of 8 bf16 experts of
-// 1024 x 512 27 us, all of it latency: two launches, the routing, an expert's h on its way from block to block.
+// 56 experts, 2.0 to 2.5 GB) 383-395 us, 7.0 TB/s in the first product and 5.2 in the second, whose items' h comes behind
+// their own first weights; 7 tokens on 6 of 160 bf16 experts of 5120 x 1408 (1.67 GB) 279 us; one token on 2 of 8 bf16 experts of
+// 1024 x 512 26 us, all of it latency: two launches, the routing, an expert's h on its way from block to block.  (With two numbers
+// of h and a third longer chunks 92, 378 and 275 us.)
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -349,7 +350,8 @@ template <int WT> __global__ __launch_bounds__(MD_WAVES * 64) void moe_decode_ke
     {
         const MoeDecodeArgs &p = args.p;
         const int K = p.K;
-        // ---- routing
+        // ---- routing (picks by reductions, here not by the heads of sorted lists where there are many: 256 experts, 8 picks, one
+        // token 32.2 us in all, by heads 30.6)
         for (int i = threadIdx.x; i < MD_MAX_EXPERTS; i += MD_WAVES * 64)
             sh.expert_mask[i] = 0;
         for (int t = w; t < T; t += MD_WAVES) {
