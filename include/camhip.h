@@ -433,7 +433,7 @@ CAMHIP_API camhipStatus camhipQuantMatmul(void *workspace, uint64_t workspaceSiz
  * block scales [numExperts, n/128, k/128]).  Shared expert (optional): the same for one expert of shareGmm1HiddenSize / 2
  * columns, of the same type.  xActiveMask [numTokens] bool (1 byte) or NULL: a token that is not active gets ids -1,
  * weights 0 and a row of zeros.  Slots without an expert (id -1, see camhipMoeRouteGrouped) add nothing; but an active token
- * that has none because its row holds a NaN, or infinities that cancel in its logits, gets a row of NaN.
+ * that has no expert at all and whose row of x is not finite (a NaN, infinities that cancel in its logits) gets a row of NaN.
  * A token's results are the same bits in any batch.  The second product of an expert waits, bounded, for its first within the
  * launch; a wait that outlasts its bound (2 s, which only other work that holds the compute units could cause) sets the device's
  * sync status (camhipGetSyncStatus) and leaves NaN in the rows of the expert's tokens.  Limits: numTokens <= 16, hidden <= 8192 and I, the shared one too,

@@ -196,3 +196,16 @@ def test_finite_numbers_beside_an_infinite_z_stay_finite(dtype):
     out = umdk_amd.lora_add(torch.zeros(3, N, dtype=dtype, device=DEV), x.to(DEV), a.to(DEV), b.to(DEV),
                             torch.zeros(3, dtype=torch.int32, device=DEV))
     assert (out == float("inf")).all()
+
+
+def test_a_row_whose_logits_are_all_minus_infinity():
+    """No expert, as the routing has it: NaN for a row that is not finite, an empty sum for one whose logits pass 32 bits."""
+    H, E, I = 256, 4, 128
+    x = torch.zeros(3, H, dtype=torch.bfloat16)
+    x[0, 3], x[1, 3], x[2, 3] = float("inf"), 1e38, 1.0
+    router = torch.full((E, H), -1.0)
+    router[:, 3] = -1e30
+    w1, w2 = torch.ones(E, 2 * I, H, dtype=torch.bfloat16), torch.ones(E, H, I, dtype=torch.bfloat16)
+    out, ids, gates = umdk_amd.moe_decode_layer(x.to(DEV), router.to(DEV), None, w1.to(DEV), None, w2.to(DEV), None, 2)
+    assert (ids[:2] == -1).all() and (gates[:2] == 0).all() and (ids[2] >= 0).all()
+    assert out[0].isnan().all() and (out[1] == 0).all() and out[2].isfinite().all()
